@@ -13,6 +13,10 @@
  *     device, memory, streams, events, graphs.
  *  3. The key-switching driver (pcx_*), the launch sequences of crates/pc-gpu (ks.rs, rotate.rs, ntt.rs, keygen.rs)
  *     restated in C++ over the table: a context of one chain, setup-time plans per limb top, key groups, rotations.
+ *
+ * Beside them, the clear side of an encrypted transformer block (pcx_rotary, pcx_qk_norm_rotary, pcx_attention): the
+ * operators that make the plaintext queries and the keys an encrypted scoring starts from, and the attention in the
+ * clear that its decrypted scores are held against. They take no context.
  */
 #ifndef PC_HIP_H
 #define PC_HIP_H
@@ -1082,6 +1086,96 @@ pcx_decryptor* pcx_decryptor_new(pcx_ctx* c, int d, int k_max, int* err);
 void pcx_decryptor_free(pcx_decryptor* x);
 int pcx_decryptor_load_secret(pcx_decryptor* x, const uint32_t* s_rows, int nwhich, pc_stream_t s);
 int pcx_decrypt_rows(pcx_decryptor* x, const void* ct, int K, int top, int which, void* out, pc_stream_t s);
+
+/* ------------------------------------------------------------------------------------------ the clear side */
+/* No counterpart in the reference's kernels: its plain model parts run in its Python front end. These operators work
+ * on heads of floating-point values in device memory, in the launchers' manner: they read *args, enqueue on the stream
+ * and return 0, -1 for NULL or inconsistent arguments, -2 for sizes, strides or alignments outside the kernels' range,
+ * or a positive HIP error; they never allocate, free or synchronise, and may be captured. Arithmetic is in 32 bits,
+ * each output rounded once (to nearest even).
+ *
+ * A tensor [tokens][heads][dim]: element (t, h, d) at base[t token + h head + d], the strides in elements. */
+typedef struct HeadsRef {
+    void* base;
+    int64_t token, head;
+} HeadsRef;
+PC_STATIC_ASSERT(sizeof(HeadsRef) == 24, "HeadsRef layout");
+#define PCX_BF16 0
+#define PCX_F16 1
+#define PCX_F32 2
+
+/* Rotary positions. The pairs i < rot / 2 of each head, (x_a, x_b) at (i, i + rot / 2), or (2 i, 2 i + 1) where
+ * `interleaved`, become (x_a c - x_b s, x_b c + x_a s) with (c, s) = table[positions[t]][i]; `inverse` takes -s (undoes
+ * a rotation). Dimensions from rot on are copied. table: f32 [places][rot / 2][2] (perseus_amd.clear.rotary_table makes
+ * it, scaled for long contexts too); a position outside [0, places) gives NaN in the rotated dimensions. out may be x
+ * itself (the same base and strides); any other overlap is not allowed. rot even, 0 <= rot <= dim <= 512 (rot 0: a
+ * copy; table and positions unread). */
+typedef struct RotaryArgs {
+    HeadsRef x, out;
+    const int32_t* positions; /* [tokens] */
+    const float* table;
+    int64_t places;
+    int32_t tokens, heads, dim, rot;
+    int32_t type, interleaved, inverse, pad;
+} RotaryArgs;
+PC_STATIC_ASSERT(sizeof(RotaryArgs) == 104, "RotaryArgs layout");
+int pcx_rotary(const RotaryArgs* args, pc_stream_t s);
+
+/* The norms of queries and keys with the rotation in the same pass: each head x of q and k becomes x w /
+ * sqrt(mean(x^2) + eps) over its dim values (w: f32 [dim], NULL for ones), then is rotated as by pcx_rotary. v (base
+ * NULL: none) is copied to v_out, so one pass fills a cache: key and value row t goes to row slots[t] of k_out and
+ * v_out (NULL: row t). A slot outside [0, cache_rows) is not written. q_out may be q, k_out may be k where slots is
+ * NULL. heads or kv_heads may be 0 (that tensor unread). */
+typedef struct QkNormRotaryArgs {
+    HeadsRef q, k, v, q_out, k_out, v_out;
+    const float *q_weight, *k_weight;
+    const int32_t* positions;
+    const float* table;
+    const int64_t* slots;
+    int64_t places, cache_rows;
+    int32_t tokens, heads, kv_heads, dim, rot;
+    int32_t type, interleaved;
+    float eps;
+} QkNormRotaryArgs;
+PC_STATIC_ASSERT(sizeof(QkNormRotaryArgs) == 232, "QkNormRotaryArgs layout");
+int pcx_qk_norm_rotary(const QkNormRotaryArgs* args, pc_stream_t s);
+
+/* Attention of packed sequences over keys and values that lie packed or in caches, heads / kv_heads query heads to each
+ * key head (query head h reads key head h kv_heads / heads). Sequence b has the query rows q_start[b] .. q_start[b + 1]
+ * - 1 (n_b of them) and the key rows k_start[b] .. k_start[b] + k_len[b] - 1; its query i sees key j < k_len[b], and
+ * where `causal` only j <= k_len[b] - n_b + i (the last query sees the last key, so a chunk or one token appended to a
+ * cache is the same call). For each query and head
+ *     z_j = scale q . k_j over the keys seen,  lse = log sum_j exp(z_j),  o = sum_j exp(z_j - lse) v_j;
+ * where it sees no key o = 0 and lse = -infinity. lse: f32 [tokens][heads], or NULL. Keys and values that a query does
+ * not see do not reach it, whatever they hold.
+ *
+ * The lengths are device arrays, read by the kernels, so that a captured step follows them; what lies outside the
+ * buffers (query rows from `tokens` on, key rows from kv_rows on) is cut off. Query rows of no sequence are left
+ * unwritten; sequences may not share query rows. max_q and max_k are the longest query run and the longest key run that
+ * the caller expects: they choose kernels and splits and no result depends on them beyond the order of its sums.
+ *
+ * Types bf16 and f16 (q, k, v, out alike); dim a multiple of 8 up to 256; base addresses of 16 bytes and strides of
+ * whole 16-byte groups, key and value rows at most 2^22 elements apart; scale > 0 and finite. work (of work_bytes, 16-byte aligned) holds the partial sums where keys are split
+ * over the chip: pcx_attention_workspace's bytes let the call choose its splits freely, with less it splits less (NULL,
+ * 0: never). One workspace serves one stream at a time. */
+typedef struct AttentionArgs {
+    HeadsRef q, k, v, out;
+    float* lse;
+    const int32_t* q_start; /* [seqs + 1], not falling */
+    const int64_t* k_start; /* [seqs] */
+    const int32_t* k_len;   /* [seqs] */
+    void* work;
+    uint64_t work_bytes;
+    int64_t kv_rows;
+    int32_t tokens, seqs, heads, kv_heads, dim;
+    int32_t type, causal, max_q, max_k;
+    float scale;
+} AttentionArgs;
+PC_STATIC_ASSERT(sizeof(AttentionArgs) == 192, "AttentionArgs layout");
+int pcx_attention(const AttentionArgs* args, pc_stream_t s);
+/* the workspace bytes of the splits that pcx_attention would choose for these arguments (0: none, or arguments it
+ * refuses); work and work_bytes are not read */
+uint64_t pcx_attention_workspace(const AttentionArgs* args);
 
 /* Stage timing, for measurement: while on, the driver records a HIP event pair on the launch stream around each
  * stage it enqueues (0 ModUp INTT, 1 ModUp conversion, 2 ModUp NTT, 3 key dot, 4 ModDown INTT, 5 ModDown conversion,

@@ -130,6 +130,10 @@ _SIGS = {
     "pcx_decryptor_free": (None, [vp]),
     "pcx_decryptor_load_secret": (C.c_int, [vp, u32p, C.c_int, vp]),
     "pcx_decrypt_rows": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp, vp]),
+    "pcx_rotary": (C.c_int, [vp, vp]),
+    "pcx_qk_norm_rotary": (C.c_int, [vp, vp]),
+    "pcx_attention": (C.c_int, [vp, vp]),
+    "pcx_attention_workspace": (C.c_uint64, [vp]),
 }
 for _name, (_res, _args) in _SIGS.items():
     _f = getattr(LIB, _name)

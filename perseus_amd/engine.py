@@ -30,6 +30,14 @@ class Stream:
         self.h = C.c_void_p()
         check(LIB.pc_hip_stream_create(C.byref(self.h)), "stream_create")
 
+    @classmethod
+    def of(cls, handle):
+        """The stream with this HIP handle (0: the default stream), made and destroyed by another library of the
+        process, so that work enqueued here is ordered with that library's."""
+        s = _Borrowed()
+        s.h = C.c_void_p(int(handle))
+        return s
+
     def sync(self):
         check(LIB.pc_hip_stream_sync(self.h), "stream_sync")
 
@@ -41,6 +49,14 @@ class Stream:
         if getattr(self, "h", None):
             LIB.pc_hip_stream_destroy(self.h)
             self.h = None
+
+
+class _Borrowed(Stream):
+    def __init__(self):
+        pass
+
+    def __del__(self):
+        pass
 
 
 class Event:
