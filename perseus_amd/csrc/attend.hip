@@ -1,75 +1,411 @@
 // Attention of packed sequences over keys and values that lie packed or in caches (pcx_attention).
 //
 // For a query q that sees the keys j: z_j = scale q . k_j, m = max z_j, l = sum exp(z_j - m), o = sum exp(z_j - m) v_j / l,
-// lse = m + log l. One pass over the keys holds (m, l, o) and rescales l and o where m grows. Sums, maxima and o are f32.
+// lse = m + log l. One pass over the keys holds (m, l, o) and rescales l and o where m grows.
+//
+// The rows of a tile are the (query, head) pairs of one key head, numbered query * group + head of the group: a tile of rows
+// reads its keys once for the whole group, and one token of a wide group fills a tile as a run of queries does. Everything is
+// transposed so that a lane holds one row: the 32 x 32 products z^T = K q^T leave in lane (c, h) (c = lane mod 32, h =
+// lane / 32) the scores of row c with the keys 8 i + 4 h + j (i, j < 4), so that row statistics are sums inside a lane and
+// one exchange between the two halves, and the probabilities are already the right operand of o^T += V^T p^T if V's keys
+// are taken in that order: the transposing LDS read gives four keys of a column to a lane, which is that order.
 #include "clear.h"
 
 namespace pch {
 namespace clear {
 
-constexpr int BX = 256;
 constexpr int DMAX = 256;
 constexpr int64_t TOKEN_MAX = 1 << 22;  // key rows' distance, in elements: a tile's byte offsets stay in 32 bits
 
-__device__ __forceinline__ float wg_max(float x, float* sh) {
-    for (int m = 32; m; m >>= 1) x = fmaxf(x, __shfl_xor(x, m));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
-    __syncthreads();
-    return x;
-}
-__device__ __forceinline__ float wg_sum(float x, float* sh) {
-    for (int m = 32; m; m >>= 1) x += __shfl_xor(x, m);
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = sh[0] + sh[1] + sh[2] + sh[3];
-    __syncthreads();
-    return x;
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef float v8f __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+#define PCH_LDS __attribute__((address_space(3)))
+
+template <class T>
+struct Mat;
+template <>
+struct Mat<bf16> {
+    typedef bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef bf16 v4 __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ v16f mul(v8 a, v8 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mat<f16> {
+    typedef f16 v8 __attribute__((ext_vector_type(8)));
+    typedef f16 v4 __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ v16f mul(v8 a, v8 b, v16f c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// the other half's value of a lane's row
+__device__ __forceinline__ float other(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    // r[0]: the low half's value in both halves, r[1]: the high half's
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// a workgroup per query and head, a thread per key of each 256, then a thread per output dimension
-template <class T>
-__global__ void __launch_bounds__(BX) attend_k(AttentionArgs A) {
-    __shared__ float q[DMAX], p[BX], sh[4];
-    const int t = blockIdx.x, h = blockIdx.y, i = threadIdx.x;
-    int b = 0;  // the sequence of row t: the last whose start is not above it
-    for (int lo = 0, hi = A.seqs; lo < hi;) {
-        const int mid = (lo + hi) >> 1;
-        if (A.q_start[mid + 1] > t) hi = mid, b = mid;
-        else lo = mid + 1, b = lo;
-    }
-    if (b >= A.seqs || A.q_start[b] > t) return;
-    const int q0 = max(A.q_start[b], 0), n = min(A.q_start[b + 1], A.tokens) - q0;
-    int64_t k0 = A.k_start[b], len = A.k_len[b];
-    if (k0 < 0 || k0 > A.kv_rows) k0 = len = 0;
-    len = max((int64_t)0, min(len, A.kv_rows - k0));
-    const int kh = h / (A.heads / A.kv_heads);
-    const int64_t seen = A.causal ? min(len, max((int64_t)0, len - n + (t - q0) + 1)) : len;
-    if (i < A.dim) q[i] = (float)at<T>(A.q, t, h)[i] * A.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0, o = 0;
-    for (int64_t j0 = 0; j0 < seen; j0 += BX) {
-        float z = -INFINITY;
-        if (j0 + i < seen) {
-            const T* k = at<T>(A.k, k0 + j0 + i, kh);
-            z = 0;
-            for (int d = 0; d < A.dim; ++d) z = fmaf(q[d], (float)k[d], z);
+// ------------------------------------------------------------------------------------------------ tiles of keys
+// KT rows of DP values in LDS, 16-byte chunks permuted within a row so that both readings are free of bank conflicts: keys
+// (32 lanes take one chunk of 32 rows) by xor with the row number, values (the transposing read takes 32 bytes of 8 rows) by
+// xor with twice the row number.
+template <int DP>
+struct Tile {
+    static constexpr int CPR = DP / 8;  // chunks of a row
+    static __device__ __forceinline__ int kswz(int key) { return DP == 64 ? (key >> 1) & 7 : key & 15; }
+    static __device__ __forceinline__ int vswz(int key) { return DP == 64 ? 2 * ((key >> 1) & 3) : 2 * (key & 7); }
+};
+
+// 64 lanes' 16 bytes each from a buffer into LDS at `lds` + 16 lane; lanes past the buffer's end write zeros. It counts
+// in vmcnt like a load; nothing waits for it but the caller's own s_waitcnt.
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t off) {
+    asm volatile(
+        "s_mov_b32 m0, %0\n\t"
+        "s_nop 0\n\t"
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
+        : "s"(lds), "v"(off), "s"(r)
+        : "memory");
+}
+
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return ((uint64_t)hi << 32) | lo;
+}
+
+// rows of one (sequence, key head): what a workgroup works on
+struct Work {
+    int q0, n;          // query rows of the sequence
+    int64_t k0;         // its first key row
+    int len;            // its keys
+    int tile;           // tile of rows
+    bool live;
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
+
+// item -> (sequence, tile of BM rows), the sequences' tiles one after the other, each sequence's last (longest, where
+// causal) first. Every wave finds it by itself: a prefix sum over the lanes, 64 sequences at a time.
+__device__ __forceinline__ Work locate(const AttentionArgs& A, int item, int group, int BM) {
+    const int lane = threadIdx.x & 63;
+    Work w;
+    w.live = false;
+    for (int base = 0; base < A.seqs; base += 64) {
+        const int b = base + lane;
+        int q0 = 0, n = 0, len = 0;
+        int64_t k0 = 0;
+        if (b < A.seqs) {
+            q0 = clampi(A.q_start[b], 0, A.tokens);
+            n = clampi(A.q_start[b + 1], 0, A.tokens) - q0;
+            n = n < 0 ? 0 : n;
+            k0 = A.k_start[b];
+            len = A.k_len[b];
+            if (k0 < 0 || k0 >= A.kv_rows) k0 = len = 0;
+            if (len < 0) len = 0;
+            if (len > A.kv_rows - k0) len = (int)(A.kv_rows - k0);
         }
-        const float mn = fmaxf(m, wg_max(z, sh));
-        const float e = j0 + i < seen ? expf(z - mn) : 0.0f, r = m == mn ? 1.0f : expf(m - mn);
-        p[i] = e;
-        l = l * r + wg_sum(e, sh);
-        m = mn;
-        if (i < A.dim) {
-            o *= r;
-            const int c = (int)min((int64_t)BX, seen - j0);
-            for (int j = 0; j < c; ++j) o = fmaf(p[j], (float)at<T>(A.v, k0 + j0 + j, kh)[i], o);
+        const int nt = (int)(((int64_t)n * group + BM - 1) / BM);
+        int sum = nt;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int v = __shfl_up(sum, m);
+            if (lane >= m) sum += v;
         }
-        __syncthreads();
+        const uint64_t past = __ballot(sum > item);
+        if (past) {
+            const int src = __builtin_ctzll(past);
+            w.q0 = __builtin_amdgcn_readlane(q0, src);
+            w.n = __builtin_amdgcn_readlane(n, src);
+            w.len = __builtin_amdgcn_readlane(len, src);
+            const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)k0, src);
+            const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)k0 >> 32), src);
+            w.k0 = (int64_t)(((uint64_t)hi << 32) | lo);
+            w.tile = __builtin_amdgcn_readlane(sum, src) - 1 - item;
+            w.live = true;
+            return w;
+        }
+        item -= __builtin_amdgcn_readlane(sum, 63);
     }
-    if (i < A.dim) at<T>(A.out, t, h)[i] = (T)(seen > 0 ? o / l : 0.0f);
-    if (i == 0 && A.lse) A.lse[(int64_t)t * A.heads + h] = seen > 0 ? m + logf(l) : -INFINITY;
+    return w;
+}
+
+// the keys that row r of the sequence sees (the last row's where r is past it, so that unused rows need no masks)
+__device__ __forceinline__ int seen(const Work& w, int r, int group, int causal) {
+    if (!causal) return w.len;
+    int i = r / group;
+    i = i < w.n ? i : w.n - 1;
+    return clampi(w.len - w.n + i + 1, 0, w.len);
+}
+
+// ------------------------------------------------------------------------------------------------ a wave's rows
+// 32 rows of a wave: queries, running statistics and o^T (lane (c, h): row c, dimensions 32 db + 8 i + 4 h + j)
+template <class T, int DP>
+struct Rows {
+    typename Mat<T>::v8 q[DP / 16];
+    v16f o[DP / 32];
+    float m, nm, l;  // running maximum (log2 units), its negative (0 where there is none yet), this half's sum
+    int lim;         // keys seen
+
+    __device__ __forceinline__ void begin(const AttentionArgs& A, const Work& w, int kvh, int group, int r0) {
+        const int lane = threadIdx.x & 63, r = r0 + (lane & 31), h = lane >> 5;
+        const int i = r / group, hd = kvh * group + (r - i * group);
+        const bool live = i < w.n;
+        const T* x = at<T>(A.q, w.q0 + (live ? i : 0), live ? hd : 0);
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            const int d = 16 * s + 8 * h;
+            q[s] = live && d < A.dim ? *(const typename Mat<T>::v8*)(x + d) : (typename Mat<T>::v8)(T)0.0f;
+        }
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) o[d] = (v16f)0.0f;
+        m = -INFINITY;
+        nm = 0;
+        l = 0;
+        lim = seen(w, r, group, A.causal);
+    }
+};
+
+template <class T, int DP, int KT>
+struct Wave {
+    typedef typename Mat<T>::v8 v8;
+    static constexpr int NK = KT / 32;
+    using L = Tile<DP>;
+
+    // scores of KT keys: z[kb] for the keys 32 kb ..
+    static __device__ __forceinline__ void scores(const char PCH_LDS* k, const Rows<T, DP>& R, v16f (&z)[NK]) {
+        const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+        const uint32_t row = c * DP * 2;
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb) z[kb] = (v16f)0.0f;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb) {
+                const v8 a = *(const v8 PCH_LDS*)(k + row + kb * 32 * DP * 2 + (((2 * s + h) ^ L::kswz(c)) << 4));
+                z[kb] = Mat<T>::mul(a, R.q[s], z[kb]);
+            }
+        }
+    }
+
+    // keys from the row's limit on do not count; key0: the tile's first
+    static __device__ __forceinline__ void mask(const Rows<T, DP>& R, int key0, v16f (&z)[NK]) {
+        const int left = R.lim - key0 - 4 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (32 * kb + 8 * (e >> 2) + (e & 3) >= left) z[kb][e] = -INFINITY;
+    }
+
+    // z becomes exp2(c z - m); m follows the largest score where it has grown by more than 8 (2^8 holds in every type, and
+    // most tiles then need no rescaling)
+    static __device__ __forceinline__ void softmax(Rows<T, DP>& R, float c, v16f (&z)[NK]) {
+        float top = z[0][0];
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, z[kb][e]);
+        top = fmaxf(top, other(top)) * c;
+        if (__any(top > R.m + 8.0f)) {
+            const float mn = fmaxf(R.m, top);
+            const float r = mn == R.m ? 1.0f : __builtin_amdgcn_exp2f(R.m - mn);
+            R.m = mn;
+            R.nm = mn == -INFINITY ? 0.0f : -mn;
+            R.l *= r;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) R.o[d] *= r;
+        }
+        float l = 0;
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                z[kb][e] = __builtin_amdgcn_exp2f(fmaf(z[kb][e], c, R.nm));
+                l += z[kb][e];
+            }
+        R.l += l;
+    }
+
+    // o += p V
+    static __device__ __forceinline__ void values(const char PCH_LDS* v, Rows<T, DP>& R, const v16f (&z)[NK]) {
+        const int lane = threadIdx.x & 63;
+        const int key = 4 * (lane >> 5) + ((lane & 15) >> 2), ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+        const uint32_t at = key * DP * 2 + (lane & 1) * 8;
+#pragma unroll
+        for (int s = 0; s < KT / 16; ++s) {
+            v8f pf;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pf[e] = z[s >> 1][8 * (s & 1) + e];
+            const v8 p = __builtin_convertvector(pf, v8);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) {
+                // the swizzle of rows 8 apart is the same
+                const uint32_t x = at + (((4 * d + ch) ^ L::vswz(key)) << 4) + 16 * s * DP * 2;
+                const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s PCH_LDS*)(v + x));
+                const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s PCH_LDS*)(v + x + 8 * DP * 2));
+                const v8s a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                R.o[d] = Mat<T>::mul(__builtin_bit_cast(v8, a), p, R.o[d]);
+            }
+        }
+    }
+
+    // The rare repair of the tiles that a row sees in part. There o^T += V^T p^T multiplies values that a row does not see by
+    // zero, which is not zero where they are infinite or NaN. If o came out so, o of these keys (from key0 to each row's
+    // limit: at most a tile of rows and one of keys) is summed again from memory, key by key, each row its own.
+    static __device__ __forceinline__ void repair(const AttentionArgs& A, const Work& w, int kvh, float c, int key0, int key1,
+                                               int step, Rows<T, DP>& R) {
+        const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) R.o[d] = (v16f)0.0f;
+        for (int t0 = key0; t0 < key1; t0 += step)
+            for (int j = t0; j < t0 + KT && j < key1; ++j) {
+                const T* k = at<T>(A.k, w.k0 + j, kvh);
+                const T* v = at<T>(A.v, w.k0 + j, kvh);
+                float z = 0;
+#pragma unroll
+                for (int s = 0; s < DP / 16; ++s) {
+                    if (16 * s + 8 * h < A.dim) {
+                        const v8 x = *(const v8*)(k + 16 * s + 8 * h);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) z = fmaf((float)x[e], (float)R.q[s][e], z);
+                    }
+                }
+                z += other(z);
+                if (j >= R.lim) continue;
+                const float p = (float)(T)__builtin_amdgcn_exp2f(fmaf(z, c, R.nm));
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int dd = 32 * d + 8 * i + 4 * h;
+                        if (dd < A.dim) {
+                            const typename Mat<T>::v4 x = *(const typename Mat<T>::v4*)(v + dd);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) R.o[d][4 * i + e] = fmaf(p, (float)x[e], R.o[d][4 * i + e]);
+                        }
+                    }
+            }
+    }
+    static __device__ __forceinline__ bool broken(const Rows<T, DP>& R) {
+        float x = 0;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x = fmaf(R.o[d][e], 0.0f, x);
+        return __any(!(x == 0.0f));
+    }
+
+    // o / l and lse, or (split) o, m, l of this part
+    static __device__ __forceinline__ void finish(const AttentionArgs& A, const Work& w, int kvh, int group, int r0,
+                                                  Rows<T, DP>& R) {
+        const int lane = threadIdx.x & 63, r = r0 + (lane & 31), h = lane >> 5;
+        const int i = r / group, hd = kvh * group + (r - i * group);
+        if (i >= w.n) return;
+        const float l = R.l + other(R.l);
+        const float inv = R.m == -INFINITY ? 0.0f : 1.0f / l;
+        T* y = at<T>(A.out, w.q0 + i, hd);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int dd = 32 * d + 8 * g + 4 * h;
+                if (dd < A.dim) {
+                    v4f f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = R.o[d][4 * g + e] * inv;
+                    *(typename Mat<T>::v4*)(y + dd) = __builtin_convertvector(f, typename Mat<T>::v4);
+                }
+            }
+        if (A.lse && h == 0)
+            A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = R.m == -INFINITY ? -INFINITY : (R.m + __log2f(l)) * 0.6931471805599453f;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ many rows
+// A workgroup of NW waves takes NW QB 32 rows; a tile of keys and values goes through LDS once for all of them, the next one
+// loaded while this one is used. Tiles run from the last to the first: those that rows see in part come first.
+template <class T, int DP, int QB, int NW>
+__global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, int group) {
+    constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * QB * NW, TB = KT * DP * 2, CPR = DP / 8;
+    constexpr int NL = KT * CPR / (64 * NW);  // loads a wave issues for a tile
+    using W = Wave<T, DP, KT>;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int kvh = blockIdx.x % A.kv_heads;
+    const Work w = locate(A, blockIdx.x / A.kv_heads, group, BM);
+    if (!w.live) return;
+    const int R = w.n * group, r0 = w.tile * BM, mine = r0 + wave * QB * 32;
+    const float c = A.scale * 1.4426950408889634f;
+    const int last = r0 + BM < R ? r0 + BM : R;
+    const int tiles = (seen(w, last - 1, group, A.causal) + KT - 1) / KT;
+    Rows<T, DP> rows[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) rows[b].begin(A, w, kvh, group, mine + 32 * b);
+    // this wave's part: keys [0, hi) of which [0, lo) are seen by all its rows
+    const int hi = mine < R ? seen(w, mine + QB * 32 - 1, group, A.causal) : 0;
+    const int lo = mine < R ? seen(w, mine, group, A.causal) : 0;
+    const int whole = lo / KT;  // the tiles below this one need no mask
+
+    uint32_t ko[NL], vo[NL];
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+        const int p = (n * NW + wave) * 64 + lane, key = p / CPR, cp = p % CPR;
+        const int ck = cp ^ Tile<DP>::kswz(key), cv = cp ^ Tile<DP>::vswz(key);
+        ko[n] = ck * 8 < A.dim ? key * (uint32_t)A.k.token * 2 + ck * 16 : 0x7ffffff0u;
+        vo[n] = cv * 8 < A.dim ? key * (uint32_t)A.v.token * 2 + cv * 16 : 0x7ffffff0u;
+    }
+    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds;
+    const char* kp = (const char*)uniform64((uint64_t)at<T>(A.k, w.k0, kvh));
+    const char* vp = (const char*)uniform64((uint64_t)at<T>(A.v, w.k0, kvh));
+    auto load = [&](int t) {
+        const int left = w.len - t * KT, nr = (left < KT ? left : KT) - 1;
+        const uint32_t to = base + (t & 1) * 2 * TB + wave * 1024;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)t * KT * A.k.token * 2), 0,
+                                                          (nr * (int)A.k.token + A.dim) * 2, 0x00020000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + (int64_t)t * KT * A.v.token * 2), 0,
+                                                          (nr * (int)A.v.token + A.dim) * 2, 0x00020000);
+#pragma unroll
+        for (int n = 0; n < NL; ++n) load_lds(rk, to + n * NW * 1024, ko[n]);
+#pragma unroll
+        for (int n = 0; n < NL; ++n) load_lds(rv, to + TB + n * NW * 1024, vo[n]);
+    };
+    bool checked = hi <= whole * KT;
+    if (tiles) load(tiles - 1);
+    for (int t = tiles - 1; t >= 0; --t) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (t) load(t - 1);
+        if (t * KT >= hi) continue;
+        const char PCH_LDS* kl = (const char PCH_LDS*)lds + (t & 1) * 2 * TB;
+        if (!checked && t < whole) {
+            checked = true;
+            if (A.causal)
+#pragma unroll
+                for (int b = 0; b < QB; ++b)
+                    if (W::broken(rows[b])) W::repair(A, w, kvh, c, whole * KT, hi, KT, rows[b]);
+        }
+        v16f z[QB][KT / 32];
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            W::scores(kl, rows[b], z[b]);
+            if (t >= whole) W::mask(rows[b], t * KT, z[b]);
+            W::softmax(rows[b], c, z[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < QB; ++b) W::values(kl + TB, rows[b], z[b]);
+    }
+    if (!checked && A.causal)
+#pragma unroll
+        for (int b = 0; b < QB; ++b)
+            if (W::broken(rows[b])) W::repair(A, w, kvh, c, whole * KT, hi, KT, rows[b]);
+#pragma unroll
+    for (int b = 0; b < QB; ++b) W::finish(A, w, kvh, group, mine + 32 * b, rows[b]);
 }
 
 // 0, or the error
@@ -89,8 +425,25 @@ static int checked(const AttentionArgs* a) {
         if ((uintptr_t)r->base % 16 || r->token % 8 || r->head % 8) return -2;
     if (!apart(a->out, a->tokens, a->heads, a->dim)) return -2;
     if (a->k.token > TOKEN_MAX || a->v.token > TOKEN_MAX) return -2;
+    if ((int64_t)a->tokens * a->heads > 0x7fffffff) return -2;
     if ((uintptr_t)a->work % 16) return -2;
     return 0;
+}
+
+template <class T, int DP, int QB, int NW>
+static int rows_run(const AttentionArgs& a, hipStream_t s) {
+    const int group = a.heads / a.kv_heads;
+    const int64_t items = (int64_t)a.tokens * group / (32 * QB * NW) + a.seqs;
+    if (items * a.kv_heads > 0x7fffffff) return -2;
+    hipLaunchKernelGGL((rows_k<T, DP, QB, NW>), dim3((unsigned)(items * a.kv_heads)), dim3(64 * NW), 0, s, a, group);
+    return launch_rc();
+}
+
+template <class T>
+static int run_t(const AttentionArgs& a, hipStream_t s) {
+    if (a.dim <= 64) return rows_run<T, 64, 1, 4>(a, s);
+    if (a.dim <= 128) return rows_run<T, 128, 1, 4>(a, s);
+    return rows_run<T, 256, 1, 4>(a, s);
 }
 
 }  // namespace clear
@@ -107,9 +460,5 @@ extern "C" uint64_t pcx_attention_workspace(const AttentionArgs* a) {
 extern "C" int pcx_attention(const AttentionArgs* a, pc_stream_t s) {
     if (int e = checked(a)) return e;
     if (!a->tokens || !a->seqs || !a->heads) return 0;
-    if (a->type == PCX_BF16)
-        hipLaunchKernelGGL(attend_k<bf16>, dim3(a->tokens, a->heads), dim3(BX), 0, (hipStream_t)s, *a);
-    else
-        hipLaunchKernelGGL(attend_k<f16>, dim3(a->tokens, a->heads), dim3(BX), 0, (hipStream_t)s, *a);
-    return launch_rc();
+    return a->type == PCX_BF16 ? run_t<bf16>(*a, (hipStream_t)s) : run_t<f16>(*a, (hipStream_t)s);
 }
