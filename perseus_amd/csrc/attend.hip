@@ -9,6 +9,8 @@
 // lane / 32) the scores of row c with the keys 8 i + 4 h + j (i, j < 4), so that row statistics are sums inside a lane and
 // one exchange between the two halves, and the probabilities are already the right operand of o^T += V^T p^T if V's keys
 // are taken in that order: the transposing LDS read gives four keys of a column to a lane, which is that order.
+#include <algorithm>
+
 #include "clear.h"
 
 namespace pch {
@@ -82,18 +84,38 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
 
 // rows of one (sequence, key head): what a workgroup works on
 struct Work {
-    int q0, n;          // query rows of the sequence
-    int64_t k0;         // its first key row
-    int len;            // its keys
-    int tile;           // tile of rows
+    int q0, n;       // query rows of the sequence
+    int64_t k0;      // its first key row
+    int len;         // its keys
+    int tile;        // tile of rows
+    int chunk, nc;   // part of the tile's keys, and how many parts they are split into
+    int slot;        // where the tile's partial sums begin
     bool live;
+};
+
+// How a launch splits keys: a sequence of len keys into ceil(len / size) parts, most at the most. Lengths beyond what the
+// caller expected only make the parts longer.
+struct Split {
+    int most, size;
+    float* work;  // [slot][BM][dim] sums, then [slot][BM][2] maxima and weights' sums
+    int64_t slots;
+    __device__ __forceinline__ int parts(int len) const {
+        if (most <= 1) return 1;
+        const int n = (int)(((int64_t)len + size - 1) / size);
+        return n < 1 ? 1 : n < most ? n : most;
+    }
+    __device__ __forceinline__ float* sums(int slot, int BM, int dim) const { return work + (int64_t)slot * BM * dim; }
+    __device__ __forceinline__ float* stats(int slot, int BM, int dim) const {
+        return work + slots * BM * dim + (int64_t)slot * BM * 2;
+    }
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// item -> (sequence, tile of BM rows), the sequences' tiles one after the other, each sequence's last (longest, where
-// causal) first. Every wave finds it by itself: a prefix sum over the lanes, 64 sequences at a time.
-__device__ __forceinline__ Work locate(const AttentionArgs& A, int item, int group, int BM) {
+// item -> (sequence, tile of BM rows, part of its keys), the sequences' tiles one after the other, each sequence's last
+// (longest, where causal) first; split false: all parts of a tile in one item. Every wave finds it by itself: a prefix sum
+// over the lanes, 64 sequences at a time.
+__device__ __forceinline__ Work locate(const AttentionArgs& A, const Split& S, int item, int group, int BM, bool split) {
     const int lane = threadIdx.x & 63;
     Work w;
     w.live = false;
@@ -111,7 +133,7 @@ __device__ __forceinline__ Work locate(const AttentionArgs& A, int item, int gro
             if (len < 0) len = 0;
             if (len > A.kv_rows - k0) len = (int)(A.kv_rows - k0);
         }
-        const int nt = (int)(((int64_t)n * group + BM - 1) / BM);
+        const int parts = S.parts(len), nt = (int)(((int64_t)n * group + BM - 1) / BM) * (split ? parts : 1);
         int sum = nt;
 #pragma unroll
         for (int m = 1; m < 64; m <<= 1) {
@@ -127,7 +149,12 @@ __device__ __forceinline__ Work locate(const AttentionArgs& A, int item, int gro
             const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)k0, src);
             const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)k0 >> 32), src);
             w.k0 = (int64_t)(((uint64_t)hi << 32) | lo);
-            w.tile = __builtin_amdgcn_readlane(sum, src) - 1 - item;
+            w.nc = __builtin_amdgcn_readlane(parts, src);
+            const int from_end = __builtin_amdgcn_readlane(sum, src) - 1 - item;
+            w.tile = split ? from_end / w.nc : from_end;
+            w.chunk = split ? from_end - w.tile * w.nc : 0;
+            // tiles of different sequences apart: a sequence has at most one tile more than its rows divided by BM
+            w.slot = ((int)((int64_t)w.q0 * group / BM) + base + src + w.tile) * S.most;
             w.live = true;
             return w;
         }
@@ -302,13 +329,27 @@ struct Wave {
         return __any(!(x == 0.0f));
     }
 
-    // o / l and lse, or (split) o, m, l of this part
-    static __device__ __forceinline__ void finish(const AttentionArgs& A, const Work& w, int kvh, int group, int r0,
-                                                  Rows<T, DP>& R) {
-        const int lane = threadIdx.x & 63, r = r0 + (lane & 31), h = lane >> 5;
+    // o / l and lse, or (a part of the keys) o, m and l; BM: rows of the tile, row: this lane's in it
+    static __device__ __forceinline__ void finish(const AttentionArgs& A, const Split& S, const Work& w, int kvh, int group,
+                                                  int BM, int row, Rows<T, DP>& R) {
+        const int lane = threadIdx.x & 63, r = w.tile * BM + row, h = lane >> 5;
         const int i = r / group, hd = kvh * group + (r - i * group);
         if (i >= w.n) return;
         const float l = R.l + other(R.l);
+        if (w.nc > 1) {
+            const int slot = (w.slot + w.chunk) * A.kv_heads + kvh;
+            float* y = S.sums(slot, BM, A.dim) + (int64_t)row * A.dim;
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int dd = 32 * d + 8 * g + 4 * h;
+                    if (dd < A.dim)
+                        *(v4f*)(y + dd) = v4f{R.o[d][4 * g], R.o[d][4 * g + 1], R.o[d][4 * g + 2], R.o[d][4 * g + 3]};
+                }
+            if (h == 0) *(float2*)(S.stats(slot, BM, A.dim) + row * 2) = make_float2(R.m, l);
+            return;
+        }
         const float inv = R.m == -INFINITY ? 0.0f : 1.0f / l;
         T* y = at<T>(A.out, w.q0 + i, hd);
 #pragma unroll
@@ -332,26 +373,28 @@ struct Wave {
 // A workgroup of NW waves takes NW QB 32 rows; a tile of keys and values goes through LDS once for all of them, the next one
 // loaded while this one is used. Tiles run from the last to the first: those that rows see in part come first.
 template <class T, int DP, int QB, int NW>
-__global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, int group) {
+__global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, Split S, int group) {
     constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * QB * NW, TB = KT * DP * 2, CPR = DP / 8;
     constexpr int NL = KT * CPR / (64 * NW);  // loads a wave issues for a tile
     using W = Wave<T, DP, KT>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int kvh = blockIdx.x % A.kv_heads;
-    const Work w = locate(A, blockIdx.x / A.kv_heads, group, BM);
+    const Work w = locate(A, S, blockIdx.x / A.kv_heads, group, BM, true);
     if (!w.live) return;
     const int R = w.n * group, r0 = w.tile * BM, mine = r0 + wave * QB * 32;
     const float c = A.scale * 1.4426950408889634f;
     const int last = r0 + BM < R ? r0 + BM : R;
-    const int tiles = (seen(w, last - 1, group, A.causal) + KT - 1) / KT;
+    const int all = (seen(w, last - 1, group, A.causal) + KT - 1) / KT;
+    const int first = (int)((int64_t)all * w.chunk / w.nc), tiles = (int)((int64_t)all * (w.chunk + 1) / w.nc);
     Rows<T, DP> rows[QB];
 #pragma unroll
     for (int b = 0; b < QB; ++b) rows[b].begin(A, w, kvh, group, mine + 32 * b);
     // this wave's part: keys [0, hi) of which [0, lo) are seen by all its rows
-    const int hi = mine < R ? seen(w, mine + QB * 32 - 1, group, A.causal) : 0;
+    const int sees = mine < R ? seen(w, mine + QB * 32 - 1, group, A.causal) : 0;
+    const int hi = sees < tiles * KT ? sees : tiles * KT;
     const int lo = mine < R ? seen(w, mine, group, A.causal) : 0;
-    const int whole = lo / KT;  // the tiles below this one need no mask
+    const int whole = lo / KT > first ? lo / KT : first;  // the tiles below this one need no mask
 
     uint32_t ko[NL], vo[NL];
 #pragma unroll
@@ -377,10 +420,10 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
         for (int n = 0; n < NL; ++n) load_lds(rv, to + TB + n * NW * 1024, vo[n]);
     };
     bool checked = hi <= whole * KT;
-    if (tiles) load(tiles - 1);
-    for (int t = tiles - 1; t >= 0; --t) {
+    if (tiles > first) load(tiles - 1);
+    for (int t = tiles - 1; t >= first; --t) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t) load(t - 1);
+        if (t > first) load(t - 1);
         if (t * KT >= hi) continue;
         const char PCH_LDS* kl = (const char PCH_LDS*)lds + (t & 1) * 2 * TB;
         if (!checked && t < whole) {
@@ -405,7 +448,178 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
         for (int b = 0; b < QB; ++b)
             if (W::broken(rows[b])) W::repair(A, w, kvh, c, whole * KT, hi, KT, rows[b]);
 #pragma unroll
-    for (int b = 0; b < QB; ++b) W::finish(A, w, kvh, group, mine + 32 * b, rows[b]);
+    for (int b = 0; b < QB; ++b) W::finish(A, S, w, kvh, group, BM, (wave * QB + b) * 32 + (lane & 31), rows[b]);
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// A workgroup of NW waves takes 32 rows (one token's heads of a group, mostly) and a part of their keys; the waves take its
+// tiles of 32 keys in turn, each with LDS, statistics and sums of its own, and join at the end. What bounds it is the reading
+// of the keys: every wave keeps a whole tile of keys and of values on its way while it works on the one before.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <class T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, int group) {
+    constexpr int KT = 32, BM = 32, TB = KT * DP * 2, CPR = DP / 8, NL = KT * CPR / 64, PAD = DP + 4;
+    using W = Wave<T, DP, KT>;
+    __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * TB];
+    static_assert(NW * 4 * TB >= (NW * BM * PAD + NW * BM * 2) * 4, "the join fits the tiles' memory");
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int kvh = blockIdx.x % A.kv_heads;
+    const Work w = locate(A, S, blockIdx.x / A.kv_heads, group, BM, true);
+    if (!w.live) return;
+    const int R = w.n * group, r0 = w.tile * BM;
+    const float c = A.scale * 1.4426950408889634f;
+    const int rn = R - r0 < BM ? R - r0 : BM;
+    const int sees = seen(w, r0 + rn - 1, group, A.causal);
+    const int all = (sees + KT - 1) / KT;
+    const int first = (int)((int64_t)all * w.chunk / w.nc), tiles = (int)((int64_t)all * (w.chunk + 1) / w.nc);
+    const int hi = sees < tiles * KT ? sees : tiles * KT;
+    const int lo = seen(w, r0, group, A.causal);
+    const int whole = lo / KT > first ? lo / KT : first;
+    Rows<T, DP> row;
+    row.begin(A, w, kvh, group, r0);
+
+    uint32_t ko[NL], vo[NL];
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+        const int p = n * 64 + lane, key = p / CPR, cp = p % CPR;
+        const int ck = cp ^ Tile<DP>::kswz(key), cv = cp ^ Tile<DP>::vswz(key);
+        ko[n] = ck * 8 < A.dim ? key * (uint32_t)A.k.token * 2 + ck * 16 : 0x7ffffff0u;
+        vo[n] = cv * 8 < A.dim ? key * (uint32_t)A.v.token * 2 + cv * 16 : 0x7ffffff0u;
+    }
+    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 4 * TB;
+    const char* kp = (const char*)uniform64((uint64_t)at<T>(A.k, w.k0, kvh));
+    const char* vp = (const char*)uniform64((uint64_t)at<T>(A.v, w.k0, kvh));
+    auto load = [&](int t, int half) {
+        const int left = w.len - t * KT, nr = (left < KT ? left : KT) - 1;
+        const uint32_t to = base + half * 2 * TB;
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)t * KT * A.k.token * 2), 0,
+                                                          (nr * (int)A.k.token + A.dim) * 2, 0x00020000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + (int64_t)t * KT * A.v.token * 2), 0,
+                                                          (nr * (int)A.v.token + A.dim) * 2, 0x00020000);
+#pragma unroll
+        for (int n = 0; n < NL; ++n) load_lds(rk, to + n * 1024, ko[n]);
+#pragma unroll
+        for (int n = 0; n < NL; ++n) load_lds(rv, to + TB + n * 1024, vo[n]);
+    };
+    // this wave's tiles, from the last of those that are `wave` mod NW after the first
+    const int mine = tiles - first > wave ? (tiles - first - wave + NW - 1) / NW : 0;
+    bool unchecked = false;
+    const auto mend = [&] {
+        unchecked = false;
+        if (W::broken(row)) {
+            const int skip = whole - first > wave ? (whole - first - wave + NW - 1) / NW : 0;
+            W::repair(A, w, kvh, c, (first + wave + skip * NW) * KT, hi, KT * NW, row);
+        }
+    };
+    if (mine) load(first + wave + (mine - 1) * NW, (mine - 1) & 1);
+    for (int u = mine - 1; u >= 0; --u) {
+        const int t = first + wave + u * NW;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last tile's reads are done: its memory takes the next one
+        if (u) {
+            load(t - NW, (u - 1) & 1);
+            wait_loads<3 * NL>();
+        } else {
+            wait_loads<NL>();
+        }
+        const char PCH_LDS* kl = (const char PCH_LDS*)lds + wave * 4 * TB + (u & 1) * 2 * TB;
+        v16f z[1];
+        W::scores(kl, row, z);
+        if (t >= whole) {
+            W::mask(row, t * KT, z);
+            unchecked |= A.causal && (t + 1) * KT > lo && lo < w.len;
+        } else if (unchecked) {
+            mend();
+        }
+        W::softmax(row, c, z);
+        if (u)
+            wait_loads<2 * NL>();
+        else
+            wait_loads<0>();
+        W::values(kl + TB, row, z);
+    }
+    if (unchecked) mend();
+
+    // the waves' sums joined: each scaled to the largest maximum, in the order of the waves
+    float PCH_LDS* sh = (float PCH_LDS*)lds;
+    float PCH_LDS* st = sh + NW * BM * PAD;
+    const int cc = lane & 31, h = lane >> 5;
+    const float l = row.l + other(row.l);
+    __syncthreads();
+    if (h == 0) st[wave * BM + cc] = row.m;
+    __syncthreads();
+    float m = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) m = fmaxf(m, st[x * BM + cc]);
+    const float f = row.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(row.m - m);
+    if (h == 0) st[NW * BM + wave * BM + cc] = l * f;
+    if (cc < rn)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *(v4f PCH_LDS*)(sh + (wave * BM + cc) * PAD + 32 * d + 8 * g + 4 * h) =
+                    v4f{row.o[d][4 * g] * f, row.o[d][4 * g + 1] * f, row.o[d][4 * g + 2] * f, row.o[d][4 * g + 3] * f};
+    __syncthreads();
+    const int slot = (w.slot + w.chunk) * A.kv_heads + kvh;
+    const int q4 = A.dim >> 2;
+    for (int x = threadIdx.x; x < rn * q4; x += 64 * NW) {
+        const int r = x / q4, d = (x - r * q4) * 4;
+        v4f o = *(const v4f PCH_LDS*)(sh + r * PAD + d);
+        float lr = st[NW * BM + r], mr = st[r];
+#pragma unroll
+        for (int y = 1; y < NW; ++y) {
+            o += *(const v4f PCH_LDS*)(sh + (y * BM + r) * PAD + d);
+            lr += st[NW * BM + y * BM + r];
+            mr = fmaxf(mr, st[y * BM + r]);
+        }
+        if (w.nc > 1) {
+            *(v4f*)(S.sums(slot, BM, A.dim) + r * A.dim + d) = o;
+            if (d == 0) *(float2*)(S.stats(slot, BM, A.dim) + r * 2) = make_float2(mr, lr);
+        } else {
+            const int i = (r0 + r) / group, hd = kvh * group + (r0 + r - i * group);
+            const float inv = mr == -INFINITY ? 0.0f : 1.0f / lr;
+            *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
+            if (A.lse && d == 0)
+                A.lse[(int64_t)(w.q0 + i) * A.heads + hd] =
+                    mr == -INFINITY ? -INFINITY : (mr + __log2f(lr)) * 0.6931471805599453f;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ parts of the keys joined
+// A workgroup per tile of rows and key head, a thread per row and 4 dimensions: the parts in their order, each scaled to the
+// largest maximum.
+template <class T>
+__global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, int group, int BM) {
+    const int kvh = blockIdx.x % A.kv_heads;
+    const Work w = locate(A, S, blockIdx.x / A.kv_heads, group, BM, false);
+    if (!w.live || w.nc == 1) return;
+    const int R = w.n * group, r0 = w.tile * BM, rn = R - r0 < BM ? R - r0 : BM, q4 = A.dim >> 2;
+    for (int x = blockIdx.y * 256 + threadIdx.x; x < rn * q4; x += 256 * gridDim.y) {
+        const int r = x / q4, d = (x - r * q4) * 4;
+        float m = -INFINITY;
+        for (int p = 0; p < w.nc; ++p) m = fmaxf(m, S.stats((w.slot + p) * A.kv_heads + kvh, BM, A.dim)[r * 2]);
+        float l = 0;
+        v4f o = (v4f)0.0f;
+        for (int p = 0; p < w.nc; ++p) {
+            const int slot = (w.slot + p) * A.kv_heads + kvh;
+            const float2 st = *(const float2*)(S.stats(slot, BM, A.dim) + r * 2);
+            const v4f y = *(const v4f*)(S.sums(slot, BM, A.dim) + (int64_t)r * A.dim + d);
+            if (st.x == -INFINITY) continue;
+            const float f = __builtin_amdgcn_exp2f(st.x - m);
+            l = fmaf(st.y, f, l);
+            o += y * f;
+        }
+        const int i = (r0 + r) / group, hd = kvh * group + (r0 + r - i * group);
+        const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+        *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
+        if (A.lse && d == 0)
+            A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = m == -INFINITY ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+    }
 }
 
 // 0, or the error
@@ -430,20 +644,60 @@ static int checked(const AttentionArgs* a) {
     return 0;
 }
 
-template <class T, int DP, int QB, int NW>
-static int rows_run(const AttentionArgs& a, hipStream_t s) {
+// the kernel and the split of a call
+struct Choice {
+    int few;      // few_k, else rows_k
+    int BM;       // rows of a tile
+    int64_t items;  // (sequence, tile) pairs at most
+    int most, size;
+};
+static uint64_t work_bytes(const AttentionArgs& a, const Choice& c) {
+    return c.most > 1 ? (uint64_t)c.items * c.most * a.kv_heads * c.BM * (a.dim + 2) * 4 : 0;
+}
+
+#ifndef PCH_WANT
+#define PCH_WANT 1024
+#endif
+static Choice choose(const AttentionArgs& a) {
     const int group = a.heads / a.kv_heads;
-    const int64_t items = (int64_t)a.tokens * group / (32 * QB * NW) + a.seqs;
-    if (items * a.kv_heads > 0x7fffffff) return -2;
-    hipLaunchKernelGGL((rows_k<T, DP, QB, NW>), dim3((unsigned)(items * a.kv_heads)), dim3(64 * NW), 0, s, a, group);
+    Choice c;
+    c.few = (int64_t)a.max_q * group <= 32;
+    c.BM = c.few ? 32 : 128;
+    c.items = (int64_t)a.tokens * group / c.BM + a.seqs;
+    const int64_t want = PCH_WANT;
+    const int64_t base = c.items * a.kv_heads;
+    const int64_t shortest = 256;  // keys of a part at least
+    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / shortest));
+    c.size = (a.max_k + c.most - 1) / std::max(1, c.most);
+    return c;
+}
+
+template <class T, int DP>
+static int run_t(const AttentionArgs& a, hipStream_t s) {
+    const int group = a.heads / a.kv_heads;
+    Choice c = choose(a);
+    while (c.most > 1 && work_bytes(a, c) > (a.work ? a.work_bytes : 0)) c.most = c.most / 2;
+    if (c.most > 1) c.size = (a.max_k + c.most - 1) / c.most;
+    const int64_t blocks = c.items * c.most * a.kv_heads;
+    if (blocks > 0x7fffffff) return -2;
+    const Split S = {c.most, c.size, (float*)a.work, c.items * c.most * a.kv_heads};
+    constexpr int NW = DP > 128 ? 2 : 4;
+    if (c.few)
+        hipLaunchKernelGGL((few_k<T, DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, a, S, group);
+    else
+        hipLaunchKernelGGL((rows_k<T, DP, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a, S, group);
+    if (c.most > 1) {
+        if (int e = launch_rc()) return e;
+        hipLaunchKernelGGL(join_k<T>, dim3((unsigned)(c.items * a.kv_heads), c.few ? 1 : 8), dim3(256), 0, s, a, S, group, c.BM);
+    }
     return launch_rc();
 }
 
 template <class T>
-static int run_t(const AttentionArgs& a, hipStream_t s) {
-    if (a.dim <= 64) return rows_run<T, 64, 1, 4>(a, s);
-    if (a.dim <= 128) return rows_run<T, 128, 1, 4>(a, s);
-    return rows_run<T, 256, 1, 4>(a, s);
+static int run(const AttentionArgs& a, hipStream_t s) {
+    if (a.dim <= 64) return run_t<T, 64>(a, s);
+    if (a.dim <= 128) return run_t<T, 128>(a, s);
+    return run_t<T, 256>(a, s);
 }
 
 }  // namespace clear
@@ -453,12 +707,12 @@ using namespace pch;
 using namespace pch::clear;
 
 extern "C" uint64_t pcx_attention_workspace(const AttentionArgs* a) {
-    (void)a;
-    return 0;
+    if (checked(a) || !a->tokens || !a->seqs || !a->heads) return 0;
+    return work_bytes(*a, choose(*a));
 }
 
 extern "C" int pcx_attention(const AttentionArgs* a, pc_stream_t s) {
     if (int e = checked(a)) return e;
     if (!a->tokens || !a->seqs || !a->heads) return 0;
-    return a->type == PCX_BF16 ? run_t<bf16>(*a, (hipStream_t)s) : run_t<f16>(*a, (hipStream_t)s);
+    return a->type == PCX_BF16 ? run<bf16>(*a, (hipStream_t)s) : run<f16>(*a, (hipStream_t)s);
 }
