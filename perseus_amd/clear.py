@@ -11,6 +11,7 @@ stride() and dtype; their last dimension is dense, the others may have any strid
 on the Clear's stream; nothing is allocated, synchronised or copied by a call.
 """
 import ctypes as C
+import struct
 
 import numpy as np
 
@@ -107,6 +108,17 @@ class Array:
     def stride(self):
         return self._strides
 
+    def numel(self):
+        return int(np.prod(self.shape, dtype=np.int64))
+
+    def is_contiguous(self):
+        n = 1
+        for size, step in zip(reversed(self.shape), reversed(self._strides)):
+            if size != 1 and step != n:
+                return not all(self.shape)
+            n *= size
+        return True
+
 
 # ---------------------------------------------------------------------------------------------------- rotation tables
 
@@ -182,6 +194,11 @@ class AttentionArgs(C.Structure):
                 ("max_q", _i32), ("max_k", _i32), ("scale", _f32)]
 
 
+# the same layouts for struct.pack: a call packs its arguments in about a microsecond, a ctypes Structure takes four
+_ROTARY = struct.Struct("@" + "Pqq" * 2 + "PPq" + "i" * 8)
+_QK_NORM_ROTARY = struct.Struct("@" + "Pqq" * 6 + "P" * 5 + "qq" + "i" * 7 + "f")
+_ATTENTION = struct.Struct("@" + "Pqq" * 4 + "P" * 5 + "Qq" + "i" * 9 + "f")
+assert (_ROTARY.size, _QK_NORM_ROTARY.size, _ATTENTION.size) == (104, 232, 192)
 assert (C.sizeof(RotaryArgs), C.sizeof(QkNormRotaryArgs), C.sizeof(AttentionArgs)) == (104, 232, 192)
 
 
@@ -194,22 +211,19 @@ def _heads(x, name):
         raise ValueError(f"{name}: not on the device")
     if st[2] != 1 and shape[2] > 1:
         raise ValueError(f"{name}: its last dimension is not dense")
-    return x.data_ptr(), st[0], st[1], shape, _type(x.dtype)
+    return x.data_ptr(), st[0], st[1], shape, _known.get(x.dtype) or _type(x.dtype)
 
 
 def _flat(x, name, dtype, count):
     """the address of a dense tensor of `count` values (None: any number) of one type"""
     if not x.is_cuda:
         raise ValueError(f"{name}: not on the device")
-    if _type(x.dtype) != dtype:
+    if (_known.get(x.dtype) or _type(x.dtype)) != dtype:
         raise ValueError(f"{name}: {dtype} is wanted, got {x.dtype}")
-    n, st = 1, x.stride()
-    for size, step in zip(reversed(x.shape), reversed(st)):
-        if size != 1 and step != n:
-            raise ValueError(f"{name}: not dense")
-        n *= size
-    if count is not None and n != count:
-        raise ValueError(f"{name}: {count} values are wanted, got {n}")
+    if not x.is_contiguous():
+        raise ValueError(f"{name}: not dense")
+    if count is not None and x.numel() != count:
+        raise ValueError(f"{name}: {count} values are wanted, got {x.numel()}")
     return x.data_ptr()
 
 
@@ -222,7 +236,7 @@ def _layout(layout):
 def _table(table, positions, tokens):
     """(positions' address, table's address, places, rot)"""
     if table is None:
-        return None, None, 0, 0
+        return 0, 0, 0, 0
     if len(table.shape) != 3 or table.shape[2] != 2:
         raise ValueError("table: [places][rot / 2][2] is wanted")
     return (_flat(positions, "positions", "i32", tokens), _flat(table, "table", "f32", None), table.shape[0],
@@ -236,7 +250,7 @@ class Clear:
     def __init__(self, stream, workspace=64 << 20):
         self.stream = stream
         self.work = DevBuf(-(-int(workspace) // 4)) if workspace else None
-        self._work = (self.work.ptr.value, 4 * self.work.words) if workspace else (None, 0)
+        self._work = (self.work.ptr.value, 4 * self.work.words) if workspace else (0, 0)
 
     def rotary(self, x, positions, table, out, layout="half", inverse=False):
         """out = x [tokens][heads][dim] with the first rot dimensions of each head turned by table[positions[t]] (f32
@@ -245,12 +259,12 @@ class Clear:
         a, at, ah, shape, kind = _heads(x, "x")
         b, bt, bh, oshape, okind = _heads(out, "out")
         tokens, heads, dim = shape
-        if tuple(oshape) != tuple(shape) or okind != kind or kind not in TYPES:
+        if oshape != shape or okind != kind or kind not in TYPES:
             raise ValueError("x and out: one shape and one floating type")
         pos, tab, places, rot = _table(table, positions, tokens)
-        args = RotaryArgs(a, at, ah, b, bt, bh, pos, tab, places, tokens, heads, dim, rot, TYPES[kind], _layout(layout),
-                          bool(inverse), 0)
-        check(LIB.pcx_rotary(C.byref(args), self.stream.h), "rotary")
+        args = _ROTARY.pack(a, at, ah, b, bt, bh, pos, tab, places, tokens, heads, dim, rot, TYPES[kind], _layout(layout),
+                            bool(inverse), 0)
+        check(LIB.pcx_rotary(args, self.stream.h), "rotary")
 
     def qk_norm_rotary(self, q, k, q_weight, k_weight, positions, table, q_out, k_out, eps=1e-6, layout="half", v=None,
                        v_out=None, slots=None):
@@ -263,28 +277,28 @@ class Clear:
         d, dt, dh, kos, kok = _heads(k_out, "k_out")
         tokens, heads, dim = qs
         kv = ks[1]
-        if ks[0] != tokens or ks[2] != dim or tuple(qos) != tuple(qs) or tuple(kos[1:]) != (kv, dim):
+        if ks[0] != tokens or ks[2] != dim or qos != qs or kos[1:] != ks[1:]:
             raise ValueError("q and k: the same tokens and dim, the outputs' shapes as theirs")
         if not kind == kkind == qok == kok or kind not in TYPES:
             raise ValueError("q, k and the outputs: one floating type")
         if slots is None and kos[0] != tokens:
             raise ValueError("k_out: one row for each token where there are no slots")
-        e, et, eh, f, ft, fh = None, 0, 0, None, 0, 0
+        e, et, eh, f, ft, fh = 0, 0, 0, 0, 0, 0
         if (v is None) != (v_out is None):
             raise ValueError("v and v_out go together")
         if v is not None:
             e, et, eh, vs, vk = _heads(v, "v")
             f, ft, fh, vos, vok = _heads(v_out, "v_out")
-            if tuple(vs) != tuple(ks) or tuple(vos) != tuple(kos) or not vk == vok == kind:
+            if vs != ks or vos != kos or not vk == vok == kind:
                 raise ValueError("v and v_out: the shapes and type of k and k_out")
         pos, tab, places, rot = _table(table, positions, tokens)
-        args = QkNormRotaryArgs(
+        args = _QK_NORM_ROTARY.pack(
             a, at, ah, b, bt, bh, e, et, eh, c, ct, ch, d, dt, dh, f, ft, fh,
-            None if q_weight is None else _flat(q_weight, "q_weight", "f32", dim),
-            None if k_weight is None else _flat(k_weight, "k_weight", "f32", dim), pos, tab,
-            None if slots is None else _flat(slots, "slots", "i64", tokens), places, kos[0], tokens, heads, kv, dim, rot,
+            0 if q_weight is None else _flat(q_weight, "q_weight", "f32", dim),
+            0 if k_weight is None else _flat(k_weight, "k_weight", "f32", dim), pos, tab,
+            0 if slots is None else _flat(slots, "slots", "i64", tokens), places, kos[0], tokens, heads, kv, dim, rot,
             TYPES[kind], _layout(layout), eps)
-        check(LIB.pcx_qk_norm_rotary(C.byref(args), self.stream.h), "qk_norm_rotary")
+        check(LIB.pcx_qk_norm_rotary(args, self.stream.h), "qk_norm_rotary")
 
     def attention(self, q, k, v, q_start, k_start, k_len, out, lse=None, scale=None, causal=True, max_q=None, max_k=None):
         """out [tokens][heads][dim] and lse (f32 [tokens][heads], or None) of the packed queries q over k and v [rows][kv
@@ -292,25 +306,27 @@ class Clear:
         (i64, i32; device arrays). causal: the last query sees the last key, each earlier one a key less. scale: 1 /
         sqrt(dim) unless given. max_q, max_k: the longest runs expected (the buffers' rows unless given); they only
         choose kernels."""
-        args = self.attention_args(q, k, v, q_start, k_start, k_len, out, lse, scale, causal, max_q, max_k)
-        check(LIB.pcx_attention(C.byref(args), self.stream.h), "attention")
+        args = self._attention(q, k, v, q_start, k_start, k_len, out, lse, scale, causal, max_q, max_k)
+        check(LIB.pcx_attention(args, self.stream.h), "attention")
 
-    def attention_args(self, q, k, v, q_start, k_start, k_len, out, lse=None, scale=None, causal=True, max_q=None,
-                       max_k=None):
-        """attention's checked arguments, for pcx_attention or pcx_attention_workspace."""
+    def attention_args(self, *args, **kw):
+        """attention's checked arguments as the struct that pcx_attention and pcx_attention_workspace take."""
+        return AttentionArgs.from_buffer_copy(self._attention(*args, **kw))
+
+    def _attention(self, q, k, v, q_start, k_start, k_len, out, lse=None, scale=None, causal=True, max_q=None, max_k=None):
         a, at, ah, qs, kind = _heads(q, "q")
         b, bt, bh, ks, kkind = _heads(k, "k")
         c, ct, ch, vs, vkind = _heads(v, "v")
         d, dt, dh, os, okind = _heads(out, "out")
         tokens, heads, dim = qs
         rows, kv, kdim = ks
-        if kdim != dim or tuple(vs) != tuple(ks) or tuple(os) != tuple(qs):
+        if kdim != dim or vs != ks or os != qs:
             raise ValueError("k and v alike, out as q, one dim")
         if not kind == kkind == vkind == okind or kind not in TYPES:
             raise ValueError("q, k, v and out: one floating type")
         seqs = k_len.shape[0]
-        return AttentionArgs(
-            a, at, ah, b, bt, bh, c, ct, ch, d, dt, dh, None if lse is None else _flat(lse, "lse", "f32", tokens * heads),
+        return _ATTENTION.pack(
+            a, at, ah, b, bt, bh, c, ct, ch, d, dt, dh, 0 if lse is None else _flat(lse, "lse", "f32", tokens * heads),
             _flat(q_start, "q_start", "i32", seqs + 1), _flat(k_start, "k_start", "i64", seqs),
             _flat(k_len, "k_len", "i32", seqs), *self._work, rows, tokens, seqs, heads, kv, dim, TYPES[kind],
             bool(causal), tokens if max_q is None else max_q, min(rows, 0x7FFFFFFF) if max_k is None else max_k,

@@ -4,6 +4,8 @@
 // Per head x of dim values: n = x w / sqrt(mean(x^2) + eps) (the norm, where wanted), then the pairs i < rot / 2 turn,
 // (a, b) -> (a c - b s, b c + a s) with (c, s) = table[position][i]. Sums, squares and products are in f32; a value is
 // rounded once, when it is stored.
+#include <algorithm>
+
 #include "clear.h"
 
 namespace pch {
@@ -23,7 +25,119 @@ struct Pass {
 
 constexpr int WAVES = 4;
 
-// a wave per head, a lane per pair or copied value
+// ------------------------------------------------------------------------------------------------ 16 values a lane
+// Two units of 8 values (16 bytes of a 16-bit type) to a lane: the two that hold its pairs' halves, or neighbours where pairs
+// are neighbours. A power of two of lanes takes a head, a wave as many heads of one token as fit.
+template <class T>
+struct Eight {
+    float v[8];
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (sizeof(T) == 2) {
+            typedef T t8 __attribute__((ext_vector_type(8)));
+            const t8 x = *(const t8*)p;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = (float)x[i];
+        } else {
+            const float4 x = ((const float4*)p)[0], y = ((const float4*)p)[1];
+            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+        }
+    }
+    template <bool PAST>
+    __device__ __forceinline__ void store(T* p) const {
+        constexpr int PER = 16 / sizeof(T);
+        typedef T tv __attribute__((ext_vector_type(PER)));
+#pragma unroll
+        for (int k = 0; k < 8; k += PER) {
+            tv x;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) x[i] = (T)v[k + i];
+            if constexpr (PAST)
+                __builtin_nontemporal_store(x, (tv*)(p + k));
+            else
+                *(tv*)(p + k) = x;
+        }
+    }
+};
+
+template <class T, bool NORM, bool INTER, bool PAST>
+__global__ void __launch_bounds__(64 * WAVES) units_k(Pass A, int lph_log, uint32_t chunks) {
+    const int lane = threadIdx.x & 63, lph = 1 << lph_log, slot = lane >> lph_log, l = lane & (lph - 1);
+    const uint32_t wv = blockIdx.x * WAVES + (threadIdx.x >> 6), t = wv / chunks;
+    const int hh = (int)(wv - t * chunks) * (64 >> lph_log) + slot;
+    if (t >= (uint32_t)A.tokens || hh >= A.total) return;  // whole heads: the lanes of one leave together
+    // q, k or v by selects: an indexed kernel argument would be a load, and the first load waits for it
+    const bool isq = !NORM || hh < A.heads, isv = NORM && hh >= A.heads + A.kv_heads;
+    const int h = isq ? hh : isv ? hh - A.heads - A.kv_heads : hh - A.heads;
+    const HeadsRef in = isq ? A.in[0] : isv ? A.in[2] : A.in[1], out = isq ? A.out[0] : isv ? A.out[2] : A.out[1];
+    const int units = A.dim >> 3, turned = isv ? 0 : A.rot >> 3;
+    // this lane's units, and whether they turn
+    int ua, ub;
+    bool ta, tb;
+    if (INTER) {
+        ua = 2 * l, ub = 2 * l + 1;
+        ta = ua < turned, tb = ub < turned;
+    } else {
+        const int half = turned >> 1;
+        ta = tb = l < half;
+        ua = ta ? l : turned + 2 * (l - half);
+        ub = ta ? l + half : ua + 1;
+    }
+    const bool va = ua < units, vb = ub < units;
+    Eight<T> a, b;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a.v[i] = b.v[i] = 0;
+    const T* x = at<T>(in, t, h);
+    if (va) a.load(x + 8 * ua);
+    if (vb) b.load(x + 8 * ub);
+    int64_t row = t;
+    if (NORM && !isq && A.slots) {
+        row = A.slots[t];
+        if (row >= A.cache_rows) row = -1;
+    }
+    float c[8], s[8];  // of this lane's pairs
+    if (ta) {
+        const int64_t pos = A.positions[t];
+        const bool inside = pos >= 0 && pos < A.places;
+        const float4* tab = (const float4*)(A.table + (inside ? pos : 0) * A.rot) + (INTER ? ua * 2 : l * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float nan = __builtin_nanf("");
+            const float4 y = !inside ? make_float4(nan, nan, nan, nan) : !INTER || i < 2 || tb ? tab[i] : make_float4(1, 0, 1, 0);
+            c[2 * i] = y.x, c[2 * i + 1] = y.z;
+            s[2 * i] = y.y * A.sign, s[2 * i + 1] = y.w * A.sign;
+        }
+    }
+    if (NORM && !isv) {
+        const float* w = isq ? A.w[0] : A.w[1];
+        Eight<float> wa, wb;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) wa.v[i] = wb.v[i] = 1;
+        if (w && va) wa.load(w + 8 * ua);
+        if (w && vb) wb.load(w + 8 * ub);
+        float sum = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = fmaf(a.v[i], a.v[i], fmaf(b.v[i], b.v[i], sum));
+        for (int m = 1; m < lph; m <<= 1) sum += __shfl_xor(sum, m);
+        const float g = 1.0f / sqrtf(sum / A.dim + A.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a.v[i] *= g * wa.v[i], b.v[i] *= g * wb.v[i];
+    }
+    if (row < 0) return;
+    if (ta)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float& x0 = INTER ? (i < 4 ? a.v[2 * i] : b.v[2 * i - 8]) : a.v[i];
+            float& x1 = INTER ? (i < 4 ? a.v[2 * i + 1] : b.v[2 * i - 7]) : b.v[i];
+            const float y0 = x0 * c[i] - x1 * s[i], y1 = x1 * c[i] + x0 * s[i];
+            if (!INTER || i < 4 || tb) x0 = y0, x1 = y1;
+        }
+    T* y = at<T>(out, row, h);
+    if (va) a.template store<PAST>(y + 8 * ua);
+    if (vb) b.template store<PAST>(y + 8 * ub);
+}
+
+// ------------------------------------------------------------------------------------------------ any size
+// Odd sizes, strides and addresses: a wave per head, a lane per pair or copied value.
 template <class T, bool NORM, bool INTER>
 __global__ void __launch_bounds__(64 * WAVES) heads_k(Pass A) {
     const int lane = threadIdx.x & 63;
@@ -67,25 +181,56 @@ __global__ void __launch_bounds__(64 * WAVES) heads_k(Pass A) {
     }
 }
 
-template <class T, bool NORM>
-static int run_t(const Pass& a, bool inter, hipStream_t s) {
+// whether units_k's 16-byte accesses and whole units fit
+template <class T>
+static bool whole_units(const Pass& a, bool inter) {
+    constexpr int per = 16 / (int)sizeof(T);
+    if (a.dim % 8 || a.rot % (inter ? 8 : 16)) return false;
+    if (((uintptr_t)a.table | (uintptr_t)a.w[0] | (uintptr_t)a.w[1]) % 16) return false;
+    for (int i = 0; i < 3; ++i)
+        for (const HeadsRef* r : {&a.in[i], &a.out[i]})
+            if (r->base && ((uintptr_t)r->base % 16 || r->token % per || r->head % per)) return false;
+    return true;
+}
+
+template <class T, bool NORM, bool INTER>
+static int run_t(const Pass& a, hipStream_t s) {
+    if (whole_units<T>(a, INTER)) {
+        int lph_log = 0;
+        while (16 << lph_log < a.dim) ++lph_log;
+        const int slots = 64 >> lph_log, all = (a.total + slots - 1) / slots;
+        const int64_t blocks = ((int64_t)a.tokens * all + WAVES - 1) / WAVES;
+        // outputs that no L2 holds until they are read go past the caches: 84 MB 38.5 -> 35.3 us, 168 MB 83 -> 78
+        const bool past = (int64_t)a.tokens * a.total * a.dim * sizeof(T) > 32 << 20;
+        if (blocks <= 0x3fffffff) {
+            const dim3 grid((unsigned)blocks);
+            if (past)
+                hipLaunchKernelGGL((units_k<T, NORM, INTER, true>), grid, dim3(64 * WAVES), 0, s, a, lph_log, (uint32_t)all);
+            else
+                hipLaunchKernelGGL((units_k<T, NORM, INTER, false>), grid, dim3(64 * WAVES), 0, s, a, lph_log, (uint32_t)all);
+            return launch_rc();
+        }
+    }
     const int64_t items = (int64_t)a.tokens * a.total;
     const int64_t blocks = (items + WAVES - 1) / WAVES;
     const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)));
-    if (inter)
-        hipLaunchKernelGGL((heads_k<T, NORM, true>), grid, dim3(64 * WAVES), 0, s, a);
-    else
-        hipLaunchKernelGGL((heads_k<T, NORM, false>), grid, dim3(64 * WAVES), 0, s, a);
+    hipLaunchKernelGGL((heads_k<T, NORM, INTER>), grid, dim3(64 * WAVES), 0, s, a);
     return launch_rc();
+}
+
+template <class T>
+static int run_l(const Pass& a, bool norm, bool inter, hipStream_t s) {
+    if (norm) return inter ? run_t<T, true, true>(a, s) : run_t<T, true, false>(a, s);
+    return inter ? run_t<T, false, true>(a, s) : run_t<T, false, false>(a, s);
 }
 
 static int run(const Pass& a, bool norm, bool inter, int type, pc_stream_t s) {
     if ((int64_t)a.tokens * a.total == 0) return 0;
     const hipStream_t st = (hipStream_t)s;
     switch (type) {
-    case PCX_BF16: return norm ? run_t<bf16, true>(a, inter, st) : run_t<bf16, false>(a, inter, st);
-    case PCX_F16: return norm ? run_t<f16, true>(a, inter, st) : run_t<f16, false>(a, inter, st);
-    default: return norm ? run_t<float, true>(a, inter, st) : run_t<float, false>(a, inter, st);
+    case PCX_BF16: return run_l<bf16>(a, norm, inter, st);
+    case PCX_F16: return run_l<f16>(a, norm, inter, st);
+    default: return run_l<float>(a, norm, inter, st);
     }
 }
 

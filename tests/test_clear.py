@@ -27,6 +27,12 @@ class Fake:
     def stride(self):
         return self._s
 
+    def numel(self):
+        return math.prod(self.shape)
+
+    def is_contiguous(self):
+        return self._s == tuple(math.prod(self.shape[i + 1:]) for i in range(len(self.shape)))
+
 
 class NoStream:
     h = None
@@ -182,3 +188,19 @@ def test_the_header_s_structs():
             for n in names:
                 want += [n, n + "_token", n + "_head"] if line.startswith("HeadsRef") else [n]
         assert [f for f, _ in getattr(clear, name)._fields_] == want
+
+
+def test_packed_arguments_are_the_structs(ops):
+    """struct.pack's layouts are the structs': the same bytes give the same fields"""
+    x, kv = Fake((4, 6, 64), strides=(512, 64, 1)), Fake((9, 2, 64), ptr=P + 64)
+    a = ops.attention_args(x, kv, kv, Fake((3,), "i32"), Fake((2,), "i64", ptr=P + 16), Fake((2,), "i32", ptr=P + 32), x,
+                           Fake((4, 6), "f32", ptr=P + 48), scale=0.5, causal=False, max_q=3, max_k=7)
+    got = {n: getattr(a, n) for n, _ in clear.AttentionArgs._fields_}
+    want = dict(q=P, q_token=512, q_head=64, k=P + 64, k_token=128, k_head=64, v=P + 64, v_token=128, v_head=64, out=P,
+                out_token=512, out_head=64, lse=P + 48, q_start=P, k_start=P + 16, k_len=P + 32, work=None, work_bytes=0,
+                kv_rows=9, tokens=4, seqs=2, heads=6, kv_heads=2, dim=64, type=0, causal=0, max_q=3, max_k=7, scale=0.5)
+    assert got == want
+    for cls, packed in ((clear.RotaryArgs, clear._ROTARY), (clear.QkNormRotaryArgs, clear._QK_NORM_ROTARY)):
+        n = len(cls._fields_)
+        b = cls.from_buffer_copy(packed.pack(*range(1, n + 1)))
+        assert [getattr(b, f) for f, _ in cls._fields_] == list(range(1, n + 1))
