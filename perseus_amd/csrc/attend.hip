@@ -26,7 +26,6 @@ typedef short v8s __attribute__((ext_vector_type(8)));
 typedef float v8f __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 #define PCH_LDS __attribute__((address_space(3)))
-
 template <class T>
 struct Mat;
 template <>
@@ -55,14 +54,14 @@ __device__ __forceinline__ float other(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------ tiles of keys
-// KT rows of DP values in LDS, 16-byte chunks permuted within a row so that both readings are free of bank conflicts: keys
-// (32 lanes take one chunk of 32 rows) by xor with the row number, values (the transposing read takes 32 bytes of 8 rows) by
-// xor with twice the row number.
+// KT rows of room for DP values in LDS (of which the products take DC), 16-byte chunks permuted within a row so that both readings are free of bank conflicts: keys
+// (16 lanes take one chunk of 16 rows) by xor with the row number, values (32 lanes of the transposing read take 64 bytes of 4
+// rows) by xor with four times the row number.
 template <int DP>
 struct Tile {
     static constexpr int CPR = DP / 8;  // chunks of a row
     static __device__ __forceinline__ int kswz(int key) { return DP == 64 ? (key >> 1) & 7 : key & 15; }
-    static __device__ __forceinline__ int vswz(int key) { return DP == 64 ? 2 * ((key >> 1) & 3) : 2 * (key & 7); }
+    static __device__ __forceinline__ int vswz(int key) { return DP == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); }
 };
 
 // 64 lanes' 16 bytes each from a buffer into LDS at `lds` + 16 lane; lanes past the buffer's end write zeros. It counts
@@ -101,7 +100,7 @@ struct Split {
     int64_t slots;
     __device__ __forceinline__ int parts(int len) const {
         if (most <= 1) return 1;
-        const int n = (int)(((int64_t)len + size - 1) / size);
+        const int n = (int)(((uint32_t)len + size - 1) / (uint32_t)size);
         return n < 1 ? 1 : n < most ? n : most;
     }
     __device__ __forceinline__ float* sums(int slot, int BM, int dim) const { return work + (int64_t)slot * BM * dim; }
@@ -112,10 +111,37 @@ struct Split {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
-// item -> (sequence, tile of BM rows, part of its keys), the sequences' tiles one after the other, each sequence's last
-// (longest, where causal) first; split false: all parts of a tile in one item. Every wave finds it by itself: a prefix sum
-// over the lanes, 64 sequences at a time.
-__device__ __forceinline__ Work locate(const AttentionArgs& A, const Split& S, int item, int group, int BM, bool split) {
+// inclusive sums over the lanes of a wave, and the largest value (by data-parallel moves: no trip through LDS)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int lane_sums(int x) {
+    x += moved<0x111, 0xf>(x);  // from 1, 2, 4 and 8 lanes below in a row of 16
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);  // the last lane of rows 0 and 2 into rows 1 and 3
+    x += moved<0x143, 0xc>(x);  // lane 31 into rows 2 and 3
+    return x;
+}
+__device__ __forceinline__ int total(int x) { return __builtin_amdgcn_readlane(lane_sums(x), 63); }
+__device__ __forceinline__ int largest(int x) {  // of values not negative
+    x = max(x, moved<0x111, 0xf>(x));
+    x = max(x, moved<0x112, 0xf>(x));
+    x = max(x, moved<0x114, 0xf>(x));
+    x = max(x, moved<0x118, 0xf>(x));
+    x = max(x, moved<0x142, 0xa>(x));
+    x = max(x, moved<0x143, 0xc>(x));
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
+// item -> (sequence, tile of BM rows, part of its keys); BYPART false: all parts of a tile in one item. Every wave finds it by
+// itself, a lane per sequence. BYLEVEL: the tiles of up to 16 sequences go longest first (a tile's level: its keys in units of
+// its rows' queries), as workgroups start in their order and a long one that starts last is waited for; else, and for more
+// sequences, where finding it would cost more, one sequence after the other, each sequence's last tile first.
+template <bool BYPART, bool BYLEVEL>
+__device__ __forceinline__ Work locate(const AttentionArgs& A, const Split& S, int item, int group, int BM) {
     const int lane = threadIdx.x & 63;
     Work w;
     w.live = false;
@@ -133,96 +159,155 @@ __device__ __forceinline__ Work locate(const AttentionArgs& A, const Split& S, i
             if (len < 0) len = 0;
             if (len > A.kv_rows - k0) len = (int)(A.kv_rows - k0);
         }
-        const int parts = S.parts(len), nt = (int)(((int64_t)n * group + BM - 1) / BM) * (split ? parts : 1);
-        int sum = nt;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int v = __shfl_up(sum, m);
-            if (lane >= m) sum += v;
-        }
-        const uint64_t past = __ballot(sum > item);
-        if (past) {
-            const int src = __builtin_ctzll(past);
-            w.q0 = __builtin_amdgcn_readlane(q0, src);
-            w.n = __builtin_amdgcn_readlane(n, src);
-            w.len = __builtin_amdgcn_readlane(len, src);
-            const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)k0, src);
-            const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)k0 >> 32), src);
-            w.k0 = (int64_t)(((uint64_t)hi << 32) | lo);
+        const int parts = S.parts(len), tiles = (int)(((int64_t)n * group + BM - 1) / BM), nc = BYPART ? parts : 1;
+        int src = 0, at;  // the lane of the item's sequence, and its number there
+        if (A.seqs == 1) {
+            const int all = __builtin_amdgcn_readfirstlane(tiles * nc);
+            if (item >= all) return w;
+            w.nc = __builtin_amdgcn_readfirstlane(parts);
+            at = all - 1 - item;
+            w.tile = BYPART && w.nc > 1 ? at / w.nc : at;
+            w.chunk = BYPART ? at - w.tile * w.nc : 0;
+        } else if (BYLEVEL && A.seqs <= 64) {
+            // a tile's level is `above` + its number, or (not causal) `above`
+            const int keys = A.causal ? (len > n ? len - n : 0) : len;
+            const int above = (int)((int64_t)keys * group / BM), span = A.causal ? tiles : tiles > 0;
+            const int each = A.causal ? nc : tiles * nc;
+            // the items of a lane's own level u and more
+            const auto count = [&](int u) {
+                int c = 0;
+                for (int x = 0; x < A.seqs; ++x) {
+                    const int sp = __builtin_amdgcn_readlane(span, x), to = __builtin_amdgcn_readlane(above, x) + sp;
+                    c += clampi(to - u, 0, sp) * __builtin_amdgcn_readlane(each, x);
+                }
+                return c;
+            };
+            // the largest level that has more than `item` items from it on: 64 levels at a time
+            int lo = 0, step = largest(above + span), over = 0;
+            do {
+                step = (step + 63) >> 6;
+                const int c = count(lo + lane * step);
+                const uint64_t past = __ballot(c > item);
+                if (!past) return w;
+                const int l = 63 - __builtin_clzll(past);
+                over = l < 63 ? __builtin_amdgcn_readlane(c, l + 1) : -1;
+                lo += l * step;
+            } while (step > 1);
+            if (over < 0) over = __builtin_amdgcn_readfirstlane(count(lo + 1));
+            item -= over;
+            const int own = (clampi(above + span - lo, 0, span) - clampi(above + span - lo - 1, 0, span)) * each;
+            const int sum = lane_sums(lane < A.seqs ? own : 0);
+            src = __builtin_ctzll(__ballot(sum > item));
+            at = item - __builtin_amdgcn_readlane(sum - own, src);
             w.nc = __builtin_amdgcn_readlane(parts, src);
-            const int from_end = __builtin_amdgcn_readlane(sum, src) - 1 - item;
-            w.tile = split ? from_end / w.nc : from_end;
-            w.chunk = split ? from_end - w.tile * w.nc : 0;
-            // tiles of different sequences apart: a sequence has at most one tile more than its rows divided by BM
-            w.slot = ((int)((int64_t)w.q0 * group / BM) + base + src + w.tile) * S.most;
-            w.live = true;
-            return w;
+            w.tile = A.causal ? lo - __builtin_amdgcn_readlane(above, src) : BYPART && w.nc > 1 ? at / w.nc : at;
+            w.chunk = !BYPART ? 0 : A.causal ? at : at - w.tile * w.nc;
+        } else {
+            const int sum = lane_sums(tiles * nc);
+            const uint64_t past = __ballot(sum > item);
+            if (!past) {
+                item -= __builtin_amdgcn_readlane(sum, 63);
+                continue;
+            }
+            src = __builtin_ctzll(past);
+            w.nc = __builtin_amdgcn_readlane(parts, src);
+            at = __builtin_amdgcn_readlane(sum, src) - 1 - item;
+            w.tile = BYPART && w.nc > 1 ? at / w.nc : at;
+            w.chunk = BYPART ? at - w.tile * w.nc : 0;
         }
-        item -= __builtin_amdgcn_readlane(sum, 63);
+        w.q0 = __builtin_amdgcn_readlane(q0, src);
+        w.n = __builtin_amdgcn_readlane(n, src);
+        w.len = __builtin_amdgcn_readlane(len, src);
+        const uint32_t k_lo = __builtin_amdgcn_readlane((int)(uint32_t)k0, src);
+        const uint32_t k_hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)k0 >> 32), src);
+        w.k0 = (int64_t)(((uint64_t)k_hi << 32) | k_lo);
+        // tiles of different sequences apart: a sequence has at most one tile more than its rows divided by BM
+        w.slot = S.most > 1 ? ((int)((int64_t)w.q0 * group / BM) + base + src + w.tile) * S.most : 0;
+        w.live = true;
+        return w;
     }
     return w;
 }
 
+// rows are numbered query * group + head of the group; exact for every int
+struct Group {
+    int n;
+    double inv;
+    __device__ __forceinline__ int query(int row) const { return (int)(((double)row + 0.5) * inv); }
+};
+
 // the keys that row r of the sequence sees (the last row's where r is past it, so that unused rows need no masks)
-__device__ __forceinline__ int seen(const Work& w, int r, int group, int causal) {
+__device__ __forceinline__ int seen(const Work& w, int r, const Group& group, int causal) {
     if (!causal) return w.len;
-    int i = r / group;
+    int i = __builtin_amdgcn_readfirstlane(group.query(r));
     i = i < w.n ? i : w.n - 1;
     return clampi(w.len - w.n + i + 1, 0, w.len);
 }
 
 // ------------------------------------------------------------------------------------------------ a wave's rows
 // 32 rows of a wave: queries, running statistics and o^T (lane (c, h): row c, dimensions 32 db + 8 i + 4 h + j)
-template <class T, int DP>
+template <class T, int DC>
 struct Rows {
-    typename Mat<T>::v8 q[DP / 16];
-    v16f o[DP / 32];
+    typename Mat<T>::v8 q[DC / 16];
+    v16f o[DC / 32];
     float m, nm, l;  // running maximum (log2 units), its negative (0 where there is none yet), this half's sum
     int lim;         // keys seen
 
-    __device__ __forceinline__ void begin(const AttentionArgs& A, const Work& w, int kvh, int group, int r0) {
-        const int lane = threadIdx.x & 63, r = r0 + (lane & 31), h = lane >> 5;
-        const int i = r / group, hd = kvh * group + (r - i * group);
-        const bool live = i < w.n;
-        const T* x = at<T>(A.q, w.q0 + (live ? i : 0), live ? hd : 0);
+    // row: this lane's in the sequence (past the last one: the last one's again, its result not kept)
+    __device__ __forceinline__ void begin(const AttentionArgs& A, const Work& w, int kvh, const Group& group, int row) {
+        const int h = (threadIdx.x & 63) >> 5;
+        int i = group.query(row), hd = kvh * group.n + (row - i * group.n);
+        if (i >= w.n) i = w.n - 1, hd = kvh * group.n;
+        const T* x = at<T>(A.q, w.q0 + i, hd);
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
+        for (int s = 0; s < DC / 16; ++s) {
             const int d = 16 * s + 8 * h;
-            q[s] = live && d < A.dim ? *(const typename Mat<T>::v8*)(x + d) : (typename Mat<T>::v8)(T)0.0f;
+            if (16 * s + 16 <= A.dim)
+                q[s] = *(const typename Mat<T>::v8*)(x + d);
+            else
+                q[s] = d < A.dim ? *(const typename Mat<T>::v8*)(x + d) : (typename Mat<T>::v8)(T)0.0f;
         }
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) o[d] = (v16f)0.0f;
+        for (int d = 0; d < DC / 32; ++d) o[d] = (v16f)0.0f;
         m = -INFINITY;
         nm = 0;
         l = 0;
-        lim = seen(w, r, group, A.causal);
+        lim = A.causal ? clampi(w.len - w.n + i + 1, 0, w.len) : w.len;
     }
 };
 
-template <class T, int DP, int KT>
+template <class T, int DP, int DC, int KT>
 struct Wave {
     typedef typename Mat<T>::v8 v8;
     static constexpr int NK = KT / 32;
     using L = Tile<DP>;
 
     // scores of KT keys: z[kb] for the keys 32 kb ..
-    static __device__ __forceinline__ void scores(const char PCH_LDS* k, const Rows<T, DP>& R, v16f (&z)[NK]) {
+    static __device__ __forceinline__ void scores(const char PCH_LDS* k, const Rows<T, DC>& R, v16f (&z)[NK]) {
         const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
         const uint32_t row = c * DP * 2;
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb) z[kb] = (v16f)0.0f;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) {
+        for (int s = 0; s < DC / 16; ++s) {
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb) {
                 const v8 a = *(const v8 PCH_LDS*)(k + row + kb * 32 * DP * 2 + (((2 * s + h) ^ L::kswz(c)) << 4));
                 z[kb] = Mat<T>::mul(a, R.q[s], z[kb]);
             }
         }
+        // four readings ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int x = 0; x < NK * DC / 16 - 4; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
     }
 
     // keys from the row's limit on do not count; key0: the tile's first
-    static __device__ __forceinline__ void mask(const Rows<T, DP>& R, int key0, v16f (&z)[NK]) {
+    static __device__ __forceinline__ void mask(const Rows<T, DC>& R, int key0, v16f (&z)[NK]) {
         const int left = R.lim - key0 - 4 * ((threadIdx.x & 63) >> 5);
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
@@ -233,7 +318,7 @@ struct Wave {
 
     // z becomes exp2(c z - m); m follows the largest score where it has grown by more than 8 (2^8 holds in every type, and
     // most tiles then need no rescaling)
-    static __device__ __forceinline__ void softmax(Rows<T, DP>& R, float c, v16f (&z)[NK]) {
+    static __device__ __forceinline__ void softmax(Rows<T, DC>& R, float c, v16f (&z)[NK]) {
         float top = z[0][0];
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
@@ -247,7 +332,7 @@ struct Wave {
             R.nm = mn == -INFINITY ? 0.0f : -mn;
             R.l *= r;
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) R.o[d] *= r;
+            for (int d = 0; d < DC / 32; ++d) R.o[d] *= r;
         }
         float l = 0;
 #pragma unroll
@@ -261,7 +346,7 @@ struct Wave {
     }
 
     // o += p V
-    static __device__ __forceinline__ void values(const char PCH_LDS* v, Rows<T, DP>& R, const v16f (&z)[NK]) {
+    static __device__ __forceinline__ void values(const char PCH_LDS* v, Rows<T, DC>& R, const v16f (&z)[NK]) {
         const int lane = threadIdx.x & 63;
         const int key = 4 * (lane >> 5) + ((lane & 15) >> 2), ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
         const uint32_t at = key * DP * 2 + (lane & 1) * 8;
@@ -272,7 +357,7 @@ struct Wave {
             for (int e = 0; e < 8; ++e) pf[e] = z[s >> 1][8 * (s & 1) + e];
             const v8 p = __builtin_convertvector(pf, v8);
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) {
+            for (int d = 0; d < DC / 32; ++d) {
                 // the swizzle of rows 8 apart is the same
                 const uint32_t x = at + (((4 * d + ch) ^ L::vswz(key)) << 4) + 16 * s * DP * 2;
                 const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s PCH_LDS*)(v + x));
@@ -287,17 +372,17 @@ struct Wave {
     // zero, which is not zero where they are infinite or NaN. If o came out so, o of these keys (from key0 to each row's
     // limit: at most a tile of rows and one of keys) is summed again from memory, key by key, each row its own.
     static __device__ __forceinline__ void repair(const AttentionArgs& A, const Work& w, int kvh, float c, int key0, int key1,
-                                               int step, Rows<T, DP>& R) {
+                                               int step, Rows<T, DC>& R) {
         const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) R.o[d] = (v16f)0.0f;
+        for (int d = 0; d < DC / 32; ++d) R.o[d] = (v16f)0.0f;
         for (int t0 = key0; t0 < key1; t0 += step)
             for (int j = t0; j < t0 + KT && j < key1; ++j) {
                 const T* k = at<T>(A.k, w.k0 + j, kvh);
                 const T* v = at<T>(A.v, w.k0 + j, kvh);
                 float z = 0;
 #pragma unroll
-                for (int s = 0; s < DP / 16; ++s) {
+                for (int s = 0; s < DC / 16; ++s) {
                     if (16 * s + 8 * h < A.dim) {
                         const v8 x = *(const v8*)(k + 16 * s + 8 * h);
 #pragma unroll
@@ -308,7 +393,7 @@ struct Wave {
                 if (j >= R.lim) continue;
                 const float p = (float)(T)__builtin_amdgcn_exp2f(fmaf(z, c, R.nm));
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d)
+                for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int dd = 32 * d + 8 * i + 4 * h;
@@ -320,27 +405,27 @@ struct Wave {
                     }
             }
     }
-    static __device__ __forceinline__ bool broken(const Rows<T, DP>& R) {
+    static __device__ __forceinline__ bool broken(const Rows<T, DC>& R) {
         float x = 0;
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
             for (int e = 0; e < 16; ++e) x = fmaf(R.o[d][e], 0.0f, x);
         return __any(!(x == 0.0f));
     }
 
     // o / l and lse, or (a part of the keys) o, m and l; BM: rows of the tile, row: this lane's in it
-    static __device__ __forceinline__ void finish(const AttentionArgs& A, const Split& S, const Work& w, int kvh, int group,
-                                                  int BM, int row, Rows<T, DP>& R) {
-        const int lane = threadIdx.x & 63, r = w.tile * BM + row, h = lane >> 5;
-        const int i = r / group, hd = kvh * group + (r - i * group);
-        if (i >= w.n) return;
+    static __device__ __forceinline__ void finish(const AttentionArgs& A, const Split& S, const Work& w, int kvh,
+                                                  const Group& group, int BM, int row, Rows<T, DC>& R) {
+        const int h = (threadIdx.x & 63) >> 5, r = w.tile * BM + row;
+        const int i = group.query(r), hd = kvh * group.n + (r - i * group.n);
         const float l = R.l + other(R.l);
         if (w.nc > 1) {
+            if (i >= w.n) return;
             const int slot = (w.slot + w.chunk) * A.kv_heads + kvh;
             float* y = S.sums(slot, BM, A.dim) + (int64_t)row * A.dim;
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d)
+            for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const int dd = 32 * d + 8 * g + 4 * h;
@@ -352,19 +437,25 @@ struct Wave {
         }
         const float inv = R.m == -INFINITY ? 0.0f : 1.0f / l;
         T* y = at<T>(A.out, w.q0 + i, hd);
+        typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int dd = 32 * d + 8 * g + 4 * h;
-                if (dd < A.dim) {
-                    v4f f;
+            for (int g = 0; g < 4; g += 2) {
+                v2u x[2];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[e] = R.o[d][4 * g + e] * inv;
-                    *(typename Mat<T>::v4*)(y + dd) = __builtin_convertvector(f, typename Mat<T>::v4);
+                for (int e = 0; e < 2; ++e) {
+                    const int a = 4 * (g + e);
+                    const v4f f = v4f{R.o[d][a], R.o[d][a + 1], R.o[d][a + 2], R.o[d][a + 3]} * inv;
+                    x[e] = __builtin_bit_cast(v2u, __builtin_convertvector(f, typename Mat<T>::v4));
                 }
+                // the halves of a row hold 4 values each of both groups of 8: after the exchange a lane holds one group
+                const auto a = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
+                const auto b = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+                const int dd = 32 * d + 8 * (g + h);
+                if (i < w.n && dd < A.dim) *(v4u*)(y + dd) = v4u{a[0], b[0], a[1], b[1]};
             }
-        if (A.lse && h == 0)
+        if (A.lse && h == 0 && i < w.n)
             A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = R.m == -INFINITY ? -INFINITY : (R.m + __log2f(l)) * 0.6931471805599453f;
     }
 };
@@ -372,29 +463,25 @@ struct Wave {
 // ------------------------------------------------------------------------------------------------ many rows
 // A workgroup of NW waves takes NW QB 32 rows; a tile of keys and values goes through LDS once for all of them, the next one
 // loaded while this one is used. Tiles run from the last to the first: those that rows see in part come first.
-template <class T, int DP, int QB, int NW>
-__global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, Split S, int group) {
+template <class T, int DP, int DC, int QB, int NW>
+__global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * QB * NW, TB = KT * DP * 2, CPR = DP / 8;
     constexpr int NL = KT * CPR / (64 * NW);  // loads a wave issues for a tile
-    using W = Wave<T, DP, KT>;
+    using W = Wave<T, DP, DC, KT>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int kvh = blockIdx.x % A.kv_heads;
-    const Work w = locate(A, S, blockIdx.x / A.kv_heads, group, BM, true);
+    const int kvh = blockIdx.x;
+    const Work w = locate<true, true>(A, S, blockIdx.z * gridDim.y + blockIdx.y, group.n, BM);
     if (!w.live) return;
-    const int R = w.n * group, r0 = w.tile * BM, mine = r0 + wave * QB * 32;
+    const int R = w.n * group.n, r0 = w.tile * BM, mine = r0 + wave * QB * 32;
     const float c = A.scale * 1.4426950408889634f;
     const int last = r0 + BM < R ? r0 + BM : R;
     const int all = (seen(w, last - 1, group, A.causal) + KT - 1) / KT;
-    const int first = (int)((int64_t)all * w.chunk / w.nc), tiles = (int)((int64_t)all * (w.chunk + 1) / w.nc);
-    Rows<T, DP> rows[QB];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) rows[b].begin(A, w, kvh, group, mine + 32 * b);
-    // this wave's part: keys [0, hi) of which [0, lo) are seen by all its rows
-    const int sees = mine < R ? seen(w, mine + QB * 32 - 1, group, A.causal) : 0;
-    const int hi = sees < tiles * KT ? sees : tiles * KT;
-    const int lo = mine < R ? seen(w, mine, group, A.causal) : 0;
-    const int whole = lo / KT > first ? lo / KT : first;  // the tiles below this one need no mask
+    int first = 0, tiles = all;
+    if (w.nc > 1) {
+        first = (int)((int64_t)all * w.chunk / w.nc);
+        tiles = (int)((int64_t)all * (w.chunk + 1) / w.nc);
+    }
 
     uint32_t ko[NL], vo[NL];
 #pragma unroll
@@ -419,34 +506,50 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
 #pragma unroll
         for (int n = 0; n < NL; ++n) load_lds(rv, to + TB + n * NW * 1024, vo[n]);
     };
-    bool checked = hi <= whole * KT;
     if (tiles > first) load(tiles - 1);
-    for (int t = tiles - 1; t >= first; --t) {
+    Rows<T, DC> rows[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) rows[b].begin(A, w, kvh, group, mine + 32 * b + (lane & 31));
+    // the keys [0, hi) are seen by rows of this wave; tiles below `whole` by every row of the workgroup: they need no mask
+    const int sees = mine < R ? seen(w, mine + QB * 32 - 1, group, A.causal) : 0;
+    const int hi = sees < tiles * KT ? sees : tiles * KT;
+    const int every = seen(w, r0, group, A.causal) / KT;
+    const int whole = clampi(every, first, tiles);
+    const auto turn = [&](int t) {  // tile t is there; the next one on its way
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         if (t > first) load(t - 1);
+        return (const char PCH_LDS*)lds + (t & 1) * 2 * TB;
+    };
+    int t = tiles - 1;
+    for (; t >= whole; --t) {
+        const char PCH_LDS* kl = turn(t);
         if (t * KT >= hi) continue;
-        const char PCH_LDS* kl = (const char PCH_LDS*)lds + (t & 1) * 2 * TB;
-        if (!checked && t < whole) {
-            checked = true;
-            if (A.causal)
-#pragma unroll
-                for (int b = 0; b < QB; ++b)
-                    if (W::broken(rows[b])) W::repair(A, w, kvh, c, whole * KT, hi, KT, rows[b]);
-        }
         v16f z[QB][KT / 32];
 #pragma unroll
         for (int b = 0; b < QB; ++b) {
             W::scores(kl, rows[b], z[b]);
-            if (t >= whole) W::mask(rows[b], t * KT, z[b]);
+            W::mask(rows[b], t * KT, z[b]);
             W::softmax(rows[b], c, z[b]);
         }
 #pragma unroll
         for (int b = 0; b < QB; ++b) W::values(kl + TB, rows[b], z[b]);
     }
-    if (!checked && A.causal)
+    if (A.causal && hi > whole * KT)
 #pragma unroll
         for (int b = 0; b < QB; ++b)
             if (W::broken(rows[b])) W::repair(A, w, kvh, c, whole * KT, hi, KT, rows[b]);
+    for (; t >= first; --t) {
+        const char PCH_LDS* kl = turn(t);
+        if (!hi) continue;
+        v16f z[QB][KT / 32];
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            W::scores(kl, rows[b], z[b]);
+            W::softmax(rows[b], c, z[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < QB; ++b) W::values(kl + TB, rows[b], z[b]);
+    }
 #pragma unroll
     for (int b = 0; b < QB; ++b) W::finish(A, S, w, kvh, group, BM, (wave * QB + b) * 32 + (lane & 31), rows[b]);
 }
@@ -460,28 +563,29 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <class T, int DP, int NW>
-__global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, int group) {
+template <class T, int DP, int DC, int NW>
+__global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = 32, BM = 32, TB = KT * DP * 2, CPR = DP / 8, NL = KT * CPR / 64, PAD = DP + 4;
-    using W = Wave<T, DP, KT>;
+    using W = Wave<T, DP, DC, KT>;
     __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * TB];
     static_assert(NW * 4 * TB >= (NW * BM * PAD + NW * BM * 2) * 4, "the join fits the tiles' memory");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int kvh = blockIdx.x % A.kv_heads;
-    const Work w = locate(A, S, blockIdx.x / A.kv_heads, group, BM, true);
+    const int kvh = blockIdx.x;
+    const Work w = locate<true, true>(A, S, blockIdx.z * gridDim.y + blockIdx.y, group.n, BM);
     if (!w.live) return;
-    const int R = w.n * group, r0 = w.tile * BM;
+    const int R = w.n * group.n, r0 = w.tile * BM;
     const float c = A.scale * 1.4426950408889634f;
     const int rn = R - r0 < BM ? R - r0 : BM;
     const int sees = seen(w, r0 + rn - 1, group, A.causal);
     const int all = (sees + KT - 1) / KT;
-    const int first = (int)((int64_t)all * w.chunk / w.nc), tiles = (int)((int64_t)all * (w.chunk + 1) / w.nc);
+    int first = 0, tiles = all;
+    if (w.nc > 1) {
+        first = (int)((int64_t)all * w.chunk / w.nc);
+        tiles = (int)((int64_t)all * (w.chunk + 1) / w.nc);
+    }
     const int hi = sees < tiles * KT ? sees : tiles * KT;
     const int lo = seen(w, r0, group, A.causal);
     const int whole = lo / KT > first ? lo / KT : first;
-    Rows<T, DP> row;
-    row.begin(A, w, kvh, group, r0);
-
     uint32_t ko[NL], vo[NL];
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
@@ -507,6 +611,9 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, int g
     };
     // this wave's tiles, from the last of those that are `wave` mod NW after the first
     const int mine = tiles - first > wave ? (tiles - first - wave + NW - 1) / NW : 0;
+    if (mine) load(first + wave + (mine - 1) * NW, (mine - 1) & 1);
+    Rows<T, DC> row;
+    row.begin(A, w, kvh, group, r0 + (lane & 31));
     bool unchecked = false;
     const auto mend = [&] {
         unchecked = false;
@@ -515,7 +622,6 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, int g
             W::repair(A, w, kvh, c, (first + wave + skip * NW) * KT, hi, KT * NW, row);
         }
     };
-    if (mine) load(first + wave + (mine - 1) * NW, (mine - 1) & 1);
     for (int u = mine - 1; u >= 0; --u) {
         const int t = first + wave + u * NW;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last tile's reads are done: its memory takes the next one
@@ -558,7 +664,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, int g
     if (h == 0) st[NW * BM + wave * BM + cc] = l * f;
     if (cc < rn)
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
+        for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
             for (int g = 0; g < 4; ++g)
                 *(v4f PCH_LDS*)(sh + (wave * BM + cc) * PAD + 32 * d + 8 * g + 4 * h) =
@@ -580,7 +686,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, int g
             *(v4f*)(S.sums(slot, BM, A.dim) + r * A.dim + d) = o;
             if (d == 0) *(float2*)(S.stats(slot, BM, A.dim) + r * 2) = make_float2(mr, lr);
         } else {
-            const int i = (r0 + r) / group, hd = kvh * group + (r0 + r - i * group);
+            const int i = group.query(r0 + r), hd = kvh * group.n + (r0 + r - i * group.n);
             const float inv = mr == -INFINITY ? 0.0f : 1.0f / lr;
             *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
             if (A.lse && d == 0)
@@ -591,30 +697,62 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, int g
 }
 
 // ------------------------------------------------------------------------------------------------ parts of the keys joined
-// A workgroup per tile of rows and key head, a thread per row and 4 dimensions: the parts in their order, each scaled to the
-// largest maximum.
-template <class T>
-__global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, int group, int BM) {
-    const int kvh = blockIdx.x % A.kv_heads;
-    const Work w = locate(A, S, blockIdx.x / A.kv_heads, group, BM, false);
+// 32 lanes of 4 dimensions to a row; PL lanes of parts, each merging every PL-th part, then the PL in their order; 8 / PL rows
+// to a workgroup. Reading the parts is all there is to do, so they are read in parallel: one
+// thread after the other through 128 parts took 120 us where this takes 4.
+template <class T, int PL>
+__global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, Group group, int BM) {
+    __shared__ v4f so[8][33];
+    __shared__ float2 ss[8];
+    const int blocks = BM * PL / 8, kvh = blockIdx.x / blocks, rb = blockIdx.x - kvh * blocks;
+    const Work w = locate<false, false>(A, S, blockIdx.z * gridDim.y + blockIdx.y, group.n, BM);
     if (!w.live || w.nc == 1) return;
-    const int R = w.n * group, r0 = w.tile * BM, rn = R - r0 < BM ? R - r0 : BM, q4 = A.dim >> 2;
-    for (int x = blockIdx.y * 256 + threadIdx.x; x < rn * q4; x += 256 * gridDim.y) {
-        const int r = x / q4, d = (x - r * q4) * 4;
-        float m = -INFINITY;
-        for (int p = 0; p < w.nc; ++p) m = fmaxf(m, S.stats((w.slot + p) * A.kv_heads + kvh, BM, A.dim)[r * 2]);
-        float l = 0;
+    const int q = threadIdx.x >> 5, pl = q % PL, dl = threadIdx.x & 31;
+    const int R = w.n * group.n, r0 = w.tile * BM, rn = R - r0 < BM ? R - r0 : BM, r = rb * (8 / PL) + q / PL;
+    const int64_t step = (int64_t)A.kv_heads * BM;
+    for (int d0 = 0; d0 < A.dim; d0 += 128) {
+        const int d = d0 + 4 * dl;
+        const float* y = S.sums(w.slot * A.kv_heads + kvh, BM, A.dim) + (int64_t)r * A.dim + d;
+        const float* st = S.stats(w.slot * A.kv_heads + kvh, BM, A.dim) + r * 2;
+        float m = -INFINITY, l = 0;
         v4f o = (v4f)0.0f;
-        for (int p = 0; p < w.nc; ++p) {
-            const int slot = (w.slot + p) * A.kv_heads + kvh;
-            const float2 st = *(const float2*)(S.stats(slot, BM, A.dim) + r * 2);
-            const v4f y = *(const v4f*)(S.sums(slot, BM, A.dim) + (int64_t)r * A.dim + d);
-            if (st.x == -INFINITY) continue;
-            const float f = __builtin_amdgcn_exp2f(st.x - m);
-            l = fmaf(st.y, f, l);
-            o += y * f;
+        for (int p0 = pl; r < rn && p0 < w.nc; p0 += 4 * PL) {  // four parts at a time on their way
+            float2 x[4];
+            v4f z[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int p = p0 + PL * u;
+                const bool in = p < w.nc;
+                x[u] = in ? *(const float2*)(st + p * step * 2) : make_float2(-INFINITY, 0);
+                z[u] = in && d < A.dim ? *(const v4f*)(y + p * step * A.dim) : (v4f)0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (x[u].x == -INFINITY) continue;
+                const float mn = fmaxf(m, x[u].x), a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(x[u].x - mn);
+                m = mn;
+                l = l * a + x[u].y * b;
+                o = o * a + z[u] * b;
+            }
         }
-        const int i = (r0 + r) / group, hd = kvh * group + (r0 + r - i * group);
+        if (PL > 1) {
+            __syncthreads();
+            so[q][dl] = o;
+            if (dl == 0) ss[q] = make_float2(m, l);
+            __syncthreads();
+            if (pl == 0) {
+                for (int p = 1; p < PL; ++p) m = fmaxf(m, ss[q + p].x);
+                l = 0;
+                o = (v4f)0.0f;
+                for (int p = 0; p < PL; ++p) {
+                    const float f = ss[q + p].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ss[q + p].x - m);
+                    l = fmaf(ss[q + p].y, f, l);
+                    o += so[q + p][dl] * f;
+                }
+            }
+        }
+        if (pl || r >= rn || d >= A.dim) continue;
+        const int i = group.query(r0 + r), hd = kvh * group.n + (r0 + r - i * group.n);
         const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
         *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
         if (A.lse && d == 0)
@@ -655,49 +793,55 @@ static uint64_t work_bytes(const AttentionArgs& a, const Choice& c) {
     return c.most > 1 ? (uint64_t)c.items * c.most * a.kv_heads * c.BM * (a.dim + 2) * 4 : 0;
 }
 
-#ifndef PCH_WANT
-#define PCH_WANT 1024
-#endif
 static Choice choose(const AttentionArgs& a) {
     const int group = a.heads / a.kv_heads;
     Choice c;
     c.few = (int64_t)a.max_q * group <= 32;
     c.BM = c.few ? 32 : 128;
     c.items = (int64_t)a.tokens * group / c.BM + a.seqs;
-    const int64_t want = PCH_WANT;
-    const int64_t base = c.items * a.kv_heads;
-    const int64_t shortest = 256;  // keys of a part at least
-    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / shortest));
-    c.size = (a.max_k + c.most - 1) / std::max(1, c.most);
+    // the tiles there are likely to be: one for each sequence of few rows
+    const int64_t base = (c.few ? a.seqs : c.items) * a.kv_heads;
+    const int64_t want = c.few ? 256 : 1024;
+    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / 512));
+    c.size = (a.max_k + c.most - 1) / c.most;
     return c;
 }
 
-template <class T, int DP>
+template <class T, int DP, int DC>
 static int run_t(const AttentionArgs& a, hipStream_t s) {
     const int group = a.heads / a.kv_heads;
     Choice c = choose(a);
     while (c.most > 1 && work_bytes(a, c) > (a.work ? a.work_bytes : 0)) c.most = c.most / 2;
     if (c.most > 1) c.size = (a.max_k + c.most - 1) / c.most;
-    const int64_t blocks = c.items * c.most * a.kv_heads;
-    if (blocks > 0x7fffffff) return -2;
+    const Group g = {group, 1.0 / group};
+    const int64_t tall = c.items * c.most, high = std::min<int64_t>(tall, 65535), deep = (tall + high - 1) / high;
+    if (deep > 65535) return -2;
+    const dim3 grid((unsigned)a.kv_heads, (unsigned)high, (unsigned)deep);
     const Split S = {c.most, c.size, (float*)a.work, c.items * c.most * a.kv_heads};
     constexpr int NW = DP > 128 ? 2 : 4;
     if (c.few)
-        hipLaunchKernelGGL((few_k<T, DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, a, S, group);
+        hipLaunchKernelGGL((few_k<T, DP, DC, NW>), grid, dim3(64 * NW), 0, s, a, S, g);
     else
-        hipLaunchKernelGGL((rows_k<T, DP, 1, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a, S, group);
+        hipLaunchKernelGGL((rows_k<T, DP, DC, 1, 4>), grid, dim3(256), 0, s, a, S, g);
     if (c.most > 1) {
         if (int e = launch_rc()) return e;
-        hipLaunchKernelGGL(join_k<T>, dim3((unsigned)(c.items * a.kv_heads), c.few ? 1 : 8), dim3(256), 0, s, a, S, group, c.BM);
+        const int64_t jh = std::min<int64_t>(c.items, 65535), jd = (c.items + jh - 1) / jh;
+        const dim3 jg((unsigned)(a.kv_heads * (c.few ? c.BM : c.BM / 8)), (unsigned)jh, (unsigned)jd);
+        if (c.few)
+            hipLaunchKernelGGL((join_k<T, 8>), jg, dim3(256), 0, s, a, S, g, c.BM);
+        else
+            hipLaunchKernelGGL((join_k<T, 1>), jg, dim3(256), 0, s, a, S, g, c.BM);
     }
     return launch_rc();
 }
 
 template <class T>
 static int run(const AttentionArgs& a, hipStream_t s) {
-    if (a.dim <= 64) return run_t<T, 64>(a, s);
-    if (a.dim <= 128) return run_t<T, 128>(a, s);
-    return run_t<T, 256>(a, s);
+    if (a.dim <= 64) return run_t<T, 64, 64>(a, s);
+    if (a.dim <= 96) return run_t<T, 128, 96>(a, s);
+    if (a.dim <= 128) return run_t<T, 128, 128>(a, s);
+    if (a.dim <= 192) return run_t<T, 256, 192>(a, s);
+    return run_t<T, 256, 256>(a, s);
 }
 
 }  // namespace clear
