@@ -76,6 +76,11 @@ __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t lds,
         : "memory");
 }
 
+// log of a row's sum l of exp2(. - m), in natural units; no key: l = 0 gives -infinity
+__device__ __forceinline__ float logsum(float m, float l) {
+    return l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+}
+
 __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
     return ((uint64_t)hi << 32) | lo;
@@ -283,6 +288,7 @@ struct Wave {
     using L = Tile<DP>;
 
     // scores of KT keys: z[kb] for the keys 32 kb ..
+    template <bool ALONE = true>
     static __device__ __forceinline__ void scores(const char PCH_LDS* k, const Rows<T, DC>& R, v16f (&z)[NK]) {
         const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
         const uint32_t row = c * DP * 2;
@@ -297,6 +303,7 @@ struct Wave {
             }
         }
         // four readings ahead of the products
+        if (!ALONE) return;
         __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
 #pragma unroll
         for (int x = 0; x < NK * DC / 16 - 4; ++x) {
@@ -313,17 +320,27 @@ struct Wave {
         for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
+            {
                 if (32 * kb + 8 * (e >> 2) + (e & 3) >= left) z[kb][e] = -INFINITY;
+                if ((e & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // not all comparisons at once: they would not fit
+            }
     }
 
     // z becomes exp2(c z - m); m follows the largest score where it has grown by more than 8 (2^8 holds in every type, and
     // most tiles then need no rescaling)
     static __device__ __forceinline__ void softmax(Rows<T, DC>& R, float c, v16f (&z)[NK]) {
+        grow(R, c, largest_of(z));
+        weigh(R, c, z);
+    }
+    static __device__ __forceinline__ float largest_of(const v16f (&z)[NK]) {
         float top = z[0][0];
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, z[kb][e]);
+        return top;
+    }
+    static __device__ __forceinline__ void grow(Rows<T, DC>& R, float c, float top) {
         top = fmaxf(top, other(top)) * c;
         if (__any(top > R.m + 8.0f)) {
             const float mn = fmaxf(R.m, top);
@@ -334,6 +351,8 @@ struct Wave {
 #pragma unroll
             for (int d = 0; d < DC / 32; ++d) R.o[d] *= r;
         }
+    }
+    static __device__ __forceinline__ void weigh(Rows<T, DC>& R, float c, v16f (&z)[NK]) {
         float l = 0;
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
@@ -406,12 +425,12 @@ struct Wave {
             }
     }
     static __device__ __forceinline__ bool broken(const Rows<T, DC>& R) {
-        float x = 0;
+        float x[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x = fmaf(R.o[d][e], 0.0f, x);
-        return __any(!(x == 0.0f));
+            for (int e = 0; e < 16; ++e) x[e & 3] = fmaf(R.o[d][e], 0.0f, x[e & 3]);
+        return __any(!((x[0] + x[1]) + (x[2] + x[3]) == 0.0f));
     }
 
     // o / l and lse, or (a part of the keys) o, m and l; BM: rows of the tile, row: this lane's in it
@@ -435,7 +454,7 @@ struct Wave {
             if (h == 0) *(float2*)(S.stats(slot, BM, A.dim) + row * 2) = make_float2(R.m, l);
             return;
         }
-        const float inv = R.m == -INFINITY ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         T* y = at<T>(A.out, w.q0 + i, hd);
         typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 #pragma unroll
@@ -456,24 +475,24 @@ struct Wave {
                 if (i < w.n && dd < A.dim) *(v4u*)(y + dd) = v4u{a[0], b[0], a[1], b[1]};
             }
         if (A.lse && h == 0 && i < w.n)
-            A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = R.m == -INFINITY ? -INFINITY : (R.m + __log2f(l)) * 0.6931471805599453f;
+            A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = logsum(R.m, l);
     }
 };
 
 // ------------------------------------------------------------------------------------------------ many rows
 // A workgroup of NW waves takes NW QB 32 rows; a tile of keys and values goes through LDS once for all of them, the next one
 // loaded while this one is used. Tiles run from the last to the first: those that rows see in part come first.
-template <class T, int DP, int DC, int QB, int NW>
+template <class T, int DP, int DC, int NW>
 __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, Split S, Group group) {
-    constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * QB * NW, TB = KT * DP * 2, CPR = DP / 8;
-    constexpr int NL = KT * CPR / (64 * NW);  // loads a wave issues for a tile
+    constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * NW, TB = KT * DP * 2, CPR = DP / 8, NK = KT / 32;
+    constexpr int NL = KT * CPR / (64 * NW);  // loads a wave issues for a tile of keys, or of values
     using W = Wave<T, DP, DC, KT>;
     __shared__ __attribute__((aligned(1024))) char lds[4 * TB];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int kvh = blockIdx.x;
     const Work w = locate<true, true>(A, S, blockIdx.z * gridDim.y + blockIdx.y, group.n, BM);
     if (!w.live) return;
-    const int R = w.n * group.n, r0 = w.tile * BM, mine = r0 + wave * QB * 32;
+    const int R = w.n * group.n, r0 = w.tile * BM, mine = r0 + wave * 32;
     const float c = A.scale * 1.4426950408889634f;
     const int last = r0 + BM < R ? r0 + BM : R;
     const int all = (seen(w, last - 1, group, A.causal) + KT - 1) / KT;
@@ -491,67 +510,80 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
         ko[n] = ck * 8 < A.dim ? key * (uint32_t)A.k.token * 2 + ck * 16 : 0x7ffffff0u;
         vo[n] = cv * 8 < A.dim ? key * (uint32_t)A.v.token * 2 + cv * 16 : 0x7ffffff0u;
     }
-    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds;
+    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 1024;
     const char* kp = (const char*)uniform64((uint64_t)at<T>(A.k, w.k0, kvh));
     const char* vp = (const char*)uniform64((uint64_t)at<T>(A.v, w.k0, kvh));
-    auto load = [&](int t) {
+    const auto load = [&](const char* p, int64_t token, int t, uint32_t to, const uint32_t (&off)[NL]) {
         const int left = w.len - t * KT, nr = (left < KT ? left : KT) - 1;
-        const uint32_t to = base + (t & 1) * 2 * TB + wave * 1024;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)t * KT * A.k.token * 2), 0,
-                                                          (nr * (int)A.k.token + A.dim) * 2, 0x00020000);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + (int64_t)t * KT * A.v.token * 2), 0,
-                                                          (nr * (int)A.v.token + A.dim) * 2, 0x00020000);
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)t * KT * token * 2), 0,
+                                                         (nr * (int)token + A.dim) * 2, 0x00020000);
 #pragma unroll
-        for (int n = 0; n < NL; ++n) load_lds(rk, to + n * NW * 1024, ko[n]);
-#pragma unroll
-        for (int n = 0; n < NL; ++n) load_lds(rv, to + TB + n * NW * 1024, vo[n]);
+        for (int n = 0; n < NL; ++n) load_lds(r, to + n * NW * 1024, off[n]);
     };
-    if (tiles > first) load(tiles - 1);
-    Rows<T, DC> rows[QB];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) rows[b].begin(A, w, kvh, group, mine + 32 * b + (lane & 31));
+    const auto load_k = [&](int t) {
+        if (t >= first) load(kp, A.k.token, t, base + (t & 1) * TB, ko);
+    };
+    const auto load_v = [&](int t) {
+        if (t >= first) load(vp, A.v.token, t, base + (2 + (t & 1)) * TB, vo);
+    };
+    const auto arrived = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    const auto keys = [&](int t) { return (const char PCH_LDS*)lds + (t & 1) * TB; };
+    const auto values = [&](int t) { return (const char PCH_LDS*)lds + (2 + (t & 1)) * TB; };
+    if (tiles > first) {
+        load_k(tiles - 1);
+        load_v(tiles - 1);
+        load_k(tiles - 2);
+    }
+    Rows<T, DC> row;
+    row.begin(A, w, kvh, group, mine + (lane & 31));
     // the keys [0, hi) are seen by rows of this wave; tiles below `whole` by every row of the workgroup: they need no mask
-    const int sees = mine < R ? seen(w, mine + QB * 32 - 1, group, A.causal) : 0;
+    const int sees = mine < R ? seen(w, mine + 31, group, A.causal) : 0;
     const int hi = sees < tiles * KT ? sees : tiles * KT;
     const int every = seen(w, r0, group, A.causal) / KT;
     const int whole = clampi(every, first, tiles);
-    const auto turn = [&](int t) {  // tile t is there; the next one on its way
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t > first) load(t - 1);
-        return (const char PCH_LDS*)lds + (t & 1) * 2 * TB;
-    };
+
+    // z: the scores of tile t, made while tile t + 1 was worked on
+    v16f z[NK], zn[NK];
     int t = tiles - 1;
+    arrived();
+    if (t >= first && t * KT < hi) W::scores(keys(t), row, z);
     for (; t >= whole; --t) {
-        const char PCH_LDS* kl = turn(t);
-        if (t * KT >= hi) continue;
-        v16f z[QB][KT / 32];
-#pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            W::scores(kl, rows[b], z[b]);
-            W::mask(rows[b], t * KT, z[b]);
-            W::softmax(rows[b], c, z[b]);
+        arrived();
+        load_k(t - 2);
+        load_v(t - 1);
+        if (t > first && (t - 1) * KT < hi) W::scores(keys(t - 1), row, zn);
+        if (t * KT < hi) {
+            W::mask(row, t * KT, z);
+            W::softmax(row, c, z);
+            W::values(values(t), row, z);
         }
 #pragma unroll
-        for (int b = 0; b < QB; ++b) W::values(kl + TB, rows[b], z[b]);
+        for (int kb = 0; kb < NK; ++kb) z[kb] = zn[kb];
     }
-    if (A.causal && hi > whole * KT)
-#pragma unroll
-        for (int b = 0; b < QB; ++b)
-            if (W::broken(rows[b])) W::repair(A, w, kvh, c, whole * KT, hi, KT, rows[b]);
-    for (; t >= first; --t) {
-        const char PCH_LDS* kl = turn(t);
+    if (A.causal && hi > whole * KT && W::broken(row)) W::repair(A, w, kvh, c, whole * KT, hi, KT, row);
+    float top = hi ? W::largest_of(z) : 0;
+    for (; t > first; --t) {
+        arrived();
+        load_k(t - 2);
+        load_v(t - 1);
         if (!hi) continue;
-        v16f z[QB][KT / 32];
+        W::grow(row, c, top);
+        W::template scores<false>(keys(t - 1), row, zn);
+        W::weigh(row, c, z);
+        W::values(values(t), row, z);
+        top = W::largest_of(zn);
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            W::scores(kl, rows[b], z[b]);
-            W::softmax(rows[b], c, z[b]);
-        }
-#pragma unroll
-        for (int b = 0; b < QB; ++b) W::values(kl + TB, rows[b], z[b]);
+        for (int kb = 0; kb < NK; ++kb) z[kb] = zn[kb];
     }
-#pragma unroll
-    for (int b = 0; b < QB; ++b) W::finish(A, S, w, kvh, group, BM, (wave * QB + b) * 32 + (lane & 31), rows[b]);
+    if (t == first) {
+        arrived();
+        if (hi) {
+            W::grow(row, c, top);
+            W::weigh(row, c, z);
+            W::values(values(t), row, z);
+        }
+    }
+    W::finish(A, S, w, kvh, group, BM, wave * 32 + (lane & 31), row);
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -660,7 +692,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     float m = -INFINITY;
 #pragma unroll
     for (int x = 0; x < NW; ++x) m = fmaxf(m, st[x * BM + cc]);
-    const float f = row.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(row.m - m);
+    const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(row.m - m);
     if (h == 0) st[NW * BM + wave * BM + cc] = l * f;
     if (cc < rn)
 #pragma unroll
@@ -687,11 +719,10 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
             if (d == 0) *(float2*)(S.stats(slot, BM, A.dim) + r * 2) = make_float2(mr, lr);
         } else {
             const int i = group.query(r0 + r), hd = kvh * group.n + (r0 + r - i * group.n);
-            const float inv = mr == -INFINITY ? 0.0f : 1.0f / lr;
+            const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
             *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
             if (A.lse && d == 0)
-                A.lse[(int64_t)(w.q0 + i) * A.heads + hd] =
-                    mr == -INFINITY ? -INFINITY : (mr + __log2f(lr)) * 0.6931471805599453f;
+                A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = logsum(mr, lr);
         }
     }
 }
@@ -728,7 +759,7 @@ __global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, Group gr
             }
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                if (x[u].x == -INFINITY) continue;
+                if (x[u].y == 0.0f) continue;  // no key
                 const float mn = fmaxf(m, x[u].x), a = __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(x[u].x - mn);
                 m = mn;
                 l = l * a + x[u].y * b;
@@ -745,7 +776,7 @@ __global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, Group gr
                 l = 0;
                 o = (v4f)0.0f;
                 for (int p = 0; p < PL; ++p) {
-                    const float f = ss[q + p].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ss[q + p].x - m);
+                    const float f = ss[q + p].y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(ss[q + p].x - m);
                     l = fmaf(ss[q + p].y, f, l);
                     o += so[q + p][dl] * f;
                 }
@@ -753,10 +784,9 @@ __global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, Group gr
         }
         if (pl || r >= rn || d >= A.dim) continue;
         const int i = group.query(r0 + r), hd = kvh * group.n + (r0 + r - i * group.n);
-        const float inv = m == -INFINITY ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
-        if (A.lse && d == 0)
-            A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = m == -INFINITY ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
+        if (A.lse && d == 0) A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = logsum(m, l);
     }
 }
 
@@ -796,13 +826,14 @@ static uint64_t work_bytes(const AttentionArgs& a, const Choice& c) {
 static Choice choose(const AttentionArgs& a) {
     const int group = a.heads / a.kv_heads;
     Choice c;
-    c.few = (int64_t)a.max_q * group <= 32;
+    const int64_t rows = (int64_t)a.max_q * group, tiles = (int64_t)a.tokens * group / 128 + a.seqs;
+    c.few = rows <= 64 || (a.dim <= 64 && tiles * a.kv_heads < 256);
     c.BM = c.few ? 32 : 128;
     c.items = (int64_t)a.tokens * group / c.BM + a.seqs;
-    // the tiles there are likely to be: one for each sequence of few rows
-    const int64_t base = (c.few ? a.seqs : c.items) * a.kv_heads;
-    const int64_t want = c.few ? 256 : 1024;
-    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / 512));
+    // the tiles there are likely to be
+    const int64_t base = (rows <= c.BM ? a.seqs : c.items) * a.kv_heads;
+    const int64_t want = c.few ? 256 : 512;
+    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / 384));
     c.size = (a.max_k + c.most - 1) / c.most;
     return c;
 }
@@ -822,7 +853,7 @@ static int run_t(const AttentionArgs& a, hipStream_t s) {
     if (c.few)
         hipLaunchKernelGGL((few_k<T, DP, DC, NW>), grid, dim3(64 * NW), 0, s, a, S, g);
     else
-        hipLaunchKernelGGL((rows_k<T, DP, DC, 1, 4>), grid, dim3(256), 0, s, a, S, g);
+        hipLaunchKernelGGL((rows_k<T, DP, DC, 4>), grid, dim3(256), 0, s, a, S, g);
     if (c.most > 1) {
         if (int e = launch_rc()) return e;
         const int64_t jh = std::min<int64_t>(c.items, 65535), jd = (c.items + jh - 1) / jh;

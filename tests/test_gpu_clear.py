@@ -271,6 +271,18 @@ def test_attention_unseen_values_do_not_reach_a_query(ops, dim, heads, kv, spans
     run_attention(ops, "bf16", dim, heads, kv, spans, True, edit=edit)
 
 
+@pytest.mark.parametrize("dim,heads,kv,spans", [(128, 4, 2, [(5, 900)]), (64, 2, 2, [(1, 40), (2, 3000)]), (128, 4, 4, [(200, 200)])])
+def test_attention_of_nan_queries(ops, dim, heads, kv, spans):
+    """a query of NaN has NaN for its sums and no finite log: its neighbours in the tile and the split do not"""
+    say(f"[clear] attention with a NaN query, dim {dim} {spans}")
+
+    def edit(q, k, v, k0):
+        q[0, 0] = np.nan
+
+    got = run_attention(ops, "bf16", dim, heads, kv, spans, True, edit=edit)
+    assert np.isnan(got[0, 0]).all() and not np.isnan(got[0, 1:]).any()
+
+
 def test_attention_large_scores(ops):
     """scores in the thousands: one key takes the whole weight, each f32 exponential's argument stays exact enough"""
     say("[clear] attention, scores up to thousands; growing maxima")
