@@ -116,3 +116,62 @@ def score_streams(lanes, cts, pts, top, outs, main, radix_bits=RADIX_BITS):
         ends.append(e)
     for e in ends:
         main.wait(e)
+
+
+class ClearBlock:
+    """One attention block's clear side for a program that scores against encrypted keys: it makes the queries and keys of a
+    public prompt and of the tokens after it (norms, rotation, the cache), and the attention in the clear that decrypted
+    scores are held against. `rows` are the block's projected rows, an Array (or another library's device tensor) [tokens]
+    [heads + 2 kv_heads][dim]: queries, then keys, then values. One sequence of up to `capacity` tokens; nothing is
+    synchronised or allocated after the constructor."""
+
+    def __init__(self, ops, heads, kv_heads, dim, capacity, dtype="bf16", table=None, layout="half", q_weight=None,
+                 k_weight=None, eps=1e-6):
+        from .clear import Array
+
+        self.ops, self.heads, self.kv_heads, self.dim, self.capacity = ops, heads, kv_heads, dim, capacity
+        self.table, self.layout, self.q_weight, self.k_weight, self.eps = table, layout, q_weight, k_weight, eps
+        self.k, self.v = (Array((capacity, kv_heads, dim), dtype) for _ in range(2))
+        self.q, self.out = (Array((capacity, heads, dim), dtype) for _ in range(2))
+        self.lse = Array((capacity, heads), "f32")
+        places = np.arange(capacity, dtype=np.int64)
+        # every length the cache takes: a step points at its own, so that no call uploads anything
+        self._places, self._slots = Array.of(places, "i32"), Array.of(places, "i64")
+        self._runs = Array.of(np.stack([np.zeros(capacity + 1), np.arange(capacity + 1)], 1), "i32")
+        self._first = Array.of(np.zeros(1), "i64")
+        self.length = 0
+
+    def _rows(self, x, first, count):
+        from .clear import Array, SIZES
+
+        step = x._strides[0] * SIZES[x.dtype]
+        return Array((count,) + x.shape[1:], x.dtype, x.buf, x.offset + first * step // 4, x._strides)
+
+    def append(self, rows, causal=True):
+        """The next tokens' rows into the cache, and their attention over all of it: (q, out, lse) of these tokens, views of
+        the block's buffers. A whole prompt, a chunk of one, or one token."""
+        from .clear import Array
+
+        n, at = rows.shape[0], self.length
+        if n < 1 or at + n > self.capacity:
+            raise ValueError(f"{n} tokens after {at}: the block holds {self.capacity}")
+        H, KV = self.heads, self.kv_heads
+        if rows.shape[1] != H + 2 * KV or rows.shape[2] != self.dim:
+            raise ValueError("rows: [tokens][heads + 2 kv_heads][dim]")
+        part = rows.heads if isinstance(rows, Array) else lambda a, c: rows[:, a:a + c]
+        q, out = self._rows(self.q, at, n), self._rows(self.out, at, n)
+        lse = Array((n, H), "f32", self.lse.buf, at * H)
+        self.ops.qk_norm_rotary(part(0, H), part(H, KV), self.q_weight, self.k_weight,
+                                None if self.table is None else Array((n,), "i32", self._places.buf, at), self.table, q,
+                                self.k, eps=self.eps, layout=self.layout, v=part(H + KV, KV), v_out=self.v,
+                                slots=Array((n,), "i64", self._slots.buf, 2 * at))
+        self.length = at + n
+        runs = self._runs.buf  # (0, n) for every n: a run's start and end, or its second alone as a length
+        self.ops.attention(q, self.k, self.v, Array((2,), "i32", runs, 2 * n), self._first,
+                           Array((1,), "i32", runs, 2 * self.length + 1), out, lse, causal=causal, max_q=n,
+                           max_k=self.length)
+        return q, out, lse
+
+    def keys(self):
+        """The cached keys on the host, float32 [length][kv_heads dim]: what key_slots packs for encryption."""
+        return self.k.numpy(self.ops.stream)[:self.length].reshape(self.length, -1)
