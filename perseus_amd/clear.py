@@ -250,6 +250,8 @@ class Clear:
     def __init__(self, stream, workspace=64 << 20):
         self.stream = stream
         self.work = DevBuf(-(-int(workspace) // 4)) if workspace else None
+        if workspace:
+            self.work.zero()  # the counters of split attention: zero before the first call, and left so by every call
         self._work = (self.work.ptr.value, 4 * self.work.words) if workspace else (0, 0)
 
     def rotary(self, x, positions, table, out, layout="half", inverse=False):

@@ -101,7 +101,8 @@ struct Work {
 // caller expected only make the parts longer.
 struct Split {
     int most, size;
-    float* work;  // [slot][BM][dim] sums, then [slot][BM][2] maxima and weights' sums
+    int* arrived;  // [tile][kv head] parts that are done, zero between calls; null: join_k joins them
+    float* work;   // [slot][BM][dim] sums, then [slot][BM][2] maxima and weights' sums
     int64_t slots;
     __device__ __forceinline__ int parts(int len) const {
         if (most <= 1) return 1;
@@ -595,6 +596,18 @@ __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
+constexpr int AT_ONCE = 16;  // parts at most that a workgroup of few_k joins, all on their way at once
+
+// two floats through the caches of this XCD to memory, and from there
+__device__ __forceinline__ void through(float* p, float x, float y) {
+    __hip_atomic_store((uint64_t*)p, (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 past(const float* p) {
+    const uint64_t v = __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
 template <class T, int DP, int DC, int NW>
 __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = 32, BM = 32, TB = KT * DP * 2, CPR = DP / 8, NL = KT * CPR / 64, PAD = DP + 4;
@@ -704,6 +717,12 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     __syncthreads();
     const int slot = (w.slot + w.chunk) * A.kv_heads + kvh;
     const int q4 = A.dim >> 2;
+    const auto store = [&](int r, int d, v4f o, float mr, float lr) {
+        const int i = group.query(r0 + r), hd = kvh * group.n + (r0 + r - i * group.n);
+        const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
+        *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
+        if (A.lse && d == 0) A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = logsum(mr, lr);
+    };
     for (int x = threadIdx.x; x < rn * q4; x += 64 * NW) {
         const int r = x / q4, d = (x - r * q4) * 4;
         v4f o = *(const v4f PCH_LDS*)(sh + r * PAD + d);
@@ -715,15 +734,59 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
             mr = fmaxf(mr, st[y * BM + r]);
         }
         if (w.nc > 1) {
-            *(v4f*)(S.sums(slot, BM, A.dim) + r * A.dim + d) = o;
-            if (d == 0) *(float2*)(S.stats(slot, BM, A.dim) + r * 2) = make_float2(mr, lr);
+            float* const y = S.sums(slot, BM, A.dim) + r * A.dim + d;
+            float* const ml = S.stats(slot, BM, A.dim) + r * 2;
+            if (S.arrived) {
+                through(y, o[0], o[1]);
+                through(y + 2, o[2], o[3]);
+                if (d == 0) through(ml, mr, lr);
+            } else {
+                *(v4f*)y = o;
+                if (d == 0) *(float2*)ml = make_float2(mr, lr);
+            }
         } else {
-            const int i = group.query(r0 + r), hd = kvh * group.n + (r0 + r - i * group.n);
-            const float inv = lr == 0.0f ? 0.0f : 1.0f / lr;
-            *(typename Mat<T>::v4*)(at<T>(A.out, w.q0 + i, hd) + d) = __builtin_convertvector(o * inv, typename Mat<T>::v4);
-            if (A.lse && d == 0)
-                A.lse[(int64_t)(w.q0 + i) * A.heads + hd] = logsum(mr, lr);
+            store(r, d, o, mr, lr);
         }
+    }
+    if (w.nc == 1 || !S.arrived) return;
+
+    // The part that is done last joins them all, in their order whatever order they were done in, where that is quicker than
+    // join_k's launch. The sums go through the caches to memory that all XCDs see, and are there before the part is counted.
+    __shared__ int last;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    int* const counter = S.arrived + w.slot / S.most * A.kv_heads + kvh;
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == w.nc - 1;
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int64_t step = (int64_t)A.kv_heads * BM;
+    for (int x = threadIdx.x; x < rn * q4; x += 64 * NW) {
+        const int r = x / q4, d = (x - r * q4) * 4;
+        const float* y = S.sums(w.slot * A.kv_heads + kvh, BM, A.dim) + (int64_t)r * A.dim + d;
+        const float* s2 = S.stats(w.slot * A.kv_heads + kvh, BM, A.dim) + r * 2;
+        float mr = -INFINITY, lr = 0;
+        v4f o = (v4f)0.0f;
+        float2 a[AT_ONCE];
+        v4f z[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int p = u < w.nc ? u : 0;
+            const float* const g = y + p * step * A.dim;
+            a[u] = past(s2 + p * step * 2);
+            const float2 lo = past(g), hi = past(g + 2);
+            z[u] = v4f{lo.x, lo.y, hi.x, hi.y};
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            if (u >= w.nc || a[u].y == 0.0f) continue;  // no such part, or no key in it
+            const float mn = fmaxf(mr, a[u].x), f = __builtin_amdgcn_exp2f(mr - mn), g = __builtin_amdgcn_exp2f(a[u].x - mn);
+            mr = mn;
+            lr = lr * f + a[u].y * g;
+            o = o * f + z[u] * g;
+        }
+        store(r, d, o, mr, lr);
     }
 }
 
@@ -812,6 +875,8 @@ static int checked(const AttentionArgs* a) {
     return 0;
 }
 
+constexpr int COUNTERS = PCX_ATTENTION_COUNTERS;
+
 // the kernel and the split of a call
 struct Choice {
     int few;      // few_k, else rows_k
@@ -820,7 +885,7 @@ struct Choice {
     int most, size;
 };
 static uint64_t work_bytes(const AttentionArgs& a, const Choice& c) {
-    return c.most > 1 ? (uint64_t)c.items * c.most * a.kv_heads * c.BM * (a.dim + 2) * 4 : 0;
+    return c.most > 1 ? COUNTERS * 4 + (uint64_t)c.items * c.most * a.kv_heads * c.BM * (a.dim + 2) * 4 : 0;
 }
 
 static Choice choose(const AttentionArgs& a) {
@@ -848,13 +913,17 @@ static int run_t(const AttentionArgs& a, hipStream_t s) {
     const int64_t tall = c.items * c.most, high = std::min<int64_t>(tall, 65535), deep = (tall + high - 1) / high;
     if (deep > 65535) return -2;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)high, (unsigned)deep);
-    const Split S = {c.most, c.size, (float*)a.work, c.items * c.most * a.kv_heads};
     constexpr int NW = DP > 128 ? 2 : 4;
+    // joined by the last part where its workgroup reads them all at once: 12 sequences x 2 parts 41 -> 35 us, 5 parts of 4 rows
+    // 15.7 -> 14.9, but 52 parts of 8 rows 16.2 -> 20.4, 16 parts of 32 rows 22.6 -> 29.5
+    const int64_t rows = std::min<int64_t>((int64_t)a.max_q * group, 32);
+    const bool fused = c.few && c.most > 1 && c.most <= AT_ONCE && rows * a.dim <= 4 * 64 * NW && c.items * a.kv_heads <= COUNTERS;
+    const Split S = {c.most, c.size, fused ? (int*)a.work : nullptr, (float*)a.work + COUNTERS, c.items * c.most * a.kv_heads};
     if (c.few)
         hipLaunchKernelGGL((few_k<T, DP, DC, NW>), grid, dim3(64 * NW), 0, s, a, S, g);
     else
         hipLaunchKernelGGL((rows_k<T, DP, DC, 4>), grid, dim3(256), 0, s, a, S, g);
-    if (c.most > 1) {
+    if (c.most > 1 && !fused) {
         if (int e = launch_rc()) return e;
         const int64_t jh = std::min<int64_t>(c.items, 65535), jd = (c.items + jh - 1) / jh;
         const dim3 jg((unsigned)(a.kv_heads * (c.few ? c.BM : c.BM / 8)), (unsigned)jh, (unsigned)jd);
