@@ -1,7 +1,12 @@
 // Attention of packed sequences over keys and values that lie packed or in caches (pcx_attention).
 //
 // For a query q that sees the keys j: z_j = scale q . k_j, m = max z_j, l = sum exp(z_j - m), o = sum exp(z_j - m) v_j / l,
-// lse = m + log l. One pass over the keys holds (m, l, o) and rescales l and o where m grows.
+// lse = m + log l. One pass over the keys holds (m, l, o) and rescales l and o where m grows. Scores, exponentials, sums and o are
+// f32; the weights exp(z_j - m) are rounded to the type for their product with v (the matrix cores take that type: 2^-9 relative
+// of each weight for bf16, 2^-12 for f16, as much again as the output's own rounding), l sums them unrounded.
+//
+// rows_k takes many rows (prompts, chunks), few_k the rows of a token or two and splits the keys over the chip; join_k joins
+// the parts.
 //
 // The rows of a tile are the (query, head) pairs of one key head, numbered query * group + head of the group: a tile of rows
 // reads its keys once for the whole group, and one token of a wide group fills a tile as a run of queries does. Everything is
@@ -26,6 +31,7 @@ typedef short v8s __attribute__((ext_vector_type(8)));
 typedef float v8f __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 #define PCH_LDS __attribute__((address_space(3)))
+
 template <class T>
 struct Mat;
 template <>
@@ -54,9 +60,10 @@ __device__ __forceinline__ float other(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------ tiles of keys
-// KT rows of room for DP values in LDS (of which the products take DC), 16-byte chunks permuted within a row so that both readings are free of bank conflicts: keys
-// (16 lanes take one chunk of 16 rows) by xor with the row number, values (32 lanes of the transposing read take 64 bytes of 4
-// rows) by xor with four times the row number.
+// KT rows of room for DP values in LDS (of which the products take DC), 16-byte chunks permuted within a row so that both
+// readings are free of bank conflicts: keys (16 lanes take one chunk of 16 rows) by xor with the row number, values (32 lanes of
+// the transposing read take 64 bytes of 4 rows) by xor with four times the row number (twice it: 67 million conflict cycles at
+// 16384 tokens x 16 heads; so: none).
 template <int DP>
 struct Tile {
     static constexpr int CPR = DP / 8;  // chunks of a row
@@ -65,15 +72,17 @@ struct Tile {
 };
 
 // 64 lanes' 16 bytes each from a buffer into LDS at `lds` + 16 lane; lanes past the buffer's end write zeros. It counts
-// in vmcnt like a load; nothing waits for it but the caller's own s_waitcnt.
+// in vmcnt like a load; nothing waits for it but the caller's own s_waitcnt (the builtin's loads are waited for, all of them,
+// before the next LDS reading, the tiles on their way too). The operands' scalar registers may have been written by vector
+// instructions (a spilled one is read back by v_readlane): five states until a buffer instruction may read them.
 __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t off) {
     asm volatile(
         "s_mov_b32 m0, %0\n\t"
-        "s_nop 0\n\t"
+        "s_nop 4\n\t"
         "buffer_load_dwordx4 %1, %2, 0 offen lds"
         :
         : "s"(lds), "v"(off), "s"(r)
-        : "memory");
+        : "memory", "m0");
 }
 
 // log of a row's sum l of exp2(. - m), in natural units; no key: l = 0 gives -infinity
@@ -143,9 +152,10 @@ __device__ __forceinline__ int largest(int x) {  // of values not negative
 }
 
 // item -> (sequence, tile of BM rows, part of its keys); BYPART false: all parts of a tile in one item. Every wave finds it by
-// itself, a lane per sequence. BYLEVEL: the tiles of up to 16 sequences go longest first (a tile's level: its keys in units of
-// its rows' queries), as workgroups start in their order and a long one that starts last is waited for; else, and for more
-// sequences, where finding it would cost more, one sequence after the other, each sequence's last tile first.
+// itself, a lane per sequence. BYLEVEL: the tiles of up to 64 sequences go longest first (a tile's level: its keys in units of
+// its rows' queries), as workgroups start in their order and a long one that starts last is waited for (48 caches of 89 to 8000
+// keys, one token each: 174 -> 159 us); else, and for more sequences, one sequence after the other, each sequence's last tile
+// first.
 template <bool BYPART, bool BYLEVEL>
 __device__ __forceinline__ Work locate(const AttentionArgs& A, const Split& S, int item, int group, int BM) {
     const int lane = threadIdx.x & 63;
@@ -320,8 +330,7 @@ struct Wave {
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb)
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-            {
+            for (int e = 0; e < 16; ++e) {
                 if (32 * kb + 8 * (e >> 2) + (e & 3) >= left) z[kb][e] = -INFINITY;
                 if ((e & 3) == 3) __builtin_amdgcn_sched_barrier(0);  // not all comparisons at once: they would not fit
             }
@@ -481,8 +490,18 @@ struct Wave {
 };
 
 // ------------------------------------------------------------------------------------------------ many rows
-// A workgroup of NW waves takes NW QB 32 rows; a tile of keys and values goes through LDS once for all of them, the next one
-// loaded while this one is used. Tiles run from the last to the first: those that rows see in part come first.
+// A workgroup of NW waves takes 32 NW rows; a tile of keys and values goes through LDS once for all of them, the next one loaded
+// while this one is used (two buffers of each: 64 KB at 128 dimensions, so that two workgroups share a CU). Tiles run from the
+// last to the first: those that rows see in part come first, and if they hold infinities or NaN that some row does not see their
+// sums are made again (repair) before the rest is added. The scores of tile t - 1 are made in tile t's step, beside its
+// exponentials, so that a wave has matrix and vector work at once.
+//
+// 16384 tokens x 16 heads of 128, causal, f16: 1.08 ms, 1017 TFLOP/s, 80% of what a 16384^3 product reaches; the matrix cores are
+// busy 57% of the cycles at 1.7 GHz, to which the card's power takes the clock: nine orderings of the step are within 2%, and
+// without any softmax the same products take 0.95 ms. 32 rows a wave: 64 would halve the LDS readings (256 bytes a cycle: half
+// used) but spill. Tiles of 64 keys (32 above 128 dimensions, where o takes half the registers). Nine prompts of 269 to 2048
+// tokens x 32 heads, bf16: 202 us, 797 TFLOP/s; a fifth of a workgroup's cycles is its start and end (finding its tile, first
+// loads, queries, output).
 template <class T, int DP, int DC, int NW>
 __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * NW, TB = KT * DP * 2, CPR = DP / 8, NK = KT / 32;
@@ -596,7 +615,9 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
 // ------------------------------------------------------------------------------------------------ few rows
 // A workgroup of NW waves takes 32 rows (one token's heads of a group, mostly) and a part of their keys; the waves take its
 // tiles of 32 keys in turn, each with LDS, statistics and sums of its own, and join at the end. What bounds it is the reading
-// of the keys: every wave keeps a whole tile of keys and of values on its way while it works on the one before.
+// of the keys: every wave keeps a whole tile of keys and of values on its way while it works on the one before (64 KB a CU at 128
+// dimensions). One token, 64 heads on 8 key heads of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0); 48 caches of 89 to
+// 8000 keys: 160 us, 5.1 TB/s. The 32 x 32 products leave most columns unused there; they take a tenth of the time of the reading.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -797,9 +818,9 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
 }
 
 // ------------------------------------------------------------------------------------------------ parts of the keys joined
-// 32 lanes of 4 dimensions to a row; PL lanes of parts, each merging every PL-th part, then the PL in their order; 8 / PL rows
-// to a workgroup. Reading the parts is all there is to do, so they are read in parallel: one
-// thread after the other through 128 parts took 120 us where this takes 4.
+// 32 lanes of 4 dimensions to a row; PL lanes of parts (8 after few_k, whose parts may be many, 1 after rows_k, whose rows are),
+// each merging every PL-th part, then the PL in their order; 8 / PL rows to a workgroup. Reading the parts is all there is to
+// do, so they are read in parallel: one thread after the other through 128 parts took 120 us, 32 parts so take 5.5.
 template <class T, int PL>
 __global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, Group group, int BM) {
     __shared__ v4f so[8][33];
@@ -883,10 +904,16 @@ static int checked(const AttentionArgs* a) {
 
 constexpr int COUNTERS = PCX_ATTENTION_COUNTERS;
 
-// the kernel and the split of a call
+// The kernel and the split of a call, by the lengths that the caller expects.
+//  few_k: up to 64 rows of a key head (16 queries x 4 heads over 8000 keys: rows_k 27 us, few_k 22; 64 x 4: 30 and 40), and at 64
+//  dimensions, where two of its workgroups share a CU, prompts whose tiles of 128 rows would not fill the chip (1024 tokens x 12
+//  heads: 21 and 14 us; 2048: 32 and 26; at 128 dimensions, 500 tokens x 32: 16 and 22).
+//  Splits: few_k to 256 workgroups, one a CU (131072 keys x 8 key heads: 192 or 256 workgroups 103 us, 384 114, 512 111) of at
+//  least 384 keys (512 keys in two parts: 11.3 -> 13 us; 2000 in five: 18.2 -> 15.7); rows_k to 512 of at least 512 keys (64 x 4
+//  rows over 8000 keys: no split 166 us, 256 workgroups 32.5, 512 29.5; 2000 tokens x 32 heads: none 49, two parts 71).
 struct Choice {
-    int few;      // few_k, else rows_k
-    int BM;       // rows of a tile
+    bool few;       // few_k, else rows_k
+    int BM;         // rows of a tile
     int64_t items;  // (sequence, tile) pairs at most
     int most, size;
 };
@@ -904,7 +931,7 @@ static Choice choose(const AttentionArgs& a) {
     // the tiles there are likely to be
     const int64_t base = (rows <= c.BM ? a.seqs : c.items) * a.kv_heads;
     const int64_t want = c.few ? 256 : 512;
-    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / 384));
+    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / (c.few ? 384 : 512)));
     c.size = (a.max_k + c.most - 1) / c.most;
     return c;
 }

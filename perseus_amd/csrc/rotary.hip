@@ -4,8 +4,6 @@
 // Per head x of dim values: n = x w / sqrt(mean(x^2) + eps) (the norm, where wanted), then the pairs i < rot / 2 turn,
 // (a, b) -> (a c - b s, b c + a s) with (c, s) = table[position][i]. Sums, squares and products are in f32; a value is
 // rounded once, when it is stored.
-#include <algorithm>
-
 #include "clear.h"
 
 namespace pch {
@@ -27,7 +25,10 @@ constexpr int WAVES = 4;
 
 // ------------------------------------------------------------------------------------------------ 16 values a lane
 // Two units of 8 values (16 bytes of a 16-bit type) to a lane: the two that hold its pairs' halves, or neighbours where pairs
-// are neighbours. A power of two of lanes takes a head, a wave as many heads of one token as fit.
+// are neighbours. A power of two of lanes takes a head, a wave as many heads of one token as fit: short waves, many of them (a
+// wave that went on to a second and third eight of heads, or a second token, kept fewer loads on their way: 16384 tokens x 40
+// heads 90 to 137 us where this took 84). The bound is the memory: 8191 tokens x 40 heads of 128 in 16 bits 35 us, 4.8 TB/s (a
+// large copy: 5.0); 16384 x 8 heads in 32 bits 29 us, 4.9; with the norms, 16384 x 40 heads out of rows of 48: 78 us, 4.4.
 template <class T>
 struct Eight {
     float v[8];
@@ -137,7 +138,8 @@ __global__ void __launch_bounds__(64 * WAVES) units_k(Pass A, int lph_log, uint3
 }
 
 // ------------------------------------------------------------------------------------------------ any size
-// Odd sizes, strides and addresses: a wave per head, a lane per pair or copied value.
+// Odd sizes, strides and addresses, what 16-byte accesses do not fit: a wave per head, a lane per pair or copied value (8191
+// tokens x 40 heads of 128 147 us).
 template <class T, bool NORM, bool INTER>
 __global__ void __launch_bounds__(64 * WAVES) heads_k(Pass A) {
     const int lane = threadIdx.x & 63;
