@@ -2,8 +2,10 @@
 //
 // For a query q that sees the keys j: z_j = scale q . k_j, m = max z_j, l = sum exp(z_j - m), o = sum exp(z_j - m) v_j / l,
 // lse = m + log l. One pass over the keys holds (m, l, o) and rescales l and o where m grows. Scores, exponentials, sums and o are
-// f32; the weights exp(z_j - m) are rounded to the type for their product with v (the matrix cores take that type: 2^-9 relative
-// of each weight for bf16, 2^-12 for f16, as much again as the output's own rounding), l sums them unrounded.
+// f32; the weights exp(z_j - m) are rounded to the type for their product with v, which the matrix cores take, and l sums them
+// unrounded. That rounding costs as much again as the output's own (2^-9 relative of each weight for bf16, 2^-12 for f16: the
+// error against 64 bits is 1.3 to 1.4 times that of one rounding). For the rows of a token, which are bound by the reading of the
+// keys, what it leaves is a second product, and the error is that of the output's rounding alone.
 //
 // rows_k takes many rows (prompts, chunks), few_k the rows of a token or two and splits the keys over the chip; join_k joins
 // the parts.
@@ -374,7 +376,8 @@ struct Wave {
         R.l += l;
     }
 
-    // o += p V
+    // o += p V; TWICE: with what the weights' rounding left as a second product
+    template <bool TWICE = false>
     static __device__ __forceinline__ void values(const char PCH_LDS* v, Rows<T, DC>& R, const v16f (&z)[NK]) {
         const int lane = threadIdx.x & 63;
         const int key = 4 * (lane >> 5) + ((lane & 15) >> 2), ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
@@ -385,6 +388,8 @@ struct Wave {
 #pragma unroll
             for (int e = 0; e < 8; ++e) pf[e] = z[s >> 1][8 * (s & 1) + e];
             const v8 p = __builtin_convertvector(pf, v8);
+            v8 rest;
+            if (TWICE) rest = __builtin_convertvector(pf - __builtin_convertvector(p, v8f), v8);
 #pragma unroll
             for (int d = 0; d < DC / 32; ++d) {
                 // the swizzle of rows 8 apart is the same
@@ -393,6 +398,7 @@ struct Wave {
                 const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s PCH_LDS*)(v + x + 8 * DP * 2));
                 const v8s a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
                 R.o[d] = Mat<T>::mul(__builtin_bit_cast(v8, a), p, R.o[d]);
+                if (TWICE) R.o[d] = Mat<T>::mul(__builtin_bit_cast(v8, a), rest, R.o[d]);
             }
         }
     }
@@ -420,7 +426,7 @@ struct Wave {
                 }
                 z += other(z);
                 if (j >= R.lim) continue;
-                const float p = (float)(T)__builtin_amdgcn_exp2f(fmaf(z, c, R.nm));
+                const float p = __builtin_amdgcn_exp2f(fmaf(z, c, R.nm));
 #pragma unroll
                 for (int d = 0; d < DC / 32; ++d)
 #pragma unroll
@@ -635,7 +641,7 @@ __device__ __forceinline__ float2 past(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-template <class T, int DP, int DC, int NW>
+template <class T, int DP, int DC, int NW, bool TWICE>
 __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = 32, BM = 32, TB = KT * DP * 2, CPR = DP / 8, NL = KT * CPR / 64, PAD = DP + 4;
     using W = Wave<T, DP, DC, KT>;
@@ -717,7 +723,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
             wait_loads<2 * NL>();
         else
             wait_loads<0>();
-        W::values(kl + TB, row, z);
+        W::template values<TWICE>(kl + TB, row, z);
     }
     if (unchecked) mend();
 
@@ -952,8 +958,11 @@ static int run_t(const AttentionArgs& a, hipStream_t s) {
     const int64_t rows = std::min<int64_t>((int64_t)a.max_q * group, 32);
     const bool fused = c.few && c.most > 1 && c.most <= AT_ONCE && rows * a.dim <= 4 * 64 * NW && c.items * a.kv_heads <= COUNTERS;
     const Split S = {c.most, c.size, fused ? (int*)a.work : nullptr, (float*)a.work + COUNTERS, c.items * c.most * a.kv_heads};
-    if (c.few)
-        hipLaunchKernelGGL((few_k<T, DP, DC, NW>), grid, dim3(64 * NW), 0, s, a, S, g);
+    // the second product: not for the prompts of 64 dimensions that few_k takes, which it would make 13% slower
+    if (c.few && (DP > 64 || (int64_t)a.max_q * group <= 64))
+        hipLaunchKernelGGL((few_k<T, DP, DC, NW, true>), grid, dim3(64 * NW), 0, s, a, S, g);
+    else if (c.few)
+        hipLaunchKernelGGL((few_k<T, 64, 64, 4, false>), grid, dim3(256), 0, s, a, S, g);
     else
         hipLaunchKernelGGL((rows_k<T, DP, DC, 4>), grid, dim3(256), 0, s, a, S, g);
     if (c.most > 1 && !fused) {
