@@ -621,8 +621,9 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
 // ------------------------------------------------------------------------------------------------ few rows
 // A workgroup of NW waves takes 32 rows (one token's heads of a group, mostly) and a part of their keys; the waves take its
 // tiles of 32 keys in turn, each with LDS, statistics and sums of its own, and join at the end. What bounds it is the reading
-// of the keys: every wave keeps a whole tile of keys and of values on its way while it works on the one before (64 KB a CU at 128
-// dimensions). One token, 64 heads on 8 key heads of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0); 48 caches of 89 to
+// of the keys. ST 2: every wave keeps a whole tile of keys and of values on its way while it works on the one before (4 waves: 64
+// KB a CU at 128 dimensions). ST 1: twice the waves, each with one tile that it waits for and works on: what is on its way is
+// much the same, and short runs, whose waves' first and last tiles count, are done sooner. One token, 64 heads on 8 key heads of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0); 48 caches of 89 to
 // 8000 keys: 160 us, 5.1 TB/s. The 32 x 32 products leave most columns unused there; they take a tenth of the time of the reading.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -641,12 +642,12 @@ __device__ __forceinline__ float2 past(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-template <class T, int DP, int DC, int NW, bool TWICE>
+template <class T, int DP, int DC, int NW, int ST, bool TWICE>
 __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = 32, BM = 32, TB = KT * DP * 2, CPR = DP / 8, NL = KT * CPR / 64, PAD = DP + 4;
     using W = Wave<T, DP, DC, KT>;
-    __shared__ __attribute__((aligned(1024))) char lds[NW * 4 * TB];
-    static_assert(NW * 4 * TB >= (NW * BM * PAD + NW * BM * 2) * 4, "the join fits the tiles' memory");
+    constexpr int JOIN = (NW * BM * PAD + NW * BM * 2) * 4, TILES = NW * ST * 2 * TB;
+    __shared__ __attribute__((aligned(1024))) char lds[JOIN > TILES ? JOIN : TILES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int kvh = blockIdx.x;
     const Work w = locate<true, true>(A, S, blockIdx.z * gridDim.y + blockIdx.y, group.n, BM);
@@ -672,7 +673,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
         ko[n] = ck * 8 < A.dim ? key * (uint32_t)A.k.token * 2 + ck * 16 : 0x7ffffff0u;
         vo[n] = cv * 8 < A.dim ? key * (uint32_t)A.v.token * 2 + cv * 16 : 0x7ffffff0u;
     }
-    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 4 * TB;
+    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * ST * 2 * TB;
     const char* kp = (const char*)uniform64((uint64_t)at<T>(A.k, w.k0, kvh));
     const char* vp = (const char*)uniform64((uint64_t)at<T>(A.v, w.k0, kvh));
     auto load = [&](int t, int half) {
@@ -689,7 +690,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     };
     // this wave's tiles, from the last of those that are `wave` mod NW after the first
     const int mine = tiles - first > wave ? (tiles - first - wave + NW - 1) / NW : 0;
-    if (mine) load(first + wave + (mine - 1) * NW, (mine - 1) & 1);
+    if (mine) load(first + wave + (mine - 1) * NW, (mine - 1) & (ST - 1));
     Rows<T, DC> row;
     row.begin(A, w, kvh, group, r0 + (lane & 31));
     bool unchecked = false;
@@ -703,13 +704,13 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     for (int u = mine - 1; u >= 0; --u) {
         const int t = first + wave + u * NW;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last tile's reads are done: its memory takes the next one
-        if (u) {
+        if (ST == 2 && u) {
             load(t - NW, (u - 1) & 1);
             wait_loads<3 * NL>();
         } else {
             wait_loads<NL>();
         }
-        const char PCH_LDS* kl = (const char PCH_LDS*)lds + wave * 4 * TB + (u & 1) * 2 * TB;
+        const char PCH_LDS* kl = (const char PCH_LDS*)lds + wave * ST * 2 * TB + (u & (ST - 1)) * 2 * TB;
         v16f z[1];
         W::scores(kl, row, z);
         if (t >= whole) {
@@ -719,11 +720,15 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
             mend();
         }
         W::softmax(row, c, z);
-        if (u)
+        if (ST == 2 && u)
             wait_loads<2 * NL>();
         else
             wait_loads<0>();
         W::template values<TWICE>(kl + TB, row, z);
+        if (ST == 1 && u) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load(t - NW, 0);
+        }
     }
     if (unchecked) mend();
 
@@ -952,17 +957,24 @@ static int run_t(const AttentionArgs& a, hipStream_t s) {
     const int64_t tall = c.items * c.most, high = std::min<int64_t>(tall, 65535), deep = (tall + high - 1) / high;
     if (deep > 65535) return -2;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)high, (unsigned)deep);
-    constexpr int NW = DP > 128 ? 2 : 4;
+    // few_k's waves: long runs of keys are read at the full rate by 4 with two tiles each (131072 keys: 104 us, by 8 108), short ones
+    // sooner by 8 (2000 keys x 8 key heads: 16.4 and 14.8 us; 8 caches of up to 8000, 64 rows: 25.3 and 21.1). Above 128
+    // dimensions only 4 tiles fit (two waves with two tiles each: 66 -> 47 us at 256, 137 -> 99 at 192).
+    const bool longer = c.size >= 3000;
+    constexpr int FEW = DP > 128 ? 4 : 8;
+    const int NW = DP > 128 || longer ? 4 : 8;
     // joined by the last part where its workgroup reads them all at once: 12 sequences x 2 parts 41 -> 35 us, 5 parts of 4 rows
     // 15.7 -> 14.9, but 52 parts of 8 rows 16.2 -> 20.4, 16 parts of 32 rows 22.6 -> 29.5
     const int64_t rows = std::min<int64_t>((int64_t)a.max_q * group, 32);
     const bool fused = c.few && c.most > 1 && c.most <= AT_ONCE && rows * a.dim <= 4 * 64 * NW && c.items * a.kv_heads <= COUNTERS;
     const Split S = {c.most, c.size, fused ? (int*)a.work : nullptr, (float*)a.work + COUNTERS, c.items * c.most * a.kv_heads};
     // the second product: not for the prompts of 64 dimensions that few_k takes, which it would make 13% slower
-    if (c.few && (DP > 64 || (int64_t)a.max_q * group <= 64))
-        hipLaunchKernelGGL((few_k<T, DP, DC, NW, true>), grid, dim3(64 * NW), 0, s, a, S, g);
+    if (c.few && DP == 64 && (int64_t)a.max_q * group > 64)
+        hipLaunchKernelGGL((few_k<T, 64, 64, 4, 2, false>), grid, dim3(256), 0, s, a, S, g);
+    else if (c.few && DP <= 128 && longer)
+        hipLaunchKernelGGL((few_k<T, std::min(DP, 128), std::min(DC, 128), 4, 2, true>), grid, dim3(256), 0, s, a, S, g);
     else if (c.few)
-        hipLaunchKernelGGL((few_k<T, 64, 64, 4, false>), grid, dim3(256), 0, s, a, S, g);
+        hipLaunchKernelGGL((few_k<T, DP, DC, FEW, 1, true>), grid, dim3(64 * FEW), 0, s, a, S, g);
     else
         hipLaunchKernelGGL((rows_k<T, DP, DC, 4>), grid, dim3(256), 0, s, a, S, g);
     if (c.most > 1 && !fused) {
