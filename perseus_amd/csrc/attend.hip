@@ -189,7 +189,8 @@ __device__ __forceinline__ Work locate(const AttentionArgs& A, const Split& S, i
         } else if (BYLEVEL && A.seqs <= 64) {
             // a tile's level is `above` + its number, or (not causal) `above`
             const int keys = A.causal ? (len > n ? len - n : 0) : len;
-            const int above = (int)((int64_t)keys * group / BM), span = A.causal ? tiles : tiles > 0;
+            // (a bound that only matters to the order: no sum of levels leaves 31 bits)
+            const int above = (int)std::min<int64_t>((int64_t)keys * group / BM, 1 << 30), span = A.causal ? tiles : tiles > 0;
             const int each = A.causal ? nc : tiles * nc;
             // the items of a lane's own level u and more
             const auto count = [&](int u) {
@@ -405,7 +406,7 @@ struct Wave {
 
     // The rare repair of the tiles that a row sees in part. There o^T += V^T p^T multiplies values that a row does not see by
     // zero, which is not zero where they are infinite or NaN. If o came out so, o of these keys (from key0 to each row's
-    // limit: at most a tile of rows and one of keys) is summed again from memory, key by key, each row its own.
+    // limit, a tile of KT in every `step`) is summed again from memory, key by key, each row its own.
     static __device__ __forceinline__ void repair(const AttentionArgs& A, const Work& w, int kvh, float c, int key0, int key1,
                                                int step, Rows<T, DC>& R) {
         const int h = (threadIdx.x & 63) >> 5;
@@ -623,8 +624,9 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
 // tiles of 32 keys in turn, each with LDS, statistics and sums of its own, and join at the end. What bounds it is the reading
 // of the keys. ST 2: every wave keeps a whole tile of keys and of values on its way while it works on the one before (4 waves: 64
 // KB a CU at 128 dimensions). ST 1: twice the waves, each with one tile that it waits for and works on: what is on its way is
-// much the same, and short runs, whose waves' first and last tiles count, are done sooner. One token, 64 heads on 8 key heads of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0); 48 caches of 89 to
-// 8000 keys: 160 us, 5.1 TB/s. The 32 x 32 products leave most columns unused there; they take a tenth of the time of the reading.
+// much the same, and short runs, whose waves' first and last tiles count, are done sooner. One token, 64 heads on 8 key heads
+// of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0); 48 caches of 89 to 8000 keys: 160 us, 5.1 TB/s. The 32 x 32
+// products leave most columns unused there; they take a tenth of the time of the reading.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -693,11 +695,13 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     if (mine) load(first + wave + (mine - 1) * NW, (mine - 1) & (ST - 1));
     Rows<T, DC> row;
     row.begin(A, w, kvh, group, r0 + (lane & 31));
-    bool unchecked = false;
+    // TWICE: an infinite value times what the weights' rounding leaves, which has either sign or is zero, is no infinity of the
+    // value's sign: there all of the wave's tiles are checked, at the end; else those that rows see in part, once they are done
+    bool unchecked = TWICE;
     const auto mend = [&] {
         unchecked = false;
         if (W::broken(row)) {
-            const int skip = whole - first > wave ? (whole - first - wave + NW - 1) / NW : 0;
+            const int from = TWICE ? first : whole, skip = from - first > wave ? (from - first - wave + NW - 1) / NW : 0;
             W::repair(A, w, kvh, c, (first + wave + skip * NW) * KT, hi, KT * NW, row);
         }
     };
@@ -716,7 +720,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
         if (t >= whole) {
             W::mask(row, t * KT, z);
             unchecked |= A.causal && (t + 1) * KT > lo && lo < w.len;
-        } else if (unchecked) {
+        } else if (!TWICE && unchecked) {
             mend();
         }
         W::softmax(row, c, z);
@@ -943,7 +947,7 @@ static Choice choose(const AttentionArgs& a) {
     const int64_t base = (rows <= c.BM ? a.seqs : c.items) * a.kv_heads;
     const int64_t want = c.few ? 256 : 512;
     c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / (c.few ? 384 : 512)));
-    c.size = (a.max_k + c.most - 1) / c.most;
+    c.size = (int)(((int64_t)a.max_k + c.most - 1) / c.most);
     return c;
 }
 
@@ -952,7 +956,7 @@ static int run_t(const AttentionArgs& a, hipStream_t s) {
     const int group = a.heads / a.kv_heads;
     Choice c = choose(a);
     while (c.most > 1 && work_bytes(a, c) > (a.work ? a.work_bytes : 0)) c.most = c.most / 2;
-    if (c.most > 1) c.size = (a.max_k + c.most - 1) / c.most;
+    if (c.most > 1) c.size = (int)(((int64_t)a.max_k + c.most - 1) / c.most);
     const Group g = {group, 1.0 / group};
     const int64_t tall = c.items * c.most, high = std::min<int64_t>(tall, 65535), deep = (tall + high - 1) / high;
     if (deep > 65535) return -2;

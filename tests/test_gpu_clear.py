@@ -271,6 +271,24 @@ def test_attention_unseen_values_do_not_reach_a_query(ops, dim, heads, kv, spans
     run_attention(ops, "bf16", dim, heads, kv, spans, True, edit=edit)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,heads,kv,spans", [
+    (128, 4, 2, [(1, 900), (3, 100)]), (64, 2, 2, [(1, 40), (2, 3000)]), (256, 4, 2, [(2, 300)]), (128, 4, 2, [(150, 150)]),
+    (64, 2, 2, [(300, 300)])])
+def test_attention_infinite_values_that_are_seen(ops, kind, dim, heads, kv, spans):
+    """an infinite value makes that dimension of the queries that see it infinite, two of different sign NaN"""
+    say(f"[clear] attention with infinite values {kind} dim {dim} {spans}")
+
+    def edit(q, k, v, k0):
+        for s in k0:
+            v[s + 3, 0, 1] = np.inf
+            v[s + 4:s + 30, -1, 2] = -np.inf
+            v[s + 9, 0, 5], v[s + 17, 0, 5] = np.inf, -np.inf
+
+    for causal in (True, False):
+        run_attention(ops, kind, dim, heads, kv, spans, causal, edit=edit)
+
+
 @pytest.mark.parametrize("dim,heads,kv,spans", [(128, 4, 2, [(5, 900)]), (64, 2, 2, [(1, 40), (2, 3000)]), (128, 4, 4, [(200, 200)])])
 def test_attention_of_nan_queries(ops, dim, heads, kv, spans):
     """a query of NaN has NaN for its sums and no finite log: its neighbours in the tile and the split do not"""
