@@ -589,24 +589,53 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
     }
     if (A.causal && hi > whole * KT && W::broken(row)) W::repair(A, w, kvh, c, whole * KT, hi, KT, row);
     float top = hi ? W::largest_of(z) : 0;
-    for (; t > first; --t) {
+    // a step: tile t's weights and values, the scores of the one before; odd: t & 1
+    const auto step = [&](int odd, v16f (&x)[NK], v16f (&y)[NK]) __attribute__((always_inline)) {
         arrived();
         load_k(t - 2);
         load_v(t - 1);
-        if (!hi) continue;
+        if (!hi) return;
         W::grow(row, c, top);
-        W::template scores<false>(keys(t - 1), row, zn);
-        // the compiler's own pattern for products between exponentials at 64 dimensions (8192 tokens x 16 heads 183 -> 173 us),
-        // for products between LDS readings above (256 dimensions 425 -> 405, prompt_long 1111 -> 1097)
-        if constexpr (DC == 64)
-            __builtin_amdgcn_iglp_opt(2);
-        else
-            __builtin_amdgcn_iglp_opt(0);
-        W::weigh(row, c, z);
-        W::values(values(t), row, z);
-        top = W::largest_of(zn);
+        W::template scores<false>(keys(odd ^ 1), row, y);
+        // the compiler's own pattern for products between LDS readings (256 dimensions 425 -> 405, prompt_long 1111 -> 1097)
+        __builtin_amdgcn_iglp_opt(0);
+        W::weigh(row, c, x);
+        W::values(values(odd), row, x);
+        top = W::largest_of(y);
+    };
+    const auto single = [&](int odd) __attribute__((always_inline)) {
+        step(odd, z, zn);
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb) z[kb] = zn[kb];
+        --t;
+    };
+    if constexpr (DC > 64) {
+        // in pairs that begin at an even tile, z and zn taking turns: no copies, and the compiler knows the buffers (256
+        // dimensions 427 -> 327 us, 192 333 -> 301, 96 127 -> 121, prompt_long 1067 -> 1048; but 64, causal, 177 -> 189)
+        if (t > first && (t & 1)) single(1);
+        while (t > first + 1) {
+            step(0, z, zn);
+            --t;
+            step(1, zn, z);
+            --t;
+        }
+        if (t > first) single(0);
+    } else {
+        for (; t > first; --t) {
+            arrived();
+            load_k(t - 2);
+            load_v(t - 1);
+            if (!hi) continue;
+            W::grow(row, c, top);
+            W::template scores<false>(keys(t - 1), row, zn);
+            // the pattern for products between exponentials (8192 tokens x 16 heads 183 -> 173 us)
+            __builtin_amdgcn_iglp_opt(2);
+            W::weigh(row, c, z);
+            W::values(values(t), row, z);
+            top = W::largest_of(zn);
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb) z[kb] = zn[kb];
+        }
     }
     if (t == first) {
         arrived();
