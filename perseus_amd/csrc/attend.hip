@@ -87,6 +87,10 @@ __device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t lds,
         : "memory", "m0");
 }
 
+// All loads are there, the compiler's own among them. It counts those alone: one of its loads before a loop (a query's, the rare
+// repair's) that it does not know to be there makes it wait for everything, the tiles on their way too, in every step.
+__device__ __forceinline__ void settled() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // log of a row's sum l of exp2(. - m), in natural units; no key: l = 0 gives -infinity
 __device__ __forceinline__ float logsum(float m, float l) {
     return l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f;
@@ -572,6 +576,7 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
     // z: the scores of tile t, made while tile t + 1 was worked on
     v16f z[NK], zn[NK];
     int t = tiles - 1;
+    settled();
     arrived();
     if (t >= first && t * KT < hi) W::scores(keys(t), row, z);
     for (; t >= whole; --t) {
@@ -588,6 +593,7 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
         for (int kb = 0; kb < NK; ++kb) z[kb] = zn[kb];
     }
     if (A.causal && hi > whole * KT && W::broken(row)) W::repair(A, w, kvh, c, whole * KT, hi, KT, row);
+    settled();
     float top = hi ? W::largest_of(z) : 0;
     // a step: tile t's weights and values, the scores of the one before; odd: t & 1
     const auto step = [&](int odd, v16f (&x)[NK], v16f (&y)[NK]) __attribute__((always_inline)) {
@@ -732,8 +738,10 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
         if (W::broken(row)) {
             const int from = TWICE ? first : whole, skip = from - first > wave ? (from - first - wave + NW - 1) / NW : 0;
             W::repair(A, w, kvh, c, (first + wave + skip * NW) * KT, hi, KT * NW, row);
+            settled();
         }
     };
+    settled();
     for (int u = mine - 1; u >= 0; --u) {
         const int t = first + wave + u * NW;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last tile's reads are done: its memory takes the next one
