@@ -73,18 +73,33 @@ struct Tile {
     static __device__ __forceinline__ int vswz(int key) { return DP == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); }
 };
 
-// 64 lanes' 16 bytes each from a buffer into LDS at `lds` + 16 lane; lanes past the buffer's end write zeros. It counts
-// in vmcnt like a load; nothing waits for it but the caller's own s_waitcnt (the builtin's loads are waited for, all of them,
-// before the next LDS reading, the tiles on their way too). The operands' scalar registers may have been written by vector
-// instructions (a spilled one is read back by v_readlane): five states until a buffer instruction may read them.
-__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t lds, uint32_t off) {
-    asm volatile(
-        "s_mov_b32 m0, %0\n\t"
-        "s_nop 4\n\t"
-        "buffer_load_dwordx4 %1, %2, 0 offen lds"
-        :
-        : "s"(lds), "v"(off), "s"(r)
-        : "memory", "m0");
+// 64 lanes' 16 bytes each from a buffer into LDS at `lds` + 16 lane, N times, STEP bytes of LDS apart; lanes past the buffer's
+// end write zeros. It counts in vmcnt like a load; nothing waits for it but the caller's own s_waitcnt (the builtin's loads are
+// waited for, all of them, before the next LDS reading, the tiles on their way too). The operands' scalar registers may have
+// been written by vector instructions (a spilled one is read back by v_readlane): five states until a buffer instruction may
+// read them, and one after m0.
+template <int STEP, int N>
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t r, uint32_t lds, const uint32_t (&off)[N]) {
+    static_assert(N == 2 || N % 4 == 0);
+    if constexpr (N == 2) {
+        asm volatile(
+            "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\t"
+            "s_add_u32 m0, m0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds"
+            :
+            : "s"(lds), "v"(off[0]), "v"(off[1]), "s"(r), "n"(STEP)
+            : "memory", "m0", "scc");
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; n += 4)
+            asm volatile(
+                "s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %5, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %2, %5, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %3, %5, 0 offen lds\n\t"
+                "s_add_u32 m0, m0, %6\n\ts_nop 0\n\tbuffer_load_dwordx4 %4, %5, 0 offen lds"
+                :
+                : "s"(lds + n * STEP), "v"(off[n]), "v"(off[n + 1]), "v"(off[n + 2]), "v"(off[n + 3]), "s"(r), "n"(STEP)
+                : "memory", "m0", "scc");
+    }
 }
 
 // All loads are there, the compiler's own among them. It counts those alone: one of its loads before a loop (a query's, the rare
@@ -548,8 +563,7 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
         const int left = w.len - t * KT, nr = (left < KT ? left : KT) - 1;
         const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)t * KT * token * 2), 0,
                                                          (nr * (int)token + A.dim) * 2, 0x00020000);
-#pragma unroll
-        for (int n = 0; n < NL; ++n) load_lds(r, to + n * NW * 1024, off[n]);
+        load_lds<NW * 1024>(r, to, off);
     };
     const auto load_k = [&](int t) {
         if (t >= first) load(kp, A.k.token, t, base + (t & 1) * TB, ko);
@@ -657,11 +671,12 @@ __global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArg
 // ------------------------------------------------------------------------------------------------ few rows
 // A workgroup of NW waves takes 32 rows (one token's heads of a group, mostly) and a part of their keys; the waves take its
 // tiles of 32 keys in turn, each with LDS, statistics and sums of its own, and join at the end. What bounds it is the reading
-// of the keys. ST 2: every wave keeps a whole tile of keys and of values on its way while it works on the one before (4 waves: 64
-// KB a CU at 128 dimensions). ST 1: twice the waves, each with one tile that it waits for and works on: what is on its way is
-// much the same, and short runs, whose waves' first and last tiles count, are done sooner. One token, 64 heads on 8 key heads
-// of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0); 48 caches of 89 to 8000 keys: 160 us, 5.1 TB/s. The 32 x 32
-// products leave most columns unused there; they take a tenth of the time of the reading.
+// of the keys: 8 waves (4 above 128 dimensions: 128 KB either way) keep a tile of keys and one of values each on their way or
+// in work, the next keys asked for as soon as the scores are made, the next values after the products (256 dimensions, 16
+// caches of up to 8000: both after the products 40.3 us, so 37.2). 4 waves of two tiles each: 20 caches of up to 4000 56 -> 54
+// us, 131072 keys 104.1 -> 103. One token, 64 heads on 8 key heads of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0);
+// 48 caches of 89 to 8000 keys: 160 us, 5.1 TB/s. The 32 x 32 products leave most columns unused there; they take a tenth of
+// the time of the reading.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -679,11 +694,11 @@ __device__ __forceinline__ float2 past(const float* p) {
     return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
 }
 
-template <class T, int DP, int DC, int NW, int ST, bool TWICE>
+template <class T, int DP, int DC, int NW, bool TWICE>
 __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = 32, BM = 32, TB = KT * DP * 2, CPR = DP / 8, NL = KT * CPR / 64, PAD = DP + 4;
     using W = Wave<T, DP, DC, KT>;
-    constexpr int JOIN = (NW * BM * PAD + NW * BM * 2) * 4, TILES = NW * ST * 2 * TB;
+    constexpr int JOIN = (NW * BM * PAD + NW * BM * 2) * 4, TILES = NW * 2 * TB;
     __shared__ __attribute__((aligned(1024))) char lds[JOIN > TILES ? JOIN : TILES];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int kvh = blockIdx.x;
@@ -710,24 +725,23 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
         ko[n] = ck * 8 < A.dim ? key * (uint32_t)A.k.token * 2 + ck * 16 : 0x7ffffff0u;
         vo[n] = cv * 8 < A.dim ? key * (uint32_t)A.v.token * 2 + cv * 16 : 0x7ffffff0u;
     }
-    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * ST * 2 * TB;
+    const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 2 * TB;
     const char* kp = (const char*)uniform64((uint64_t)at<T>(A.k, w.k0, kvh));
     const char* vp = (const char*)uniform64((uint64_t)at<T>(A.v, w.k0, kvh));
-    auto load = [&](int t, int half) {
+    const auto load = [&](const char* p, int64_t token, int t, uint32_t to, const uint32_t (&off)[NL]) {
         const int left = w.len - t * KT, nr = (left < KT ? left : KT) - 1;
-        const uint32_t to = base + half * 2 * TB;
-        const auto rk = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)t * KT * A.k.token * 2), 0,
-                                                          (nr * (int)A.k.token + A.dim) * 2, 0x00020000);
-        const auto rv = __builtin_amdgcn_make_buffer_rsrc((void*)(vp + (int64_t)t * KT * A.v.token * 2), 0,
-                                                          (nr * (int)A.v.token + A.dim) * 2, 0x00020000);
-#pragma unroll
-        for (int n = 0; n < NL; ++n) load_lds(rk, to + n * 1024, ko[n]);
-#pragma unroll
-        for (int n = 0; n < NL; ++n) load_lds(rv, to + TB + n * 1024, vo[n]);
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(p + (int64_t)t * KT * token * 2), 0,
+                                                         (nr * (int)token + A.dim) * 2, 0x00020000);
+        load_lds<1024>(r, to, off);
     };
+    const auto load_k = [&](int t) { load(kp, A.k.token, t, base, ko); };
+    const auto load_v = [&](int t) { load(vp, A.v.token, t, base + TB, vo); };
     // this wave's tiles, from the last of those that are `wave` mod NW after the first
     const int mine = tiles - first > wave ? (tiles - first - wave + NW - 1) / NW : 0;
-    if (mine) load(first + wave + (mine - 1) * NW, (mine - 1) & (ST - 1));
+    if (mine) {
+        load_k(first + wave + (mine - 1) * NW);
+        load_v(first + wave + (mine - 1) * NW);
+    }
     Rows<T, DC> row;
     row.begin(A, w, kvh, group, r0 + (lane & 31));
     // TWICE: an infinite value times what the weights' rounding leaves, which has either sign or is zero, is no infinity of the
@@ -741,19 +755,18 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
             settled();
         }
     };
+    const char PCH_LDS* const tl = (const char PCH_LDS*)lds + wave * 2 * TB;
+    const auto read = [] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };  // a tile's memory takes the next one
     settled();
     for (int u = mine - 1; u >= 0; --u) {
         const int t = first + wave + u * NW;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last tile's reads are done: its memory takes the next one
-        if (ST == 2 && u) {
-            load(t - NW, (u - 1) & 1);
-            wait_loads<3 * NL>();
-        } else {
-            wait_loads<NL>();
-        }
-        const char PCH_LDS* kl = (const char PCH_LDS*)lds + wave * ST * 2 * TB + (u & (ST - 1)) * 2 * TB;
+        wait_loads<NL>();
         v16f z[1];
-        W::scores(kl, row, z);
+        W::scores(tl, row, z);
+        if (TWICE && u) {
+            read();
+            load_k(t - NW);
+        }
         if (t >= whole) {
             W::mask(row, t * KT, z);
             unchecked |= A.causal && (t + 1) * KT > lo && lo < w.len;
@@ -761,14 +774,15 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
             mend();
         }
         W::softmax(row, c, z);
-        if (ST == 2 && u)
-            wait_loads<2 * NL>();
+        if (TWICE && u)
+            wait_loads<NL>();
         else
             wait_loads<0>();
-        W::template values<TWICE>(kl + TB, row, z);
-        if (ST == 1 && u) {
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            load(t - NW, 0);
+        W::template values<TWICE>(tl + TB, row, z);
+        if (u) {
+            read();
+            if (!TWICE) load_k(t - NW);  // a prompt's, from L2: 2000 tokens x 12 heads of 64 26.4 us if asked for above, so 25.1
+            load_v(t - NW);
         }
     }
     if (unchecked) mend();
@@ -967,6 +981,7 @@ struct Choice {
     bool few;       // few_k, else rows_k
     int BM;         // rows of a tile
     int64_t items;  // (sequence, tile) pairs at most
+    int64_t base;   // workgroups there are likely to be without a split
     int most, size;
 };
 static uint64_t work_bytes(const AttentionArgs& a, const Choice& c) {
@@ -984,9 +999,9 @@ static Choice choose(const AttentionArgs& a) {
     // idle (512 queries x 32/8 heads over 30000 keys: 3 parts 301 us, 4 fill it, 268)
     const int64_t spare = std::max<int64_t>((int64_t)a.seqs * c.BM / 2, c.BM - 1);
     const int64_t guess = std::min((rows + c.BM - 1) / c.BM * a.seqs, ((int64_t)a.tokens * group + spare) / c.BM);
-    const int64_t base = std::max<int64_t>(a.seqs, guess) * a.kv_heads;
+    c.base = std::max<int64_t>(a.seqs, guess) * a.kv_heads;
     const int64_t want = c.few ? 256 : 512;
-    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(base, 1), a.max_k / (c.few ? 384 : 512)));
+    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(c.base, 1), a.max_k / (c.few ? 384 : 512)));
     c.size = (int)(((int64_t)a.max_k + c.most - 1) / c.most);
     return c;
 }
@@ -1001,24 +1016,22 @@ static int run_t(const AttentionArgs& a, hipStream_t s) {
     const int64_t tall = c.items * c.most, high = std::min<int64_t>(tall, 65535), deep = (tall + high - 1) / high;
     if (deep > 65535) return -2;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)high, (unsigned)deep);
-    // few_k's waves: long runs of keys are read at the full rate by 4 with two tiles each (131072 keys: 104 us, by 8 108), short ones
-    // sooner by 8 (2000 keys x 8 key heads: 16.4 and 14.8 us; 8 caches of up to 8000, 64 rows: 25.3 and 21.1). Above 128
-    // dimensions only 4 tiles fit (two waves with two tiles each: 66 -> 47 us at 256, 137 -> 99 at 192).
-    const bool longer = c.size >= 3000;
-    constexpr int FEW = DP > 128 ? 4 : 8;
-    const int NW = DP > 128 || longer ? 4 : 8;
+    constexpr int NW = DP > 128 ? 4 : 8;
     // joined by the last part where its workgroup reads them all at once: 12 sequences x 2 parts 41 -> 35 us, 5 parts of 4 rows
     // 15.7 -> 14.9, but 52 parts of 8 rows 16.2 -> 20.4, 16 parts of 32 rows 22.6 -> 29.5
     const int64_t rows = std::min<int64_t>((int64_t)a.max_q * group, 32);
     const bool fused = c.few && c.most > 1 && c.most <= AT_ONCE && rows * a.dim <= 4 * 64 * NW && c.items * a.kv_heads <= COUNTERS;
     const Split S = {c.most, c.size, fused ? (int*)a.work : nullptr, (float*)a.work + COUNTERS, c.items * c.most * a.kv_heads};
-    // the second product: not for the prompts of 64 dimensions that few_k takes, which it would make 13% slower
-    if (c.few && DP == 64 && (int64_t)a.max_q * group > 64)
-        hipLaunchKernelGGL((few_k<T, 64, 64, 4, 2, false>), grid, dim3(256), 0, s, a, S, g);
-    else if (c.few && DP <= 128 && longer)
-        hipLaunchKernelGGL((few_k<T, std::min(DP, 128), std::min(DC, 128), 4, 2, true>), grid, dim3(256), 0, s, a, S, g);
+    // the second product: not for the prompts of 64 dimensions that few_k takes, which it would make 13% slower; 4 waves for them
+    // where there are workgroups for two a CU (1024 tokens x 12 heads: 8 waves 15.3 us, 4 13.4; 100 queries x 8 heads over
+    // 4000 keys, 2 key heads: 16.1 and 18.8)
+    const bool prompt = c.few && DP == 64 && (int64_t)a.max_q * group > 64;
+    if (prompt && c.base > 256)
+        hipLaunchKernelGGL((few_k<T, 64, 64, 4, false>), grid, dim3(256), 0, s, a, S, g);
+    else if (prompt)
+        hipLaunchKernelGGL((few_k<T, 64, 64, 8, false>), grid, dim3(512), 0, s, a, S, g);
     else if (c.few)
-        hipLaunchKernelGGL((few_k<T, DP, DC, FEW, 1, true>), grid, dim3(64 * FEW), 0, s, a, S, g);
+        hipLaunchKernelGGL((few_k<T, DP, DC, NW, true>), grid, dim3(64 * NW), 0, s, a, S, g);
     else
         hipLaunchKernelGGL((rows_k<T, DP, DC, 4>), grid, dim3(256), 0, s, a, S, g);
     if (c.most > 1 && !fused) {
