@@ -525,11 +525,12 @@ struct Wave {
 // 16384 tokens x 16 heads of 128, causal, f16: 1.08 ms, 1017 TFLOP/s, 80% of what a 16384^3 product reaches; the matrix cores are
 // busy 57% of the cycles at 1.7 GHz, to which the card's power takes the clock: nine orderings of the step are within 2%, and
 // without any softmax the same products take 0.95 ms. 32 rows a wave: 64 would halve the LDS readings (256 bytes a cycle: half
-// used) but spill. Tiles of 64 keys (32 above 128 dimensions, where o takes half the registers). Nine prompts of 269 to 2048
+// used) but spill. Tiles of 64 keys, 32 above 128 dimensions, where o takes half the registers; two waves a SIMD up to 192
+// dimensions (one: 274 us, two: 216, 2 x 4000 tokens x 16 heads), one above (two spill). Nine prompts of 269 to 2048
 // tokens x 32 heads, bf16: 202 us, 797 TFLOP/s; a fifth of a workgroup's cycles is its start and end (finding its tile, first
 // loads, queries, output).
 template <class T, int DP, int DC, int NW>
-__global__ void __launch_bounds__(64 * NW, DP > 128 ? 1 : 2) rows_k(AttentionArgs A, Split S, Group group) {
+__global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * NW, TB = KT * DP * 2, CPR = DP / 8, NK = KT / 32;
     constexpr int NL = KT * CPR / (64 * NW);  // loads a wave issues for a tile of keys, or of values
     using W = Wave<T, DP, DC, KT>;
