@@ -972,9 +972,12 @@ static int checked(const AttentionArgs* a) {
 constexpr int COUNTERS = PCX_ATTENTION_COUNTERS;
 
 // The kernel and the split of a call, by the lengths that the caller expects.
-//  few_k: up to 64 rows of a key head (16 queries x 4 heads over 8000 keys: rows_k 27 us, few_k 22; 64 x 4: 30 and 40), and at 64
-//  dimensions, where two of its workgroups share a CU, prompts whose tiles of 128 rows would not fill the chip (1024 tokens x 12
-//  heads: 21 and 14 us; 2048: 32 and 26; at 128 dimensions, 500 tokens x 32: 16 and 22).
+//  few_k: up to 32 rows of a key head; up to 128, whose tiles of 32 each read the keys, where those tiles are no more than the CUs
+//  (rows_k and few_k in us: 16 queries x 32/8 heads over 8000 keys 24 and 19, 24 queries 24.8 and 21.5, 6 x 25 queries of 256
+//  dimensions over 2000 41 and 30; but 30 x 16 queries over 1000 30 and 50) and above 64 rows the keys not many (24 queries over
+//  16000 31 and 26, 32 over 50000 62 and 78); and at 64 dimensions, where two of its workgroups share a CU, prompts whose tiles
+//  of 128 rows would not fill the chip (1024 tokens x 12 heads: 22 and 13; 2048: 34 and 25; at 128 dimensions, 500 tokens x 32:
+//  16 and 22).
 //  Splits: few_k to 256 workgroups, one a CU (131072 keys x 8 key heads: 192 or 256 workgroups 103 us, 384 114, 512 111) of at
 //  least 384 keys (512 keys in two parts: 11.3 -> 13 us; 2000 in five: 18.2 -> 15.7); rows_k to 512 of at least 512 keys (64 x 4
 //  rows over 8000 keys: no split 166 us, 256 workgroups 32.5, 512 29.5; 2000 tokens x 32 heads: none 49, two parts 71).
@@ -993,7 +996,9 @@ static Choice choose(const AttentionArgs& a) {
     const int group = a.heads / a.kv_heads;
     Choice c;
     const int64_t rows = (int64_t)a.max_q * group, tiles = (int64_t)a.tokens * group / 128 + a.seqs;
-    c.few = rows <= 64 || (a.dim <= 64 && tiles * a.kv_heads < 256);
+    const int64_t work = std::min<int64_t>((rows + 31) / 32, 5) * a.seqs * a.kv_heads;
+    c.few = rows <= 32 || (rows <= 128 && work <= 256 && (rows <= 64 || work * a.max_k <= 3 << 18)) ||
+            (a.dim <= 64 && tiles * a.kv_heads < 256);
     c.BM = c.few ? 32 : 128;
     c.items = (int64_t)a.tokens * group / c.BM + a.seqs;
     // the tiles there are likely to be, half a tile of each sequence's last one unused: one too many and a quarter of the chip may
