@@ -522,13 +522,15 @@ struct Wave {
 // sums are made again (repair) before the rest is added. The scores of tile t - 1 are made in tile t's step, beside its
 // exponentials, so that a wave has matrix and vector work at once.
 //
-// 16384 tokens x 16 heads of 128, causal, f16: 1.08 ms, 1017 TFLOP/s, 80% of what a 16384^3 product reaches; the matrix cores are
-// busy 57% of the cycles at 1.7 GHz, to which the card's power takes the clock: nine orderings of the step are within 2%, and
-// without any softmax the same products take 0.95 ms. 32 rows a wave: 64 would halve the LDS readings (256 bytes a cycle: half
-// used) but spill. Tiles of 64 keys, 32 above 128 dimensions, where o takes half the registers; two waves a SIMD up to 192
-// dimensions (one: 274 us, two: 216, 2 x 4000 tokens x 16 heads), one above (two spill). Nine prompts of 269 to 2048
-// tokens x 32 heads, bf16: 202 us, 797 TFLOP/s; a fifth of a workgroup's cycles is its start and end (finding its tile, first
-// loads, queries, output).
+// 16384 tokens x 16 heads of 128, causal, f16: 1.02 to 1.10 ms by the card, 1080 to 1000 TFLOP/s (a 16384^3 product: 1267); the
+// matrix cores are busy 59% of the cycles at the 1.6 to 1.75 GHz to which the card's power takes the clock, and without any
+// softmax the same products take 0.95 ms. 32 rows a wave: 64 would halve the LDS readings (256 bytes a cycle: half used) but
+// spill. One wave of two a SIMD needs 2500 cycles for a step whose products take 1050 and whose vector instructions take 1100:
+// two hide each other's waits (four buffers for one wave a SIMD: 197 -> 286 us, the packed prompts below). Tiles of 64 keys, 32
+// above 128 dimensions, where o takes half the registers (64 at 256: 321 -> 402 us; 32 at 128: 1107 -> 1132); two waves a SIMD up
+// to 192 dimensions (one: 274 us, two: 216, 2 x 4000 tokens x 16 heads), one above (two spill). Nine prompts of 269 to 2048
+// tokens x 32 heads, bf16: 189 to 198 us, 850 to 815 TFLOP/s; a fifth of a workgroup's cycles is its start and end (finding its
+// tile, first loads, queries, output).
 template <class T, int DP, int DC, int NW>
 __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArgs A, Split S, Group group) {
     constexpr int KT = DP > 128 ? 32 : 64, BM = 32 * NW, TB = KT * DP * 2, CPR = DP / 8, NK = KT / 32;
