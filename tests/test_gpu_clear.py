@@ -246,6 +246,17 @@ def test_attention(ops, kind, causal, shape):
     run_attention(ops, kind, dim, heads, kv, spans, causal)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,heads,kv,spans", [
+    (128, 8, 2, [(32, 900)]), (128, 8, 2, [(16, 1500), (9, 33)]), (192, 4, 1, [(30, 500), (7, 64)]), (136, 4, 2, [(150, 330)]),
+    (192, 3, 1, [(43, 43), (300, 300)]), (256, 4, 1, [(25, 700)]), (64, 8, 1, [(100, 1300)]), (32, 4, 1, [(128, 128)] * 3)])
+def test_attention_between_few_rows_and_many(ops, kind, dim, heads, kv, spans):
+    """33 to 128 rows of a key head and a little more, with the keys split and whole; widths between 129 and 192"""
+    say(f"[clear] attention {kind} dim {dim} heads {heads}/{kv} {spans}")
+    for causal in (True, False):
+        run_attention(ops, kind, dim, heads, kv, spans, causal)
+
+
 @pytest.mark.parametrize("order", ["padded", "heads"])
 @pytest.mark.parametrize("dim,heads,kv,spans", [
     (128, 8, 2, [(1, 100), (1, 33), (1, 64)]), (64, 4, 4, [(90, 90), (30, 200)]), (80, 6, 2, [(50, 70), (1, 40)])])
