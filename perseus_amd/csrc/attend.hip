@@ -981,7 +981,8 @@ constexpr int COUNTERS = PCX_ATTENTION_COUNTERS;
 //  of 128 rows would not fill the chip (1024 tokens x 12 heads: 22 and 13; 2048: 34 and 25; at 128 dimensions, 500 tokens x 32:
 //  16 and 22).
 //  Splits: few_k to 256 workgroups, one a CU (131072 keys x 8 key heads: 192 or 256 workgroups 103 us, 384 114, 512 111) of at
-//  least 384 keys (512 keys in two parts: 11.3 -> 13 us; 2000 in five: 18.2 -> 15.7); rows_k to 512 of at least 512 keys (64 x 4
+//  least 384 keys, 48 a wave (4500 keys x 8 key heads: 256 a part 17.2 us, 384 14.4, the rest alike), 192 above 128 dimensions,
+//  where the waves are 4 (2000 keys x 2 key heads of 256: 384 19.4, 192 16.6); rows_k to 512 of at least 512 keys (64 x 4
 //  rows over 8000 keys: no split 166 us, 256 workgroups 32.5, 512 29.5; 2000 tokens x 32 heads: none 49, two parts 71).
 struct Choice {
     bool few;       // few_k, else rows_k
@@ -1009,7 +1010,8 @@ static Choice choose(const AttentionArgs& a) {
     const int64_t guess = std::min((rows + c.BM - 1) / c.BM * a.seqs, ((int64_t)a.tokens * group + spare) / c.BM);
     c.base = std::max<int64_t>(a.seqs, guess) * a.kv_heads;
     const int64_t want = c.few ? 256 : 512;
-    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(c.base, 1), a.max_k / (c.few ? 384 : 512)));
+    const int shortest = !c.few ? 512 : a.dim > 128 ? 192 : 384;
+    c.most = (int)std::max<int64_t>(1, std::min<int64_t>(want / std::max<int64_t>(c.base, 1), a.max_k / shortest));
     c.size = (int)(((int64_t)a.max_k + c.most - 1) / c.most);
     return c;
 }
