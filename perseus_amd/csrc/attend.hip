@@ -147,6 +147,16 @@ struct Split {
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 
+// tiles of KT keys that n keys take, and the keys of so many tiles: up to 2^31, one more than an int holds
+template <int KT>
+__device__ __forceinline__ int tiles_of(int n) {
+    return (int)(((uint32_t)n + KT - 1) / KT);
+}
+template <int KT>
+__device__ __forceinline__ int keys_of(int tiles, int most) {
+    return (int)min((uint32_t)tiles * KT, (uint32_t)most);
+}
+
 // inclusive sums over the lanes of a wave, and the largest value (by data-parallel moves: no trip through LDS)
 template <int CTRL, int ROWS>
 __device__ __forceinline__ int moved(int x) {
@@ -426,13 +436,13 @@ struct Wave {
     // The rare repair of the tiles that a row sees in part. There o^T += V^T p^T multiplies values that a row does not see by
     // zero, which is not zero where they are infinite or NaN. If o came out so, o of these keys (from key0 to each row's
     // limit, a tile of KT in every `step`) is summed again from memory, key by key, each row its own.
-    static __device__ __forceinline__ void repair(const AttentionArgs& A, const Work& w, int kvh, float c, int key0, int key1,
-                                               int step, Rows<T, DC>& R) {
+    static __device__ __forceinline__ void repair(const AttentionArgs& A, const Work& w, int kvh, float c, uint32_t key0,
+                                               uint32_t key1, uint32_t step, Rows<T, DC>& R) {
         const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
         for (int d = 0; d < DC / 32; ++d) R.o[d] = (v16f)0.0f;
-        for (int t0 = key0; t0 < key1; t0 += step)
-            for (int j = t0; j < t0 + KT && j < key1; ++j) {
+        for (uint32_t t0 = key0; t0 < key1; t0 += step)
+            for (uint32_t j = t0; j < t0 + KT && j < key1; ++j) {
                 const T* k = at<T>(A.k, w.k0 + j, kvh);
                 const T* v = at<T>(A.v, w.k0 + j, kvh);
                 float z = 0;
@@ -445,7 +455,7 @@ struct Wave {
                     }
                 }
                 z += other(z);
-                if (j >= R.lim) continue;
+                if ((int)j >= R.lim) continue;
                 const float p = __builtin_amdgcn_exp2f(fmaf(z, c, R.nm));
 #pragma unroll
                 for (int d = 0; d < DC / 32; ++d)
@@ -544,7 +554,7 @@ __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArg
     const int R = w.n * group.n, r0 = w.tile * BM, mine = r0 + wave * 32;
     const float c = A.scale * 1.4426950408889634f;
     const int last = r0 + BM < R ? r0 + BM : R;
-    const int all = (seen(w, last - 1, group, A.causal) + KT - 1) / KT;
+    const int all = tiles_of<KT>(seen(w, last - 1, group, A.causal));
     int first = 0, tiles = all;
     if (w.nc > 1) {
         first = (int)((int64_t)all * w.chunk / w.nc);
@@ -586,7 +596,7 @@ __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArg
     row.begin(A, w, kvh, group, mine + (lane & 31));
     // the keys [0, hi) are seen by rows of this wave; tiles below `whole` by every row of the workgroup: they need no mask
     const int sees = mine < R ? seen(w, mine + 31, group, A.causal) : 0;
-    const int hi = sees < tiles * KT ? sees : tiles * KT;
+    const int hi = keys_of<KT>(tiles, sees);
     const int every = seen(w, r0, group, A.causal) / KT;
     const int whole = clampi(every, first, tiles);
 
@@ -609,7 +619,7 @@ __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArg
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb) z[kb] = zn[kb];
     }
-    if (A.causal && hi > whole * KT && W::broken(row)) W::repair(A, w, kvh, c, whole * KT, hi, KT, row);
+    if (A.causal && tiles_of<KT>(hi) > whole && W::broken(row)) W::repair(A, w, kvh, c, whole * KT, hi, KT, row);
     settled();
     float top = hi ? W::largest_of(z) : 0;
     // a step: tile t's weights and values, the scores of the one before; odd: t & 1
@@ -711,13 +721,13 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     const float c = A.scale * 1.4426950408889634f;
     const int rn = R - r0 < BM ? R - r0 : BM;
     const int sees = seen(w, r0 + rn - 1, group, A.causal);
-    const int all = (sees + KT - 1) / KT;
+    const int all = tiles_of<KT>(sees);
     int first = 0, tiles = all;
     if (w.nc > 1) {
         first = (int)((int64_t)all * w.chunk / w.nc);
         tiles = (int)((int64_t)all * (w.chunk + 1) / w.nc);
     }
-    const int hi = sees < tiles * KT ? sees : tiles * KT;
+    const int hi = keys_of<KT>(tiles, sees);
     const int lo = seen(w, r0, group, A.causal);
     const int whole = lo / KT > first ? lo / KT : first;
     uint32_t ko[NL], vo[NL];
@@ -754,7 +764,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
         unchecked = false;
         if (W::broken(row)) {
             const int from = TWICE ? first : whole, skip = from - first > wave ? (from - first - wave + NW - 1) / NW : 0;
-            W::repair(A, w, kvh, c, (first + wave + skip * NW) * KT, hi, KT * NW, row);
+            W::repair(A, w, kvh, c, (uint32_t)(first + wave + skip * NW) * KT, hi, KT * NW, row);
             settled();
         }
     };
@@ -772,7 +782,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
         }
         if (t >= whole) {
             W::mask(row, t * KT, z);
-            unchecked |= A.causal && (t + 1) * KT > lo && lo < w.len;
+            unchecked |= A.causal && lo < w.len;
         } else if (!TWICE && unchecked) {
             mend();
         }
