@@ -25,6 +25,7 @@ namespace clear {
 
 constexpr int DMAX = 256;
 constexpr int64_t TOKEN_MAX = 1 << 22;  // key rows' distance, in elements: a tile's byte offsets stay in 32 bits
+constexpr int64_t ROWS_MAX = 0x7fffffff - 127;  // query heads: the last row of a tile of 128 stays in 31 bits
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -976,7 +977,7 @@ static int checked(const AttentionArgs* a) {
         if ((uintptr_t)r->base % 16 || r->token % 8 || r->head % 8) return -2;
     if (!apart(a->out, a->tokens, a->heads, a->dim)) return -2;
     if (a->k.token > TOKEN_MAX || a->v.token > TOKEN_MAX) return -2;
-    if ((int64_t)a->tokens * a->heads > 0x7fffffff) return -2;
+    if ((int64_t)a->tokens * a->heads > ROWS_MAX) return -2;
     if ((uintptr_t)a->work % 16) return -2;
     return 0;
 }
