@@ -1,0 +1,16 @@
+"""The ends of the clear side's ranges without a GPU: what its entries refuse there is decided before any device call, so the
+addresses are never dereferenced."""
+import ctypes as C
+
+import pytest
+
+from perseus_amd._lib import LIB
+from tests.test_clear import attention_args
+
+
+@pytest.mark.parametrize("tokens,heads,kv", [(2 ** 31 - 1, 1, 1), (2 ** 31 - 127, 1, 1), (2 ** 28, 8, 2), (2 ** 29 - 31, 4, 1)])
+def test_attention_refuses_rows_near_2_31(tokens, heads, kv):
+    """a tile of 128 rows that ends past 2^31 - 1"""
+    a = attention_args(tokens=tokens, heads=heads, kv_heads=kv, q_token=64 * heads, out_token=64 * heads)
+    assert LIB.pcx_attention(C.byref(a), None) == -2
+    assert LIB.pcx_attention_workspace(C.byref(a)) == 0
