@@ -1155,7 +1155,8 @@ int pcx_qk_norm_rotary(const QkNormRotaryArgs* args, pc_stream_t s);
  * the caller expects: they choose kernels and splits and no result depends on them beyond the order of its sums.
  *
  * Types bf16 and f16 (q, k, v, out alike); dim a multiple of 8 up to 256; base addresses of 16 bytes and strides of
- * whole 16-byte groups, key and value rows at most 2^22 elements apart; tokens heads < 2^31 - 127; scale > 0 and finite.
+ * whole 16-byte groups, key and value rows at most 2^22 elements apart; tokens heads < 2^31 - 127, kv_heads
+ * < 2^23, tokens heads / (32 kv_heads) + seqs <= 2^31 - 2^16; scale > 0 and finite.
  * work (of work_bytes, 16-byte aligned) holds the partial sums where keys are split over the chip:
  * pcx_attention_workspace's bytes let the call choose its splits freely, with less it splits less (NULL, 0: never). Its
  * first PCX_ATTENTION_COUNTERS words are zero before its first use; every call leaves them so. One workspace serves one

@@ -26,6 +26,8 @@ namespace clear {
 constexpr int DMAX = 256;
 constexpr int64_t TOKEN_MAX = 1 << 22;  // key rows' distance, in elements: a tile's byte offsets stay in 32 bits
 constexpr int64_t ROWS_MAX = 0x7fffffff - 127;  // query heads: the last row of a tile of 128 stays in 31 bits
+constexpr int64_t ITEMS_MAX = 0x7fffffff - 65535;  // (sequence, tile, part): their number in a grid of rows of 65535
+constexpr int32_t KV_HEADS_MAX = (1 << 23) - 1;  // a grid's threads in one dimension, 512 to a key head: below 2^32
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
@@ -978,6 +980,8 @@ static int checked(const AttentionArgs* a) {
     if (!apart(a->out, a->tokens, a->heads, a->dim)) return -2;
     if (a->k.token > TOKEN_MAX || a->v.token > TOKEN_MAX) return -2;
     if ((int64_t)a->tokens * a->heads > ROWS_MAX) return -2;
+    if (a->kv_heads > KV_HEADS_MAX) return -2;
+    if (a->kv_heads && (int64_t)a->tokens * (a->heads / a->kv_heads) / 32 + a->seqs > ITEMS_MAX) return -2;
     if ((uintptr_t)a->work % 16) return -2;
     return 0;
 }
@@ -1031,11 +1035,10 @@ template <class T, int DP, int DC>
 static int run_t(const AttentionArgs& a, hipStream_t s) {
     const int group = a.heads / a.kv_heads;
     Choice c = choose(a);
-    while (c.most > 1 && work_bytes(a, c) > (a.work ? a.work_bytes : 0)) c.most = c.most / 2;
+    while (c.most > 1 && (work_bytes(a, c) > (a.work ? a.work_bytes : 0) || c.items * c.most > ITEMS_MAX)) c.most = c.most / 2;
     if (c.most > 1) c.size = (int)(((int64_t)a.max_k + c.most - 1) / c.most);
     const Group g = {group, 1.0 / group};
     const int64_t tall = c.items * c.most, high = std::min<int64_t>(tall, 65535), deep = (tall + high - 1) / high;
-    if (deep > 65535) return -2;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)high, (unsigned)deep);
     constexpr int NW = DP > 128 ? 4 : 8;
     // joined by the last part where its workgroup reads them all at once: 12 sequences x 2 parts 41 -> 35 us, 5 parts of 4 rows

@@ -14,3 +14,13 @@ def test_attention_refuses_rows_near_2_31(tokens, heads, kv):
     a = attention_args(tokens=tokens, heads=heads, kv_heads=kv, q_token=64 * heads, out_token=64 * heads)
     assert LIB.pcx_attention(C.byref(a), None) == -2
     assert LIB.pcx_attention_workspace(C.byref(a)) == 0
+
+
+@pytest.mark.parametrize("bad", [
+    dict(seqs=2 ** 31 - 1), dict(seqs=2 ** 31 - 65535), dict(seqs=2 ** 31 - 2 ** 25, tokens=2 ** 29, heads=2, kv_heads=1, q_token=128, out_token=128),
+    dict(heads=2 ** 23, kv_heads=2 ** 23, q_token=2 ** 29, out_token=2 ** 29, k_token=2 ** 22, k_head=0, v_token=2 ** 22, v_head=0)])
+def test_attention_refuses_what_no_grid_holds(bad):
+    """more (sequence, tile) pairs than 31 bits number, more key heads than 32 bits of threads take"""
+    a = attention_args(**bad)
+    assert LIB.pcx_attention(C.byref(a), None) == -2
+    assert LIB.pcx_attention_workspace(C.byref(a)) == 0
