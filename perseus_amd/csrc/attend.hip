@@ -37,12 +37,16 @@ typedef float v8f __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 #define PCH_LDS __attribute__((address_space(3)))
 
+// BELOW: how far under a row's largest score (log2 units) the m is kept that its weights exp2(z - m) are taken from. f16 ends
+// at 2^-25, half its smallest step: with m at the largest score 31 weights of 2^-25.2 beside a 1 were lost whole (an output of
+// 8.7e-4 came as 0); 7 below they begin at 2^-32 of the largest, and end, m lagging by up to 8, at 2^15, within f16.
 template <class T>
 struct Mat;
 template <>
 struct Mat<bf16> {
     typedef bf16 v8 __attribute__((ext_vector_type(8)));
     typedef bf16 v4 __attribute__((ext_vector_type(4)));
+    static constexpr float BELOW = 0;
     static __device__ __forceinline__ v16f mul(v8 a, v8 b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
@@ -51,6 +55,7 @@ template <>
 struct Mat<f16> {
     typedef f16 v8 __attribute__((ext_vector_type(8)));
     typedef f16 v4 __attribute__((ext_vector_type(4)));
+    static constexpr float BELOW = 7;
     static __device__ __forceinline__ v16f mul(v8 a, v8 b, v16f c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
@@ -301,7 +306,7 @@ template <class T, int DC>
 struct Rows {
     typename Mat<T>::v8 q[DC / 16];
     v16f o[DC / 32];
-    float m, nm, l;  // running maximum (log2 units), its negative (0 where there is none yet), this half's sum
+    float m, nm, l;  // running maximum less BELOW (log2 units), its negative (0 where there is none yet), this half's sum
     int lim;         // keys seen
 
     // row: this lane's in the sequence (past the last one: the last one's again, its result not kept)
@@ -371,8 +376,8 @@ struct Wave {
             }
     }
 
-    // z becomes exp2(c z - m); m follows the largest score where it has grown by more than 8 (2^8 holds in every type, and
-    // most tiles then need no rescaling)
+    // z becomes exp2(c z - m); m follows the largest score where it has grown by more than 8 (2^8 times as much holds in every
+    // type, and most tiles then need no rescaling)
     static __device__ __forceinline__ void softmax(Rows<T, DC>& R, float c, v16f (&z)[NK]) {
         grow(R, c, largest_of(z));
         weigh(R, c, z);
@@ -386,7 +391,7 @@ struct Wave {
         return top;
     }
     static __device__ __forceinline__ void grow(Rows<T, DC>& R, float c, float top) {
-        top = fmaxf(top, other(top)) * c;
+        top = fmaf(fmaxf(top, other(top)), c, -Mat<T>::BELOW);
         if (__any(top > R.m + 8.0f)) {
             const float mn = fmaxf(R.m, top);
             const float r = mn == R.m ? 1.0f : __builtin_amdgcn_exp2f(R.m - mn);

@@ -5,7 +5,7 @@ import pytest
 
 import perseus_amd as pa
 from tests import clear_oracle as co
-from tests.test_gpu_clear import say
+from tests.test_gpu_clear import placed, say
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,61 @@ def test_attention_of_key_runs_up_to_31_bits(ops, dim, queries, causal, short):
     # 256 parts of either sum joined in f32, a division and the store's rounding; the logarithm's own error
     co.check(out.numpy(ops.stream), want, (co.UNIT["f16"] + 600 * co.E) * np.abs(want), "out")
     co.check(lse.numpy(ops.stream), np.log(seen)[:, None], 600 * co.E + 4 * co.E * 22, "lse")
+
+
+def attend(ops, kind, q, k, v, causal=True, scale=1.0, order="rows"):
+    """one sequence: (out, lse, and the oracle's out, lse, bounds' parts)"""
+    T, H, D = q.shape
+    dq, dk, dv = (placed(a, kind, order) for a in (q, k, v))
+    out, lse = placed(np.full((T, H, D), 9.0), kind, order), pa.Array((T, H), "f32")
+    ops.attention(dq, dk, dv, pa.Array.of(np.array([0, T]), "i32"), pa.Array.of(np.zeros(1), "i64"),
+                  pa.Array.of(np.array([len(k)]), "i32"), out, lse, scale=scale, causal=causal)
+    return (out.numpy(ops.stream), lse.numpy(ops.stream)) + co.attention(q, k, v, [(0, T, 0, len(k))], H // k.shape[1], scale,
+                                                                         causal)
+
+
+def small_weights_bound(out, spread, dlse, lost, twice):
+    """f16: the store's rounding; each weight's, relative, or (twice: what it leaves is a second product) its square; what falls
+    below half a subnormal step; the scores' errors and the f32 sums"""
+    u = co.UNIT["f16"]
+    n = 2 * dlse[..., None]
+    return u * np.abs(out) + co.TINY["f16"] + spread * ((u * u if twice else u) + n + 4 * co.E) + lost
+
+
+@pytest.mark.parametrize("queries,dim,keys,above", [
+    (1, 64, 131072, 17.5), (1, 128, 131072, 17.5), (2, 256, 60000, 17.0), (1, 64, 2000, 16.5), (200, 128, 100000, 17.5),
+    (150, 192, 40000, 17.0), (300, 64, 3000, 17.5), (1100, 32, 1100, 17.5)])
+def test_f16_attention_of_many_small_weights(ops, queries, dim, keys, above):
+    """one key in 32 far above the others, with a value of 0: the output is made of the others' weights, and none may be lost,
+    though each is below what f16 holds beside 1. A row's largest weight is 2^7 or more, so that half a subnormal step is 2^-32 of
+    it, for each key, over the sum of the weights."""
+    say(f"[clear] attention f16, {keys} keys, one in 32 {above} nats above the others, {queries} queries, dim {dim}")
+    rng = np.random.default_rng(keys + dim)
+    heads = 12 if dim == 32 else 1
+    q = np.zeros((queries, heads, dim), np.float32)
+    q[..., 0] = 4
+    k = np.zeros((keys, heads, dim), np.float32)
+    v = co.rounded(1000 * (1 + 0.25 * rng.random((keys, heads, dim))), "f16")
+    k[31::32, :, 0] = co.rounded(above / 4, "f16")
+    v[31::32] = 0
+    got, gl, want, wl, spread, dlse = attend(ops, "f16", q, k, v, causal=False)
+    lost = keys * 2.0 ** -32 * 1250 / (keys // 32)
+    co.check(got, want, small_weights_bound(want, spread, dlse, lost, queries <= 32), "out")
+    co.check(gl, wl, dlse, "lse")
+
+
+@pytest.mark.parametrize("queries,dim", [(1, 64), (3, 128), (200, 128), (300, 64), (150, 256)])
+@pytest.mark.parametrize("step", [7.9, 8.1, 15.0])
+def test_f16_attention_where_the_maximum_grows_late(ops, queries, dim, step):
+    """the last keys, which are taken first, lie `step` powers of two below the first ones: weights beyond 1 while the running
+    maximum lags behind must not leave f16"""
+    say(f"[clear] attention f16, maxima that grow by 2^{step}, {queries} queries, dim {dim}")
+    keys, rng = 700, np.random.default_rng(dim)
+    q = np.zeros((queries, 1, dim), np.float32)
+    q[..., 0] = 4
+    k = np.zeros((keys, 1, dim), np.float32)
+    k[:64, 0, 0] = co.rounded(step * np.log(2) / 4, "f16")
+    v = co.rounded(rng.normal(size=(keys, 1, dim)) * 1000, "f16")
+    got, gl, want, wl, spread, dlse = attend(ops, "f16", q, k, v)
+    co.check(got, want, small_weights_bound(want, spread, dlse, keys * 2.0 ** -32 * 4e3, queries <= 32), "out")
+    co.check(gl, wl, dlse, "lse")
