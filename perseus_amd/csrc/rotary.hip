@@ -204,7 +204,7 @@ static int run_t(const Pass& a, hipStream_t s) {
         const int64_t blocks = ((int64_t)a.tokens * all + WAVES - 1) / WAVES;
         // outputs that no L2 holds until they are read go past the caches: 84 MB 38.5 -> 35.3 us, 168 MB 83 -> 78
         const bool past = (int64_t)a.tokens * a.total * a.dim * sizeof(T) > 32 << 20;
-        if (blocks <= 0x3fffffff) {
+        if (blocks < 1 << 24) {  // fewer than 2^32 threads: more no launch takes, and heads_k goes on by itself
             const dim3 grid((unsigned)blocks);
             if (past)
                 hipLaunchKernelGGL((units_k<T, NORM, INTER, true>), grid, dim3(64 * WAVES), 0, s, a, lph_log, (uint32_t)all);

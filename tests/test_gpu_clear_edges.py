@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import perseus_amd as pa
+from perseus_amd import clear
 from tests import clear_oracle as co
 from tests.test_gpu_clear import placed, say
 
@@ -94,3 +95,21 @@ def test_f16_attention_where_the_maximum_grows_late(ops, queries, dim, step):
     got, gl, want, wl, spread, dlse = attend(ops, "f16", q, k, v)
     co.check(got, want, small_weights_bound(want, spread, dlse, keys * 2.0 ** -32 * 4e3, queries <= 32), "out")
     co.check(gl, wl, dlse, "lse")
+
+
+def test_rotary_of_more_tokens_than_one_grid_takes(ops):
+    """67 million tokens of one short head: 2^24 workgroups of 256 threads and more, which no launch takes"""
+    dim, period, times = 8, 50021, 1342
+    say(f"[clear] rotary of {period * times} tokens of one head of {dim}")
+    rng = np.random.default_rng(8)
+    x = co.rounded(rng.normal(size=(period, 1, dim)), "bf16")
+    pos = rng.integers(0, 100, period).astype(np.int32)
+    table = clear.rotary_table(100, dim)
+    words = clear.to_bf16(x).reshape(-1).view(np.uint32)
+    d = pa.Array((period * times, 1, dim), "bf16")
+    d.buf.upload(np.tile(words, times))
+    ops.rotary(d, pa.Array.of(np.tile(pos, times), "i32"), pa.Array.of(table), d, layout="interleaved")
+    got = d.buf.download(stream=ops.stream).reshape(times, -1)
+    assert (got == got[0]).all(), "the same rows at the same places turned differently"
+    y, mag = co.rotary(x, pos, table, "interleaved")
+    co.check(clear.from_bf16(got[0].view(np.uint16)).reshape(x.shape), y, co.rotary_bound(y, mag, "bf16"))
