@@ -967,7 +967,7 @@ __global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, Group gr
     }
 }
 
-// 0, or the error
+// 0, or the error; the workspace, which its query does not read, apart
 static int checked(const AttentionArgs* a) {
     if (!a || a->tokens < 0 || a->seqs < 0 || a->heads < 0 || a->kv_heads < 0 || a->kv_rows < 0 || a->max_q < 0 ||
         a->max_k < 0)
@@ -987,7 +987,6 @@ static int checked(const AttentionArgs* a) {
     if ((int64_t)a->tokens * a->heads > ROWS_MAX) return -2;
     if (a->kv_heads > KV_HEADS_MAX) return -2;
     if (a->kv_heads && (int64_t)a->tokens * (a->heads / a->kv_heads) / 32 + a->seqs > ITEMS_MAX) return -2;
-    if ((uintptr_t)a->work % 16) return -2;
     return 0;
 }
 
@@ -1097,6 +1096,7 @@ extern "C" uint64_t pcx_attention_workspace(const AttentionArgs* a) {
 
 extern "C" int pcx_attention(const AttentionArgs* a, pc_stream_t s) {
     if (int e = checked(a)) return e;
+    if ((uintptr_t)a->work % 16) return -2;
     if (!a->tokens || !a->seqs || !a->heads) return 0;
     return a->type == PCX_BF16 ? run<bf16>(*a, (hipStream_t)s) : run<f16>(*a, (hipStream_t)s);
 }

@@ -24,3 +24,14 @@ def test_attention_refuses_what_no_grid_holds(bad):
     a = attention_args(**bad)
     assert LIB.pcx_attention(C.byref(a), None) == -2
     assert LIB.pcx_attention_workspace(C.byref(a)) == 0
+
+
+@pytest.mark.parametrize("work", [1, 4, 2 ** 20 + 8])
+def test_the_workspace_query_reads_no_workspace(work):
+    """its bytes for a struct whose work is not set yet; the call itself refuses a workspace that is not aligned"""
+    kw = dict(seqs=1, tokens=1, max_q=1, max_k=100000, kv_rows=100000)
+    want = LIB.pcx_attention_workspace(C.byref(attention_args(**kw)))
+    assert want > 0
+    a = attention_args(work=work, work_bytes=12345, **kw)
+    assert LIB.pcx_attention_workspace(C.byref(a)) == want
+    assert LIB.pcx_attention(C.byref(a), None) == -2
