@@ -967,10 +967,15 @@ __global__ void __launch_bounds__(256) join_k(AttentionArgs A, Split S, Group gr
     }
 }
 
-// 0, or the error; the workspace, which its query does not read, apart
-static int checked(const AttentionArgs* a) {
-    if (!a || a->tokens < 0 || a->seqs < 0 || a->heads < 0 || a->kv_heads < 0 || a->kv_rows < 0 || a->max_q < 0 ||
-        a->max_k < 0)
+// 0 and the arguments with their strides settled, or the error; the workspace, which its query does not read, apart
+static int checked(const AttentionArgs* given, AttentionArgs* a) {
+    if (!given) return -1;
+    *a = *given;
+    a->q = settled(a->q, a->tokens, a->heads, a->dim);
+    a->out = settled(a->out, a->tokens, a->heads, a->dim);
+    a->k = settled(a->k, a->kv_rows, a->kv_heads, a->dim);
+    a->v = settled(a->v, a->kv_rows, a->kv_heads, a->dim);
+    if (a->tokens < 0 || a->seqs < 0 || a->heads < 0 || a->kv_heads < 0 || a->kv_rows < 0 || a->max_q < 0 || a->max_k < 0)
         return -1;
     if (a->type != PCX_BF16 && a->type != PCX_F16) return -2;
     if (a->dim < 8 || a->dim > DMAX || a->dim % 8) return -2;
@@ -1089,14 +1094,16 @@ static int run(const AttentionArgs& a, hipStream_t s) {
 using namespace pch;
 using namespace pch::clear;
 
-extern "C" uint64_t pcx_attention_workspace(const AttentionArgs* a) {
-    if (checked(a) || !a->tokens || !a->seqs || !a->heads) return 0;
-    return work_bytes(*a, choose(*a));
+extern "C" uint64_t pcx_attention_workspace(const AttentionArgs* args) {
+    AttentionArgs a;
+    if (checked(args, &a) || !a.tokens || !a.seqs || !a.heads) return 0;
+    return work_bytes(a, choose(a));
 }
 
-extern "C" int pcx_attention(const AttentionArgs* a, pc_stream_t s) {
-    if (int e = checked(a)) return e;
-    if ((uintptr_t)a->work % 16) return -2;
-    if (!a->tokens || !a->seqs || !a->heads) return 0;
-    return a->type == PCX_BF16 ? run<bf16>(*a, (hipStream_t)s) : run<f16>(*a, (hipStream_t)s);
+extern "C" int pcx_attention(const AttentionArgs* args, pc_stream_t s) {
+    AttentionArgs a;
+    if (int e = checked(args, &a)) return e;
+    if ((uintptr_t)a.work % 16) return -2;
+    if (!a.tokens || !a.seqs || !a.heads) return 0;
+    return a.type == PCX_BF16 ? run<bf16>(a, (hipStream_t)s) : run<f16>(a, (hipStream_t)s);
 }

@@ -12,6 +12,13 @@ using f16 = _Float16;
 inline bool usable(const HeadsRef& r, int64_t tokens, int64_t heads) {
     return (tokens == 0 || heads == 0 || r.base) && r.token >= 0 && r.head >= 0;
 }
+// A reference with the strides of single tokens and heads, which no address is made with and which a view may leave at any
+// value, as a dense tensor's.
+inline HeadsRef settled(HeadsRef r, int64_t tokens, int64_t heads, int64_t dim) {
+    if (tokens < 2) r.token = dim;
+    if (heads < 2) r.head = dim;
+    return r;
+}
 // Whether an output's heads lie apart (a stride of one row only matters where there is a second one).
 inline bool apart(const HeadsRef& r, int64_t tokens, int64_t heads, int64_t dim) {
     if (tokens == 0 || heads == 0) return true;

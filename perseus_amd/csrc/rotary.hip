@@ -255,8 +255,8 @@ extern "C" int pcx_rotary(const RotaryArgs* a, pc_stream_t s) {
     if (!usable(a->x, a->tokens, a->heads) || !usable(a->out, a->tokens, a->heads)) return -1;
     if (!apart(a->out, a->tokens, a->heads, a->dim)) return -2;
     Pass p = {};
-    p.in[0] = a->x;
-    p.out[0] = a->out;
+    p.in[0] = settled(a->x, a->tokens, a->heads, a->dim);
+    p.out[0] = settled(a->out, a->tokens, a->heads, a->dim);
     p.positions = a->positions;
     p.table = a->table;
     p.places = a->places;
@@ -282,8 +282,9 @@ extern "C" int pcx_qk_norm_rotary(const QkNormRotaryArgs* a, pc_stream_t s) {
         return -2;
     if ((int64_t)a->heads + 2 * (int64_t)a->kv_heads > 0x7fffffff) return -2;
     Pass p = {};
-    p.in[0] = a->q, p.in[1] = a->k, p.in[2] = a->v;
-    p.out[0] = a->q_out, p.out[1] = a->k_out, p.out[2] = a->v_out;
+    p.in[0] = settled(a->q, a->tokens, a->heads, a->dim), p.out[0] = settled(a->q_out, a->tokens, a->heads, a->dim);
+    p.in[1] = settled(a->k, a->tokens, a->kv_heads, a->dim), p.out[1] = settled(a->k_out, rows, a->kv_heads, a->dim);
+    p.in[2] = settled(a->v, a->tokens, a->kv_heads, a->dim), p.out[2] = settled(a->v_out, rows, a->kv_heads, a->dim);
     p.w[0] = a->q_weight, p.w[1] = a->k_weight;
     p.positions = a->positions;
     p.table = a->table;

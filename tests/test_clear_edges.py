@@ -35,3 +35,19 @@ def test_the_workspace_query_reads_no_workspace(work):
     a = attention_args(work=work, work_bytes=12345, **kw)
     assert LIB.pcx_attention_workspace(C.byref(a)) == want
     assert LIB.pcx_attention(C.byref(a), None) == -2
+
+
+@pytest.mark.parametrize("one", [
+    dict(tokens=1, q_token=129, out_token=3), dict(kv_rows=1, k_token=2 ** 40, v_token=1),
+    dict(heads=1, kv_heads=1, q_head=5, out_head=2 ** 41, k_head=2 ** 30 + 3, v_head=1),
+    dict(heads=2, kv_heads=1, k_head=7, v_head=9)])
+def test_strides_of_single_rows_are_not_refused(one):
+    """a stride that no address is made with: the workspace query answers as for a dense tensor"""
+    many = dict(tokens=2, seqs=1, max_q=1, max_k=100000, kv_rows=100000)
+    shape = {n: x for n, x in one.items() if n in ("tokens", "heads", "kv_heads", "kv_rows")}
+    want = LIB.pcx_attention_workspace(C.byref(attention_args(**{**many, **shape})))
+    assert want > 0
+    assert LIB.pcx_attention_workspace(C.byref(attention_args(**{**many, **one}))) == want
+    for n in one:  # and still refused where there is a second row
+        if n not in shape:
+            assert LIB.pcx_attention(C.byref(attention_args(**{n: one[n] * 2 + 1})), None) == -2

@@ -113,3 +113,39 @@ def test_rotary_of_more_tokens_than_one_grid_takes(ops):
     assert (got == got[0]).all(), "the same rows at the same places turned differently"
     y, mag = co.rotary(x, pos, table, "interleaved")
     co.check(clear.from_bf16(got[0].view(np.uint16)).reshape(x.shape), y, co.rotary_bound(y, mag, "bf16"))
+
+
+def cut(a, kind, token, head, base=0):
+    """host values [T][H][D] on the device with the strides that are given, NaN around them"""
+    x = pa.Array(a.shape, kind, strides=(token, head, 1))
+    flat = np.full(2 * x.buf.words, np.nan, np.float32)
+    np.lib.stride_tricks.as_strided(flat, a.shape, [4 * token, 4 * head, 4])[...] = a
+    raw = clear.to_bf16(flat) if kind == "bf16" else flat.astype(np.float16)
+    x.buf.upload(raw.view(np.uint32))
+    return x
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 80])
+def test_strides_of_single_tokens_and_heads_do_not_matter(ops, kind, dim):
+    """one token, one head, one key row, as views out of tensors with strides of any kind leave them"""
+    say(f"[clear] strides of dimensions of size 1, {kind} dim {dim}")
+    rng = np.random.default_rng(dim)
+    for T, H, KV, R, qt, qh, kt, kh in ((1, 4, 2, 9, 4 * dim + 3, dim, 2 * dim, dim), (3, 1, 1, 40, dim, 5, 2 * dim + 8, 7),
+                                        (1, 1, 1, 1, 1, 3, 2 ** 22 + 1, 1), (1, 1, 1, 1, 2 ** 40 + 1, 2 ** 41, 2 ** 40, 2 ** 50),
+                                        (1, 6, 1, 33, 3, dim + 8, dim, 1), (150, 1, 1, 150, dim, 9, dim, 9)):
+        q, k, v = (co.rounded(rng.normal(size=s), kind) for s in ((T, H, dim), (R, KV, dim), (R, KV, dim)))
+        dq, dk, dv, out = cut(q, kind, qt, qh), cut(k, kind, kt, kh), cut(v, kind, kt, kh), cut(0 * q, kind, qt, qh)
+        lse = pa.Array((T, H), "f32")
+        ops.attention(dq, dk, dv, pa.Array.of(np.array([0, T]), "i32"), pa.Array.of(np.zeros(1), "i64"),
+                      pa.Array.of(np.array([R]), "i32"), out, lse)
+        want, wl, spread, dlse = co.attention(q, k, v, [(0, T, 0, R)], H // KV, dim ** -0.5, True)
+        co.check(out.numpy(ops.stream), want, co.attention_bound(want, spread, dlse, kind, 5.0), f"out {T} {H} {R}")
+        co.check(lse.numpy(ops.stream), wl, dlse, "lse")
+    table, pos = clear.rotary_table(40, dim), np.array([33])
+    for H, token, head in ((3, 5, dim), (1, 2 ** 40 + 3, 7)):
+        x = co.rounded(rng.normal(size=(1, H, dim)), kind)
+        d = cut(x, kind, token, head)
+        ops.rotary(d, pa.Array.of(pos, "i32"), pa.Array.of(table), d)
+        y, mag = co.rotary(x, pos, table, "half")
+        co.check(d.numpy(ops.stream), y, co.rotary_bound(y, mag, kind), f"rotary {H}")
