@@ -1156,7 +1156,7 @@ int pcx_qk_norm_rotary(const QkNormRotaryArgs* args, pc_stream_t s);
  *
  * Types bf16 and f16 (q, k, v, out alike); dim a multiple of 8 up to 256; base addresses of 16 bytes and strides of
  * whole 16-byte groups, key and value rows at most 2^22 elements apart; tokens heads < 2^31 - 127, kv_heads
- * < 2^23, tokens heads / (32 kv_heads) + seqs <= 2^31 - 2^16; scale > 0 and finite.
+ * < 2^23, tokens heads / (32 kv_heads) + seqs <= 2^31 - 2^16; 0 < scale <= 2.35e38.
  * work (of work_bytes, 16-byte aligned) holds the partial sums where keys are split over the chip:
  * pcx_attention_workspace's bytes let the call choose its splits freely, with less it splits less (NULL, 0: never). Its
  * first PCX_ATTENTION_COUNTERS words are zero before its first use; every call leaves them so. One workspace serves one

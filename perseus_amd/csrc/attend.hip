@@ -979,7 +979,7 @@ static int checked(const AttentionArgs* given, AttentionArgs* a) {
         return -1;
     if (a->type != PCX_BF16 && a->type != PCX_F16) return -2;
     if (a->dim < 8 || a->dim > DMAX || a->dim % 8) return -2;
-    if (!(a->scale > 0) || a->scale > 3e38f) return -1;
+    if (!(a->scale > 0) || a->scale > 2.35e38f) return -1;  // times log2(e), as the kernels take it, finite
     if (a->heads && (a->kv_heads < 1 || a->heads % a->kv_heads)) return -1;
     if (a->seqs && a->tokens && a->heads && (!a->q_start || !a->k_start || !a->k_len)) return -1;
     if (!usable(a->q, a->tokens, a->heads) || !usable(a->out, a->tokens, a->heads) ||

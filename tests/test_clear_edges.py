@@ -51,3 +51,10 @@ def test_strides_of_single_rows_are_not_refused(one):
     for n in one:  # and still refused where there is a second row
         if n not in shape:
             assert LIB.pcx_attention(C.byref(attention_args(**{n: one[n] * 2 + 1})), None) == -2
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 2.9e38, 3e38])
+def test_attention_refuses_a_scale_that_leaves_f32(scale):
+    """scores are taken in powers of two: the scale times log2(e) has to be finite too"""
+    assert LIB.pcx_attention(C.byref(attention_args(scale=scale)), None) == -1
+    assert LIB.pcx_attention(C.byref(attention_args(scale=2.3e38, tokens=0)), None) == 0
