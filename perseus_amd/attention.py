@@ -127,8 +127,9 @@ class ClearBlock:
 
     def __init__(self, ops, heads, kv_heads, dim, capacity, dtype="bf16", table=None, layout="half", q_weight=None,
                  k_weight=None, eps=1e-6):
-        from .clear import Array
+        from .clear import Array, block_checked
 
+        block_checked(heads, kv_heads, dim, capacity, dtype, table, layout, q_weight, k_weight)
         self.ops, self.heads, self.kv_heads, self.dim, self.capacity = ops, heads, kv_heads, dim, capacity
         self.table, self.layout, self.q_weight, self.k_weight, self.eps = table, layout, q_weight, k_weight, eps
         self.k, self.v = (Array((capacity, kv_heads, dim), dtype) for _ in range(2))

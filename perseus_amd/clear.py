@@ -243,6 +243,24 @@ def _table(table, positions, tokens):
             2 * table.shape[1])
 
 
+def block_checked(heads, kv_heads, dim, capacity, dtype, table, layout, q_weight, k_weight):
+    """ValueError for what a block of these sizes could not be appended to, or only with NaN in its cache."""
+    if _type(dtype) not in ("bf16", "f16") or not 8 <= dim <= 256 or dim % 8:
+        raise ValueError(f"{dim} dimensions of {dtype}: attention takes bf16 and f16, a multiple of 8 up to 256")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads on {kv_heads} key heads: a whole number each")
+    if capacity < 1:
+        raise ValueError("capacity: one token or more")
+    _layout(layout)
+    if table is not None:
+        if len(table.shape) != 3 or table.shape[2] != 2 or 2 * table.shape[1] > dim or table.shape[0] < capacity:
+            raise ValueError(f"table: [places][rot / 2][2] with {capacity} places or more and rot up to {dim} is wanted")
+        _flat(table, "table", "f32", None)
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _flat(w, name, "f32", dim)
+
+
 class Clear:
     """The operators on one stream, with a workspace of `workspace` bytes for attention that splits its keys. One Clear
     serves one stream at a time; its calls do not synchronise."""

@@ -4,8 +4,10 @@ import ctypes as C
 
 import pytest
 
+import perseus_amd as pa
+from perseus_amd import attention, clear
 from perseus_amd._lib import LIB
-from tests.test_clear import attention_args
+from tests.test_clear import Fake, NoStream, attention_args
 
 
 @pytest.mark.parametrize("tokens,heads,kv", [(2 ** 31 - 1, 1, 1), (2 ** 31 - 127, 1, 1), (2 ** 28, 8, 2), (2 ** 29 - 31, 4, 1)])
@@ -58,3 +60,31 @@ def test_attention_refuses_a_scale_that_leaves_f32(scale):
     """scores are taken in powers of two: the scale times log2(e) has to be finite too"""
     assert LIB.pcx_attention(C.byref(attention_args(scale=scale)), None) == -1
     assert LIB.pcx_attention(C.byref(attention_args(scale=2.3e38, tokens=0)), None) == 0
+
+
+class HostBuf:
+    """a buffer of no memory, for arrays that are never read"""
+
+    def __init__(self, words):
+        self.words, self.ptr = int(words), C.c_void_p(1 << 20)
+
+    def upload(self, a, stream=None, offset=0):
+        assert offset + a.size <= self.words
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype="f32"), dict(dtype="i32"), dict(dim=60), dict(dim=264), dict(dim=0), dict(heads=5), dict(heads=0, kv_heads=0),
+    dict(kv_heads=0), dict(capacity=0), dict(layout="other"), dict(table=Fake((9, 32, 2), "f32")),
+    dict(table=Fake((10, 33, 2), "f32")), dict(table=Fake((10, 64), "f32")), dict(table=Fake((10, 32, 2), "f16")),
+    dict(q_weight=Fake((32,), "f32")), dict(k_weight=Fake((64,), "bf16"))])
+def test_a_block_that_no_token_could_enter_is_refused(monkeypatch, bad):
+    """when it is made: a table with fewer places than the block holds tokens would put NaN into the cache, a type or width that
+    attention refuses would fail after the cache was written"""
+    monkeypatch.setattr(clear, "DevBuf", HostBuf)
+    good = dict(heads=4, kv_heads=2, dim=64, capacity=10, dtype="f16", table=Fake((10, 32, 2), "f32"))
+    ops = pa.Clear(NoStream, workspace=0)
+    block = attention.ClearBlock(ops, **good)
+    assert block.length == 0 and block.k.shape == (10, 2, 64) and block.out.shape == (10, 4, 64)
+    attention.ClearBlock(ops, **{**good, "table": None})
+    with pytest.raises(ValueError):
+        attention.ClearBlock(ops, **{**good, **bad})
