@@ -166,11 +166,10 @@ class ClearBlock:
                                 None if self.table is None else Array((n,), "i32", self._places.buf, at), self.table, q,
                                 self.k, eps=self.eps, layout=self.layout, v=part(H + KV, KV), v_out=self.v,
                                 slots=Array((n,), "i64", self._slots.buf, 2 * at))
-        self.length = at + n
         runs = self._runs.buf  # (0, n) for every n: a run's start and end, or its second alone as a length
         self.ops.attention(q, self.k, self.v, Array((2,), "i32", runs, 2 * n), self._first,
-                           Array((1,), "i32", runs, 2 * self.length + 1), out, lse, causal=causal, max_q=n,
-                           max_k=self.length)
+                           Array((1,), "i32", runs, 2 * (at + n) + 1), out, lse, causal=causal, max_q=n, max_k=at + n)
+        self.length = at + n  # only now: tokens that failed are appended again at the same places
         return q, out, lse
 
     def keys(self):

@@ -88,3 +88,32 @@ def test_a_block_that_no_token_could_enter_is_refused(monkeypatch, bad):
     attention.ClearBlock(ops, **{**good, "table": None})
     with pytest.raises(ValueError):
         attention.ClearBlock(ops, **{**good, **bad})
+
+
+def test_a_failed_append_leaves_the_block_s_length(monkeypatch):
+    """a caller that tries again appends the same tokens at the same places"""
+    monkeypatch.setattr(clear, "DevBuf", HostBuf)
+    calls = []
+
+    class Ops:
+        stream = NoStream
+
+        def qk_norm_rotary(self, *args, slots, **kw):
+            calls.append(slots.offset)
+
+        def attention(self, *args, max_k, **kw):
+            calls.append(max_k)
+            if len(calls) == 4:
+                raise pa.HipError("attention")
+
+    class Rows(Fake):
+        def __getitem__(self, at):
+            return self
+
+    block, rows = attention.ClearBlock(Ops(), 4, 2, 64, 10), Rows((3, 8, 64))
+    block.append(rows)
+    with pytest.raises(pa.HipError):
+        block.append(rows)
+    assert block.length == 3
+    block.append(rows)
+    assert block.length == 6 and calls == [0, 3, 6, 6, 6, 6]
