@@ -442,8 +442,9 @@ struct Wave {
     }
 
     // The rare repair of the tiles that a row sees in part. There o^T += V^T p^T multiplies values that a row does not see by
-    // zero, which is not zero where they are infinite or NaN. If o came out so, o of these keys (from key0 to each row's
-    // limit, a tile of KT in every `step`) is summed again from memory, key by key, each row its own.
+    // zero, which is not zero where they are infinite or NaN: those of keys that later rows see, or, where rows of values share
+    // memory, seen ones read again past the last key (else zeros are read there). If o came out so, o of these keys (from key0 to
+    // each row's limit, a tile of KT in every `step`) is summed again from memory, key by key, each row its own.
     static __device__ __forceinline__ void repair(const AttentionArgs& A, const Work& w, int kvh, float c, uint32_t key0,
                                                uint32_t key1, uint32_t step, Rows<T, DC>& R) {
         const int h = (threadIdx.x & 63) >> 5;
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArg
 #pragma unroll
         for (int kb = 0; kb < NK; ++kb) z[kb] = zn[kb];
     }
-    if (A.causal && tiles_of<KT>(hi) > whole && W::broken(row)) W::repair(A, w, kvh, c, whole * KT, hi, KT, row);
+    if ((A.causal || A.v.token < A.dim) && tiles_of<KT>(hi) > whole && W::broken(row)) W::repair(A, w, kvh, c, whole * KT, hi, KT, row);
     settled();
     float top = hi ? W::largest_of(z) : 0;
     // a step: tile t's weights and values, the scores of the one before; odd: t & 1
@@ -790,7 +791,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
         }
         if (t >= whole) {
             W::mask(row, t * KT, z);
-            unchecked |= A.causal && lo < w.len;
+            unchecked |= (A.causal && lo < w.len) || A.v.token < A.dim;
         } else if (!TWICE && unchecked) {
             mend();
         }

@@ -149,3 +149,25 @@ def test_strides_of_single_tokens_and_heads_do_not_matter(ops, kind, dim):
         ops.rotary(d, pa.Array.of(pos, "i32"), pa.Array.of(table), d)
         y, mag = co.rotary(x, pos, table, "half")
         co.check(d.numpy(ops.stream), y, co.rotary_bound(y, mag, kind), f"rotary {H}")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("dim,queries,keys,step", [(128, 200, 70, 0), (128, 200, 600, 8), (64, 100, 45, 0), (64, 1, 45, 0), (256, 150, 33, 16), (64, 130, 97, 0)])
+def test_attention_over_values_that_share_memory(ops, kind, dim, queries, keys, step):
+    """one row of values for every key (a token stride of 0), or rows a few values apart: what is read past the last key of a
+    tile are the seen values again, an infinite one among them, and they must count nothing"""
+    say(f"[clear] attention {kind} over values {step} apart, {queries} queries, {keys} keys, dim {dim}")
+    rng = np.random.default_rng(dim + keys)
+    q, k = (co.rounded(rng.normal(size=(n, 1, dim)), kind) for n in (queries, keys))
+    flat = co.rounded(rng.normal(size=dim + step * (keys - 1) + 2), kind)
+    flat[3], flat[dim - 1] = np.inf, -np.inf
+    buf = pa.Array.of(flat, kind).buf
+    dv = pa.Array((keys, 1, dim), kind, buf, strides=(step, dim, 1))
+    v = np.lib.stride_tricks.as_strided(flat, (keys, 1, dim), (4 * step, 4 * dim, 4))
+    for causal in (False, True):
+        out, lse = pa.Array((queries, 1, dim), kind), pa.Array((queries, 1), "f32")
+        ops.attention(pa.Array.of(q, kind), pa.Array.of(k, kind), dv, pa.Array.of(np.array([0, queries]), "i32"),
+                      pa.Array.of(np.zeros(1), "i64"), pa.Array.of(np.array([keys]), "i32"), out, lse, causal=causal)
+        want, wl, spread, dlse = co.attention(q, k, v, [(0, queries, 0, keys)], 1, dim ** -0.5, causal)
+        co.check(out.numpy(ops.stream), want, co.attention_bound(want, spread, dlse, kind, 5.0), f"out, causal {causal}")
+        co.check(lse.numpy(ops.stream), wl, dlse, "lse")
