@@ -1092,7 +1092,8 @@ int pcx_decrypt_rows(pcx_decryptor* x, const void* ct, int K, int top, int which
  * on heads of floating-point values in device memory, in the launchers' manner: they read *args, enqueue on the stream
  * and return 0, -1 for NULL or inconsistent arguments, -2 for sizes, strides or alignments outside the kernels' range,
  * or a positive HIP error; they never allocate, free or synchronise, and may be captured. Arithmetic is in 32 bits,
- * each output rounded once (to nearest even).
+ * each output rounded once (to nearest even); attention's weights alone are rounded on the way (below). The stride of a
+ * dimension of size 1 is not looked at.
  *
  * A tensor [tokens][heads][dim]: element (t, h, d) at base[t token + h head + d], the strides in elements. */
 typedef struct HeadsRef {
@@ -1146,13 +1147,25 @@ int pcx_qk_norm_rotary(const QkNormRotaryArgs* args, pc_stream_t s);
  * where `causal` only j <= k_len[b] - n_b + i (the last query sees the last key, so a chunk or one token appended to a
  * cache is the same call). For each query and head
  *     z_j = scale q . k_j over the keys seen,  lse = log sum_j exp(z_j),  o = sum_j exp(z_j - lse) v_j;
- * where it sees no key o = 0 and lse = -infinity. lse: f32 [tokens][heads], or NULL. Keys and values that a query does
- * not see do not reach it, whatever they hold.
+ * where it sees no key, or only scores of -infinity, o = 0 and lse = -infinity. lse: f32 [tokens][heads], or NULL. Keys
+ * and values that a query does not see do not reach it, whatever they hold.
+ *
+ * Each weight exp(z_j - m), m near the row's largest score, is rounded to the type for its product with v_j, which the
+ * matrix cores take; its sum is of the unrounded ones. That is 2^-8 of a weight at most for bf16, 2^-11 for f16 (where
+ * what lies below 2^-32 of the largest counts 0), about as much again as the output's own rounding. Where a key head has
+ * 32 rows or fewer (max_q heads / kv_heads: tokens, which are bound by the reading of the keys) the product of what the
+ * rounding leaves is added, and the error is the output's rounding alone; so it is for up to 128 rows where few tiles of
+ * them are expected, but for dim <= 64 above 64.
+ *
+ * An infinite value that a query sees makes its output infinite (NaN where its weight is rounded to 0) and costs time:
+ * the keys of the tiles in question are summed again one by one, all of them where weights' remainders are added (one
+ * token over 131072 keys: 103 us, so 1620).
  *
  * The lengths are device arrays, read by the kernels, so that a captured step follows them; what lies outside the
  * buffers (query rows from `tokens` on, key rows from kv_rows on) is cut off. Query rows of no sequence are left
  * unwritten; sequences may not share query rows. max_q and max_k are the longest query run and the longest key run that
- * the caller expects: they choose kernels and splits and no result depends on them beyond the order of its sums.
+ * the caller expects: they choose kernels and splits, and no result depends on them beyond the order of its sums and
+ * whether the weights' remainders are added.
  *
  * Types bf16 and f16 (q, k, v, out alike); dim a multiple of 8 up to 256; base addresses of 16 bytes and strides of
  * whole 16-byte groups, key and value rows at most 2^22 elements apart; tokens heads < 2^31 - 127, kv_heads

@@ -325,7 +325,8 @@ class Clear:
         heads][dim]: sequence b has q's rows q_start[b] .. q_start[b + 1] - 1 (i32) and k's k_start[b] .. + k_len[b] - 1
         (i64, i32; device arrays). causal: the last query sees the last key, each earlier one a key less. scale: 1 /
         sqrt(dim) unless given. max_q, max_k: the longest runs expected (the buffers' rows unless given); they only
-        choose kernels."""
+        choose kernels, which differ in the order of their sums and in whether what the weights' rounding to the type leaves
+        is added (it is for tokens)."""
         args = self._attention(q, k, v, q_start, k_start, k_len, out, lse, scale, causal, max_q, max_k)
         check(LIB.pcx_attention(args, self.stream.h), "attention")
 

@@ -3,12 +3,14 @@
 // For a query q that sees the keys j: z_j = scale q . k_j, m = max z_j, l = sum exp(z_j - m), o = sum exp(z_j - m) v_j / l,
 // lse = m + log l. One pass over the keys holds (m, l, o) and rescales l and o where m grows. Scores, exponentials, sums and o are
 // f32; the weights exp(z_j - m) are rounded to the type for their product with v, which the matrix cores take, and l sums them
-// unrounded. That rounding costs as much again as the output's own (2^-9 relative of each weight for bf16, 2^-12 for f16: the
-// error against 64 bits is 1.3 to 1.4 times that of one rounding). For the rows of a token, which are bound by the reading of the
-// keys, what it leaves is a second product, and the error is that of the output's rounding alone.
+// unrounded. That rounding costs about as much again as the output's own (2^-8 of a weight at most for bf16, 2^-11 for f16: the
+// error against 64 bits is 1.1 to 1.4 times that of one rounding). Where few_k takes rows of a token or a few, which are bound by
+// the reading of the keys, what it leaves is a second product, and the error is that of the output's rounding alone; a second
+// product in rows_k, which is bound by its products, would be half as many again.
 //
-// rows_k takes many rows (prompts, chunks), few_k the rows of a token or two and splits the keys over the chip; join_k joins
-// the parts.
+// few_k takes the rows of tokens, up to 128 of a key head where they are few tiles, and the prompts of 64 dimensions whose tiles
+// of 128 rows would not fill the chip, and splits the keys over waves and workgroups; rows_k takes all others (prompts, chunks) in
+// tiles of 128 rows; join_k joins the parts of both. The rules and their measurements stand at choose().
 //
 // The rows of a tile are the (query, head) pairs of one key head, numbered query * group + head of the group: a tile of rows
 // reads its keys once for the whole group, and one token of a wide group fills a tile as a run of queries does. Everything is
@@ -541,14 +543,14 @@ struct Wave {
 // sums are made again (repair) before the rest is added. The scores of tile t - 1 are made in tile t's step, beside its
 // exponentials, so that a wave has matrix and vector work at once.
 //
-// 16384 tokens x 16 heads of 128, causal, f16: 1.02 to 1.10 ms by the card, 1080 to 1000 TFLOP/s (a 16384^3 product: 1267); the
+// 16384 tokens x 16 heads of 128, causal, f16: 1.02 to 1.13 ms by the card, 1080 to 970 TFLOP/s (a 16384^3 product: 1303); the
 // matrix cores are busy 59% of the cycles at the 1.6 to 1.75 GHz to which the card's power takes the clock, and without any
 // softmax the same products take 0.95 ms. 32 rows a wave: 64 would halve the LDS readings (256 bytes a cycle: half used) but
 // spill. One wave of two a SIMD needs 2500 cycles for a step whose products take 1050 and whose vector instructions take 1100:
 // two hide each other's waits (four buffers for one wave a SIMD: 197 -> 286 us, the packed prompts below). Tiles of 64 keys, 32
 // above 128 dimensions, where o takes half the registers (64 at 256: 321 -> 402 us; 32 at 128: 1107 -> 1132); two waves a SIMD up
 // to 192 dimensions (one: 274 us, two: 216, 2 x 4000 tokens x 16 heads), one above (two spill). Nine prompts of 269 to 2048
-// tokens x 32 heads, bf16: 189 to 198 us, 850 to 815 TFLOP/s; a fifth of a workgroup's cycles is its start and end (finding its
+// tokens x 32 heads, bf16: 189 to 206 us, 850 to 780 TFLOP/s; a fifth of a workgroup's cycles is its start and end (finding its
 // tile, first loads, queries, output).
 template <class T, int DP, int DC, int NW>
 __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArgs A, Split S, Group group) {
@@ -696,7 +698,7 @@ __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArg
 // of the keys: 8 waves (4 above 128 dimensions: 128 KB either way) keep a tile of keys and one of values each on their way or
 // in work, the next keys asked for as soon as the scores are made, the next values after the products (256 dimensions, 16
 // caches of up to 8000: both after the products 40.3 us, so 37.2). 4 waves of two tiles each: 20 caches of up to 4000 56 -> 54
-// us, 131072 keys 104.1 -> 103. One token, 64 heads on 8 key heads of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.0);
+// us, 131072 keys 104.1 -> 103. One token, 64 heads on 8 key heads of 128, 131072 keys: 103 us, 5.2 TB/s (a large copy: 5.6);
 // 48 caches of 89 to 8000 keys: 160 us, 5.1 TB/s. The 32 x 32 products leave most columns unused there; they take a tenth of
 // the time of the reading.
 template <int N>

@@ -28,7 +28,8 @@ constexpr int WAVES = 4;
 // are neighbours. A power of two of lanes takes a head, a wave as many heads of one token as fit: short waves, many of them (a
 // wave that went on to a second and third eight of heads, or a second token, kept fewer loads on their way: 16384 tokens x 40
 // heads 90 to 137 us where this took 84). The bound is the memory: 8191 tokens x 40 heads of 128 in 16 bits 35 us, 4.8 TB/s (a
-// large copy: 5.0); 16384 x 8 heads in 32 bits 29 us, 4.9; with the norms, 16384 x 40 heads out of rows of 48: 78 us, 4.4.
+// large copy: 5.6); 16384 x 8 heads in 32 bits 29 us, 4.9; with the norms, 16384 x 40 heads out of rows of 48: 78 us, 4.4, and
+// all 48, keys and values to rows of a cache: 97 us, 4.25.
 template <class T>
 struct Eight {
     float v[8];
@@ -138,8 +139,9 @@ __global__ void __launch_bounds__(64 * WAVES) units_k(Pass A, int lph_log, uint3
 }
 
 // ------------------------------------------------------------------------------------------------ any size
-// Odd sizes, strides and addresses, what 16-byte accesses do not fit: a wave per head, a lane per pair or copied value (8191
-// tokens x 40 heads of 128 147 us).
+// Odd sizes, strides and addresses, what 16-byte accesses do not fit: a wave per head, a lane per pair or copied value. Halves
+// that are not whole units of 8 too (rot 8, 24, 40, 72 in the half layout): 8191 tokens x 40 heads of 128, rot 24, 114 us (150
+// with three inputs in turn) where units_k takes 36 with rot 32.
 template <class T, bool NORM, bool INTER>
 __global__ void __launch_bounds__(64 * WAVES) heads_k(Pass A) {
     const int lane = threadIdx.x & 63;
