@@ -71,9 +71,13 @@ class Array:
 
     @classmethod
     def of(cls, a, dtype=None, stream=None):
-        """A dense copy of host values: float arrays as f32 unless dtype says bf16 or f16, integers as i32 or i64."""
+        """A dense copy of host values: float arrays as f32 unless dtype says bf16 or f16, integers as i32 or, where that does
+        not hold their type, i64."""
         a = np.asarray(a)
-        dtype = _type(dtype) if dtype else {"i": "i64" if a.dtype.itemsize == 8 else "i32"}.get(a.dtype.kind, "f32")
+        if not dtype:
+            whole = a.dtype.kind in "iu"
+            dtype = "f32" if not whole else "i32" if np.can_cast(a.dtype, np.int32) else "i64"
+        dtype = _type(dtype)
         kind = {"f16": np.float16, "f32": np.float32, "i32": np.int32, "i64": np.int64}
         raw = np.ascontiguousarray(to_bf16(a) if dtype == "bf16" else a.astype(kind[dtype])).tobytes()
         x = cls(a.shape, dtype)

@@ -2,6 +2,7 @@
 addresses are never dereferenced."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 import perseus_amd as pa
@@ -117,3 +118,19 @@ def test_a_failed_append_leaves_the_block_s_length(monkeypatch):
     assert block.length == 3
     block.append(rows)
     assert block.length == 6 and calls == [0, 3, 6, 6, 6, 6]
+
+
+@pytest.mark.parametrize("kind,want", [("u1", "i32"), ("u2", "i32"), ("u4", "i64"), ("u8", "i64"), ("i1", "i32"), ("i4", "i32"), ("i8", "i64")])
+def test_host_integers_stay_integers(monkeypatch, kind, want):
+    """unsigned ones too, in a type that holds them"""
+    got = []
+
+    class Buf(HostBuf):
+        def upload(self, a, stream=None, offset=0):
+            got.append(a.copy())
+
+    monkeypatch.setattr(clear, "DevBuf", Buf)
+    x = np.array([0, 1, np.iinfo(kind).max if kind != "u8" else 2 ** 63 - 1, 77], kind)
+    a = pa.Array.of(x)
+    assert a.dtype == want
+    assert (got[0].view({"i32": np.int32, "i64": np.int64}[want])[:4] == x.astype(np.int64)).all()
