@@ -1194,6 +1194,30 @@ int pcx_attention(const AttentionArgs* args, pc_stream_t s);
  * refuses); work and work_bytes are not read */
 uint64_t pcx_attention_workspace(const AttentionArgs* args);
 
+/* Where the keys of a sequence lie in a cache of rows (an operator's kv_rows or rows of them): key j of sequence b at row
+ * start[b] + j, or, where start is NULL, in pages: at row pages[b pages_seq + j / page_rows] page_rows + j mod page_rows.
+ * page_rows: a power of two, 16 or more; the pool has its rows' whole pages, a sequence at most `width` of them; pages may lie
+ * in any order. Table entries are read up to the page of a sequence's last key. */
+typedef struct CacheRef {
+    const int64_t* start; /* [seqs] */
+    const int32_t* pages; /* [seqs][width] */
+    int64_t pages_seq;
+    int32_t width, page_rows;
+} CacheRef;
+PC_STATIC_ASSERT(sizeof(CacheRef) == 32, "CacheRef layout");
+
+/* pcx_attention over keys and values in pages (cache.start is NULL; attention.k_start is not read): sequence b has the first
+ * k_len[b] keys of its pages, what lies past width page_rows is cut off. Sequences may share pages (a prefix that they have in
+ * common). Keys and values on a page outside the pool read as zeros: such a key's score is 0 and counts. All else is
+ * pcx_attention's, its workspace and counters too; max_k is at most width page_rows. */
+typedef struct AttentionPagedArgs {
+    AttentionArgs attention;
+    CacheRef cache;
+} AttentionPagedArgs;
+PC_STATIC_ASSERT(sizeof(AttentionPagedArgs) == 224, "AttentionPagedArgs layout");
+int pcx_attention_paged(const AttentionPagedArgs* args, pc_stream_t s);
+uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args); /* as pcx_attention_workspace */
+
 /* Stage timing, for measurement: while on, the driver records a HIP event pair on the launch stream around each
  * stage it enqueues (0 ModUp INTT, 1 ModUp conversion, 2 ModUp NTT, 3 key dot, 4 ModDown INTT, 5 ModDown conversion,
  * 6 ModDown NTT + epilogue, 7 CtS baby steps and plaintext products, 8 tensor, 9 rescale). pcx_timing(c, n) turns it

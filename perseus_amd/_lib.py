@@ -134,6 +134,8 @@ _SIGS = {
     "pcx_qk_norm_rotary": (C.c_int, [vp, vp]),
     "pcx_attention": (C.c_int, [vp, vp]),
     "pcx_attention_workspace": (C.c_uint64, [vp]),
+    "pcx_attention_paged": (C.c_int, [vp, vp]),
+    "pcx_attention_paged_workspace": (C.c_uint64, [vp]),
 }
 for _name, (_res, _args) in _SIGS.items():
     _f = getattr(LIB, _name)

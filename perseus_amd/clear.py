@@ -190,6 +190,11 @@ class QkNormRotaryArgs(C.Structure):
                 ("rot", _i32), ("type", _i32), ("interleaved", _i32), ("eps", _f32)]
 
 
+class CacheRef(C.Structure):
+    """include/pc_hip.h CacheRef."""
+    _fields_ = [("start", _vp), ("pages", _vp), ("pages_seq", _i64), ("width", _i32), ("page_rows", _i32)]
+
+
 class AttentionArgs(C.Structure):
     """include/pc_hip.h AttentionArgs."""
     _fields_ = [*_ref("q"), *_ref("k"), *_ref("v"), *_ref("out"), ("lse", _vp), ("q_start", _vp), ("k_start", _vp),
@@ -198,11 +203,18 @@ class AttentionArgs(C.Structure):
                 ("max_q", _i32), ("max_k", _i32), ("scale", _f32)]
 
 
+class AttentionPagedArgs(C.Structure):
+    """include/pc_hip.h AttentionPagedArgs."""
+    _fields_ = [("attention", AttentionArgs), ("cache", CacheRef)]
+
+
 # the same layouts for struct.pack: a call packs its arguments in about a microsecond, a ctypes Structure takes four
 _ROTARY = struct.Struct("@" + "Pqq" * 2 + "PPq" + "i" * 8)
 _QK_NORM_ROTARY = struct.Struct("@" + "Pqq" * 6 + "P" * 5 + "qq" + "i" * 7 + "f")
 _ATTENTION = struct.Struct("@" + "Pqq" * 4 + "P" * 5 + "Qq" + "i" * 9 + "f")
+_CACHE = struct.Struct("@PPqii")
 assert (_ROTARY.size, _QK_NORM_ROTARY.size, _ATTENTION.size) == (104, 232, 192)
+assert _CACHE.size == C.sizeof(CacheRef) == 32
 assert (C.sizeof(RotaryArgs), C.sizeof(QkNormRotaryArgs), C.sizeof(AttentionArgs)) == (104, 232, 192)
 
 
@@ -245,6 +257,21 @@ def _table(table, positions, tokens):
         raise ValueError("table: [places][rot / 2][2] is wanted")
     return (_flat(positions, "positions", "i32", tokens), _flat(table, "table", "f32", None), table.shape[0],
             2 * table.shape[1])
+
+
+def _pages(pages, page_rows, seqs):
+    """(address, distance of two sequences' tables, width) of a table of pages [seqs][width]"""
+    if not pages.is_cuda:
+        raise ValueError("pages: not on the device")
+    if (_known.get(pages.dtype) or _type(pages.dtype)) != "i32" or len(pages.shape) != 2:
+        raise ValueError("pages: a table [sequences][pages] of i32 is wanted")
+    n, width = pages.shape
+    step, inner = pages.stride()
+    if n != seqs or width < 1 or (inner != 1 and width > 1):
+        raise ValueError(f"pages: a row of pages for each of {seqs} sequences, dense, is wanted")
+    if page_rows < 16 or page_rows & (page_rows - 1):
+        raise ValueError(f"page_rows {page_rows}: a power of two, 16 or more")
+    return pages.data_ptr(), step if n > 1 else width, width
 
 
 def block_checked(heads, kv_heads, dim, capacity, dtype, table, layout, q_weight, k_weight):
@@ -338,6 +365,27 @@ class Clear:
         """attention's checked arguments as the struct that pcx_attention and pcx_attention_workspace take."""
         return AttentionArgs.from_buffer_copy(self._attention(*args, **kw))
 
+    def attention_paged(self, q, k, v, q_start, pages, page_rows, k_len, out, lse=None, scale=None, causal=True, max_q=None,
+                        max_k=None):
+        """attention over keys and values in pages: k and v [rows][kv heads][dim] are pools of rows / page_rows pages (page_rows:
+        a power of two, 16 or more), sequence b has the first k_len[b] keys of the pages pages[b] (i32 [sequences][width], any
+        order, shared or not): key j in row pages[b][j / page_rows] page_rows + j % page_rows, the slot that qk_norm_rotary
+        writes it to."""
+        args = self._attention_paged(q, k, v, q_start, pages, page_rows, k_len, out, lse, scale, causal, max_q, max_k)
+        check(LIB.pcx_attention_paged(args, self.stream.h), "attention_paged")
+
+    def attention_paged_args(self, *args, **kw):
+        """attention_paged's checked arguments as the struct that pcx_attention_paged and its workspace query take."""
+        return AttentionPagedArgs.from_buffer_copy(self._attention_paged(*args, **kw))
+
+    def _attention_paged(self, q, k, v, q_start, pages, page_rows, k_len, out, lse=None, scale=None, causal=True, max_q=None,
+                         max_k=None):
+        ptr, step, width = _pages(pages, page_rows, k_len.shape[0])
+        room = min(width * page_rows, 0x7FFFFFFF)
+        max_k = room if max_k is None else min(max_k, room)
+        return self._attention(q, k, v, q_start, None, k_len, out, lse, scale, causal, max_q, max_k) + _CACHE.pack(
+            0, ptr, step, width, page_rows)
+
     def _attention(self, q, k, v, q_start, k_start, k_len, out, lse=None, scale=None, causal=True, max_q=None, max_k=None):
         a, at, ah, qs, kind = _heads(q, "q")
         b, bt, bh, ks, kkind = _heads(k, "k")
@@ -352,7 +400,7 @@ class Clear:
         seqs = k_len.shape[0]
         return _ATTENTION.pack(
             a, at, ah, b, bt, bh, c, ct, ch, d, dt, dh, 0 if lse is None else _flat(lse, "lse", "f32", tokens * heads),
-            _flat(q_start, "q_start", "i32", seqs + 1), _flat(k_start, "k_start", "i64", seqs),
+            _flat(q_start, "q_start", "i32", seqs + 1), 0 if k_start is None else _flat(k_start, "k_start", "i64", seqs),
             _flat(k_len, "k_len", "i32", seqs), *self._work, rows, tokens, seqs, heads, kv, dim, TYPES[kind],
             bool(causal), tokens if max_q is None else max_q, min(rows, 0x7FFFFFFF) if max_k is None else max_k,
             dim ** -0.5 if scale is None else scale)

@@ -25,6 +25,25 @@ inline bool apart(const HeadsRef& r, int64_t tokens, int64_t heads, int64_t dim)
     return (tokens < 2 || r.token >= dim) && (heads < 2 || r.head >= dim);
 }
 
+// A cache in pages, as the kernels take it: sequence b's key j lies in row page[j >> log] << log plus j's low bits, page =
+// table + b seq, of a pool of `count` pages; a sequence has `width` pages at most.
+struct PagesRef {
+    const int32_t* table;
+    int64_t seq;
+    int32_t width, count, log;
+};
+// the pages of a cache of `rows` rows: 0, or the error
+inline int pages_of(const CacheRef& c, int64_t seqs, int64_t rows, PagesRef* p) {
+    if (seqs && !c.pages) return -1;
+    if (c.width < 1 || c.pages_seq < 0 || (seqs > 1 && c.pages_seq < c.width)) return -1;
+    if (c.page_rows < 16 || (c.page_rows & (c.page_rows - 1))) return -2;
+    int log = 4;
+    while (1 << log < c.page_rows) ++log;
+    const int64_t count = rows >> log;
+    *p = {c.pages, c.pages_seq, c.width, (int32_t)(count > 0x7fffffff ? 0x7fffffff : count), log};
+    return 0;
+}
+
 template <class T>
 __device__ __forceinline__ T* at(const HeadsRef& r, int64_t t, int64_t h) {
     return (T*)r.base + t * r.token + h * r.head;

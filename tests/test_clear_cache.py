@@ -1,0 +1,87 @@
+"""The cache's operators without a GPU: what their entries refuse is decided before any device call, so the addresses are never
+dereferenced; the argument structs are the header's."""
+import ctypes as C
+import re
+
+import pytest
+
+import perseus_amd as pa
+from perseus_amd import clear
+from perseus_amd._lib import LIB
+from tests.test_clear import P, Fake, NoStream, attention_args, fill
+
+
+@pytest.fixture
+def ops():
+    return pa.Clear(NoStream, workspace=0)
+
+
+def header_fields(name):
+    """a struct's field names in the header's order, each HeadsRef as three"""
+    text = open(pa._lib.HEADER).read()
+    end = text.index("} %s;" % name)
+    body = re.sub(r"/\*.*?\*/", "", text[text.rindex("typedef struct", 0, end):end], flags=re.S)
+    want = []
+    for line in body.split("{", 1)[1].split(";"):
+        names = re.findall(r"\*?(\w+)(?:\[\d+\])?\s*(?:,|$)", line.strip())
+        for n in names:
+            want += [n, n + "_token", n + "_head"] if line.strip().startswith("HeadsRef") and "[" not in line else [n]
+    return want
+
+
+def cache_ref(**kw):
+    return fill(clear.CacheRef, **{**dict(pages=P, pages_seq=8, width=7, page_rows=16), **kw})
+
+
+def paged_args(cache=None, **kw):
+    a = clear.AttentionPagedArgs()
+    a.attention = attention_args(**{**dict(k_start=None), **kw})
+    a.cache = cache_ref(**(cache or {}))
+    return a
+
+
+@pytest.mark.parametrize("name", ["CacheRef", "AttentionPagedArgs"])
+def test_the_header_s_structs(name):
+    assert [f for f, _ in getattr(clear, name)._fields_] == header_fields(name)
+
+
+@pytest.mark.parametrize("bad,cache,rc", [
+    (dict(tokens=-1), {}, -1), (dict(seqs=-1), {}, -1), (dict(k_len=None), {}, -1), (dict(kv_heads=3), {}, -1),
+    (dict(type=2), {}, -2), (dict(dim=60), {}, -2), (dict(k_token=129), {}, -2), (dict(k_token=1 << 40), {}, -2),
+    (dict(work=P + 4, work_bytes=1024), {}, -2), ({}, dict(pages=None), -1), ({}, dict(width=0), -1), ({}, dict(width=-1), -1),
+    ({}, dict(pages_seq=-1), -1), ({}, dict(pages_seq=6), -1), ({}, dict(start=P), -1), ({}, dict(page_rows=8), -2),
+    ({}, dict(page_rows=0), -2), ({}, dict(page_rows=-16), -2), ({}, dict(page_rows=48), -2), (dict(tokens=0), {}, 0),
+    (dict(seqs=0), dict(pages=None), 0), (dict(seqs=1, tokens=0), dict(pages_seq=0), 0), (dict(heads=0), {}, 0)])
+def test_attention_paged_refusals(bad, cache, rc):
+    a = paged_args(cache, **bad)
+    assert LIB.pcx_attention_paged(C.byref(a), None) == rc
+    if rc:
+        assert LIB.pcx_attention_paged_workspace(C.byref(a)) == 0
+    assert LIB.pcx_attention_paged(None, None) == -1 and LIB.pcx_attention_paged_workspace(None) == 0
+
+
+def test_attention_paged_s_workspace_is_attention_s():
+    kw = dict(seqs=1, tokens=1, max_q=1, max_k=100000, kv_rows=100000)
+    want = LIB.pcx_attention_workspace(C.byref(attention_args(**kw)))
+    assert want > 0 and LIB.pcx_attention_paged_workspace(C.byref(paged_args(dict(width=9000), **kw))) == want
+
+
+def test_attention_paged_shapes_are_refused(ops):
+    x, kv, q0, kl = Fake((4, 4, 64)), Fake((96, 2, 64)), Fake((3,), "i32"), Fake((2,), "i32")
+    good = dict(q=x, k=kv, v=kv, q_start=q0, pages=Fake((2, 5), "i32"), page_rows=16, k_len=kl, out=x)
+    for bad in (dict(pages=Fake((3, 5), "i32")), dict(pages=Fake((2, 5), "i64")), dict(pages=Fake((10,), "i32")),
+                dict(pages=Fake((2, 5), "i32", strides=(1, 2))), dict(pages=Fake((2, 0), "i32")), dict(page_rows=8),
+                dict(page_rows=24), dict(page_rows=0), dict(k=Fake((96, 2, 32))), dict(out=Fake((4, 4, 32))), dict(q_start=kl)):
+        with pytest.raises(ValueError):
+            ops.attention_paged(**{**good, **bad})
+
+
+def test_attention_paged_arguments(ops):
+    """the packed arguments are the struct's; the longest run expected is at most what a table holds"""
+    x, kv = Fake((4, 6, 64)), Fake((96, 2, 64), ptr=P + 64)
+    a = ops.attention_paged_args(x, kv, kv, Fake((3,), "i32"), Fake((2, 5), "i32", strides=(8, 1), ptr=P + 16), 32, Fake((2,), "i32"), x)
+    assert {n: getattr(a.cache, n) for n, _ in clear.CacheRef._fields_} == dict(start=None, pages=P + 16, pages_seq=8, width=5,
+                                                                               page_rows=32)
+    assert (a.attention.k_start, a.attention.kv_rows, a.attention.max_k, a.attention.max_q) == (None, 96, 160, 4)
+    a = ops.attention_paged_args(x, kv, kv, Fake((3,), "i32"), Fake((2, 5), "i32"), 32, Fake((2,), "i32"), x, max_k=7, max_q=2)
+    assert (a.attention.max_k, a.attention.max_q, a.cache.pages_seq) == (7, 2, 5)
