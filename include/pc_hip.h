@@ -1218,6 +1218,44 @@ PC_STATIC_ASSERT(sizeof(AttentionPagedArgs) == 224, "AttentionPagedArgs layout")
 int pcx_attention_paged(const AttentionPagedArgs* args, pc_stream_t s);
 uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args); /* as pcx_attention_workspace */
 
+/* Which keys leave a cache. Of sequence b's len = k_len[b] keys each key head keeps the min(keep, len) of largest weight, the lower
+ * key of two alike (NaN weighs less than -infinity); before all others those are kept whose place is below `first` or at
+ * least next_place[b] - recent (first + recent <= keep; places NULL: key j's place is j; next_place NULL: len). The kept keys j >= keep in rising order
+ * are to go where the evicted ones j < keep lie, in rising order: moves[b][g][i] = (from, to), i < count[b][g], for pcx_move_rows.
+ * At most `most` are written (count is what there are: at most keep, and at most len - keep); entries past them are left
+ * as they were. kept_len (NULL: none; not k_len itself): min(keep, len), what the sequence's length is once its rows have moved.
+ * Keys on a page outside the pool are evicted first. max_k: the longest run expected; it only chooses a kernel.
+ * weights: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). */
+typedef struct EvictArgs {
+    HeadsRef weights, places;
+    CacheRef cache;
+    const int32_t* k_len;      /* [seqs] */
+    const int32_t* next_place; /* [seqs] */
+    int32_t* moves;            /* [seqs][kv_heads][most][2] */
+    int32_t* count;            /* [seqs][kv_heads] */
+    int32_t* kept_len;         /* [seqs] */
+    int64_t rows;
+    int32_t seqs, kv_heads, keep, recent, first, most, max_k, pad;
+} EvictArgs;
+PC_STATIC_ASSERT(sizeof(EvictArgs) == 160, "EvictArgs layout");
+int pcx_evict(const EvictArgs* args, pc_stream_t s);
+
+/* The moves of pcx_evict, in up to four tensors [rows][kv_heads][dim[i]] at once (keys, values, weights, places), elements of
+ * size[i] = 2, 4 or 8 bytes: row `to` of sequence b and key head g becomes row `from`, i < min(count[b][g], most). Moves that leave
+ * the cache are skipped. Rows that others are moved to may not be moved from (no move of pcx_evict does that). Sequences that
+ * share rows do not keep them. */
+typedef struct MoveRowsArgs {
+    HeadsRef t[4];
+    CacheRef cache;
+    const int32_t* moves;
+    const int32_t* count;
+    int64_t rows;
+    int32_t size[4], dim[4];
+    int32_t tensors, seqs, kv_heads, most;
+} MoveRowsArgs;
+PC_STATIC_ASSERT(sizeof(MoveRowsArgs) == 200, "MoveRowsArgs layout");
+int pcx_move_rows(const MoveRowsArgs* args, pc_stream_t s);
+
 /* Stage timing, for measurement: while on, the driver records a HIP event pair on the launch stream around each
  * stage it enqueues (0 ModUp INTT, 1 ModUp conversion, 2 ModUp NTT, 3 key dot, 4 ModDown INTT, 5 ModDown conversion,
  * 6 ModDown NTT + epilogue, 7 CtS baby steps and plaintext products, 8 tensor, 9 rescale). pcx_timing(c, n) turns it

@@ -208,13 +208,34 @@ class AttentionPagedArgs(C.Structure):
     _fields_ = [("attention", AttentionArgs), ("cache", CacheRef)]
 
 
+class EvictArgs(C.Structure):
+    """include/pc_hip.h EvictArgs."""
+    _fields_ = [*_ref("weights"), *_ref("places"), ("cache", CacheRef), ("k_len", _vp), ("next_place", _vp), ("moves", _vp),
+                ("count", _vp), ("kept_len", _vp), ("rows", _i64), ("seqs", _i32), ("kv_heads", _i32), ("keep", _i32),
+                ("recent", _i32), ("first", _i32), ("most", _i32), ("max_k", _i32), ("pad", _i32)]
+
+
+class HeadsRef(C.Structure):
+    """include/pc_hip.h HeadsRef."""
+    _fields_ = [("base", _vp), ("token", _i64), ("head", _i64)]
+
+
+class MoveRowsArgs(C.Structure):
+    """include/pc_hip.h MoveRowsArgs."""
+    _fields_ = [("t", HeadsRef * 4), ("cache", CacheRef), ("moves", _vp), ("count", _vp), ("rows", _i64), ("size", _i32 * 4),
+                ("dim", _i32 * 4), ("tensors", _i32), ("seqs", _i32), ("kv_heads", _i32), ("most", _i32)]
+
+
 # the same layouts for struct.pack: a call packs its arguments in about a microsecond, a ctypes Structure takes four
 _ROTARY = struct.Struct("@" + "Pqq" * 2 + "PPq" + "i" * 8)
 _QK_NORM_ROTARY = struct.Struct("@" + "Pqq" * 6 + "P" * 5 + "qq" + "i" * 7 + "f")
 _ATTENTION = struct.Struct("@" + "Pqq" * 4 + "P" * 5 + "Qq" + "i" * 9 + "f")
 _CACHE = struct.Struct("@PPqii")
+_EVICT = struct.Struct("@" + "Pqq" * 2 + "PPqii" + "P" * 5 + "q" + "i" * 8)
+_MOVE_ROWS = struct.Struct("@" + "Pqq" * 4 + "PPqii" + "PPq" + "i" * 12)
 assert (_ROTARY.size, _QK_NORM_ROTARY.size, _ATTENTION.size) == (104, 232, 192)
 assert _CACHE.size == C.sizeof(CacheRef) == 32
+assert (_EVICT.size, C.sizeof(EvictArgs), _MOVE_ROWS.size, C.sizeof(MoveRowsArgs)) == (160, 160, 200, 200)
 assert (C.sizeof(RotaryArgs), C.sizeof(QkNormRotaryArgs), C.sizeof(AttentionArgs)) == (104, 232, 192)
 
 
@@ -272,6 +293,27 @@ def _pages(pages, page_rows, seqs):
     if page_rows < 16 or page_rows & (page_rows - 1):
         raise ValueError(f"page_rows {page_rows}: a power of two, 16 or more")
     return pages.data_ptr(), step if n > 1 else width, width
+
+
+def _cache(k_start, pages, page_rows, seqs):
+    """CacheRef's fields: one run of rows for each sequence, or its pages"""
+    if (k_start is None) == (pages is None) or (pages is None) != (page_rows is None):
+        raise ValueError("k_start, or pages and page_rows: one of them says where the keys lie")
+    if pages is None:
+        return _flat(k_start, "k_start", "i64", seqs), 0, 0, 0, 0
+    ptr, step, width = _pages(pages, page_rows, seqs)
+    return 0, ptr, step, width, page_rows
+
+
+def _per_key(x, name, dtype, shape=None):
+    """(address, row stride, head stride) of a tensor [rows][kv heads] (of this shape, if given), by any strides"""
+    if not x.is_cuda:
+        raise ValueError(f"{name}: not on the device")
+    if (_known.get(x.dtype) or _type(x.dtype)) != dtype or len(x.shape) != 2:
+        raise ValueError(f"{name}: {dtype} [rows][kv heads] is wanted, got {x.dtype} {tuple(x.shape)}")
+    if shape is not None and tuple(x.shape) != tuple(shape):
+        raise ValueError(f"{name}: {tuple(shape)} is wanted, got {tuple(x.shape)}")
+    return (x.data_ptr(), *x.stride())
 
 
 def block_checked(heads, kv_heads, dim, capacity, dtype, table, layout, q_weight, k_weight):
@@ -385,6 +427,58 @@ class Clear:
         max_k = room if max_k is None else min(max_k, room)
         return self._attention(q, k, v, q_start, None, k_len, out, lse, scale, causal, max_q, max_k) + _CACHE.pack(
             0, ptr, step, width, page_rows)
+
+    def evict(self, weights, k_len, keep, moves, count, k_start=None, pages=None, page_rows=None, places=None, next_place=None,
+              recent=0, first=0, kept_len=None, max_k=None):
+        """Which keys leave: each key head of a sequence keeps the `keep` of its k_len[b] keys with the largest weights (f32 [rows]
+        [kv heads], by any strides), the lower key of two alike; before all others those whose place (i32, as the weights; None:
+        the key's number) is below `first` or at least next_place[b] (i32; None: the length) - recent, `keep` of them at most. moves (i32 [sequences]
+        [kv heads][most][2]) and count (i32 [sequences][kv heads]) get the rows that move_rows moves, kept keys from behind
+        `keep` to the gaps before it; kept_len (i32, or None) the lengths after that. Moves past `most` are not written (there
+        are never more than keep, or than the longest run less keep). max_k: the longest run expected; it only chooses a kernel."""
+        seqs = k_len.shape[0]
+        rows, kv = weights.shape if len(weights.shape) == 2 else (0, 0)
+        if len(moves.shape) != 4 or tuple(moves.shape[:2]) != (seqs, kv) or moves.shape[3] != 2:
+            raise ValueError(f"moves: [{seqs}][{kv}][most][2] is wanted, got {tuple(moves.shape)}")
+        if min(keep, recent, first) < 0 or first + recent > keep:
+            raise ValueError(f"keep {keep}, recent {recent}, first {first}: none negative, no more protected than kept")
+        w = _per_key(weights, "weights", "f32")
+        p = (0, 0, 0) if places is None else _per_key(places, "places", "i32", (rows, kv))
+        cache = _cache(k_start, pages, page_rows, seqs)
+        room = rows if pages is None else cache[3] * page_rows
+        args = _EVICT.pack(
+            *w, *p, *cache, _flat(k_len, "k_len", "i32", seqs),
+            0 if next_place is None else _flat(next_place, "next_place", "i32", seqs),
+            _flat(moves, "moves", "i32", None), _flat(count, "count", "i32", seqs * kv),
+            0 if kept_len is None else _flat(kept_len, "kept_len", "i32", seqs), rows, seqs, kv, keep, recent, first, moves.shape[2],
+            min(room if max_k is None else max_k, 0x7FFFFFFF), 0)
+        check(LIB.pcx_evict(args, self.stream.h), "evict")
+
+    def move_rows(self, moves, count, tensors, k_start=None, pages=None, page_rows=None):
+        """The moves that evict chose, in up to four tensors [rows][kv heads][dim] or [rows][kv heads] of any types at once, by any
+        strides of rows and heads: keys, values, their weights and places. Rows move in place, all moves at once."""
+        if len(moves.shape) != 4 or moves.shape[3] != 2 or not 1 <= len(tensors) <= 4:
+            raise ValueError("moves [sequences][kv heads][most][2], and one to four tensors")
+        seqs, kv, most, _ = moves.shape
+        refs, sizes, dims, rows = [], [], [], None
+        for x in tensors:
+            if len(x.shape) == 3:
+                at, row, head, shape, kind = _heads(x, "tensors")
+                dims.append(shape[2])
+            else:
+                kind = _known.get(x.dtype) or _type(x.dtype)
+                at, row, head = _per_key(x, "tensors", kind)
+                dims.append(1)
+            if x.shape[1] != kv or rows not in (None, x.shape[0]):
+                raise ValueError(f"tensors: the same rows and {kv} key heads each")
+            rows = x.shape[0]
+            refs += at, row, head
+            sizes.append(SIZES[kind])
+        n = 4 - len(tensors)
+        args = _MOVE_ROWS.pack(*refs, *[0] * 3 * n, *_cache(k_start, pages, page_rows, seqs), _flat(moves, "moves", "i32", None),
+                               _flat(count, "count", "i32", seqs * kv), rows, *sizes, *[0] * n, *dims, *[0] * n, len(tensors), seqs, kv,
+                               most)
+        check(LIB.pcx_move_rows(args, self.stream.h), "move_rows")
 
     def _attention(self, q, k, v, q_start, k_start, k_len, out, lse=None, scale=None, causal=True, max_q=None, max_k=None):
         a, at, ah, qs, kind = _heads(q, "q")

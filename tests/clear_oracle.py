@@ -100,3 +100,19 @@ def attention_bound(out, spread, dlse, kind, vmax):
     products in f32 and the scores' errors (dlse, in numerator and denominator)"""
     n = 2 * dlse[..., None]
     return UNIT[kind] * np.abs(out) + TINY[kind] + spread * (UNIT[kind] + n + 4 * E) + TINY[kind] * 2.0 ** 12 * vmax
+
+
+def kept(w, place, nxt, keep, recent, first):
+    """the keys that stay of one (sequence, key head), and the moves (from, to) that close the gaps: weights w, places"""
+    n = len(w)
+    if n <= keep:
+        return np.arange(n), []
+    place = np.asarray(place, np.int64)
+    w = np.asarray(w, np.float64)
+    held = (place >= int(nxt) - recent) | (place < first)
+    worth = np.where(held | np.isnan(w), -np.inf, w)  # protected keys are alike
+    order = np.lexsort((np.arange(n), -worth, np.isnan(w) & ~held, ~held))
+    stay = np.sort(order[:keep])
+    gone = np.ones(n, bool)
+    gone[stay] = False
+    return stay, list(zip(stay[stay >= keep], np.flatnonzero(gone[:keep])))

@@ -85,3 +85,81 @@ def test_attention_paged_arguments(ops):
     assert (a.attention.k_start, a.attention.kv_rows, a.attention.max_k, a.attention.max_q) == (None, 96, 160, 4)
     a = ops.attention_paged_args(x, kv, kv, Fake((3,), "i32"), Fake((2, 5), "i32"), 32, Fake((2,), "i32"), x, max_k=7, max_q=2)
     assert (a.attention.max_k, a.attention.max_q, a.cache.pages_seq) == (7, 2, 5)
+
+
+@pytest.mark.parametrize("cls,packed", [("EvictArgs", "_EVICT"), ("MoveRowsArgs", "_MOVE_ROWS")])
+def test_evict_s_structs(cls, packed):
+    """the header's fields, and struct.pack's layout the same: the same bytes give the same fields"""
+    assert [f for f, _ in getattr(clear, cls)._fields_] == header_fields(cls)
+
+    def flat(x):
+        for n, _ in x._fields_:
+            v = getattr(x, n)
+            for y in v if hasattr(v, "__len__") else [v]:
+                yield from flat(y) if isinstance(y, C.Structure) else [y]
+
+    layout = getattr(clear, packed)
+    n = sum(1 for _ in flat(getattr(clear, cls)()))
+    assert list(flat(getattr(clear, cls).from_buffer_copy(layout.pack(*range(1, n + 1))))) == list(range(1, n + 1))
+
+
+def evict_args(cache=None, **kw):
+    base = dict(weights=P, weights_token=1, weights_head=200, k_len=P, moves=P, count=P, rows=200, seqs=2, kv_heads=2, keep=8, most=4,
+                max_k=50)
+    a = fill(clear.EvictArgs, **{**base, **kw})
+    a.cache = cache_ref(**(cache or {}))
+    return a
+
+
+@pytest.mark.parametrize("bad,cache,rc", [
+    (dict(seqs=-1), {}, -1), (dict(kv_heads=-1), {}, -1), (dict(keep=-1), {}, -1), (dict(recent=-1), {}, -1), (dict(first=-1), {}, -1),
+    (dict(most=-1), {}, -1), (dict(max_k=-1), {}, -1), (dict(rows=-1), {}, -1), (dict(k_len=None), {}, -1), (dict(count=None), {}, -1),
+    (dict(moves=None), {}, -1), (dict(weights=None), {}, -1), (dict(weights_token=-1), {}, -1), (dict(places=P, places_head=-1), {}, -1),
+    (dict(kept_len=P), {}, -1), (dict(recent=8, first=1), {}, -1), (dict(recent=2 ** 31 - 1, first=2 ** 31 - 1), {}, -1),
+    ({}, dict(pages=None), -1), ({}, dict(start=P), -1), ({}, dict(width=0), -1), ({}, dict(page_rows=8), -2),
+    ({}, dict(page_rows=17), -2), (dict(weights=P + 2), {}, -2), (dict(places=P + 1), {}, -2), (dict(kv_heads=65536), {}, -2),
+    (dict(seqs=0), dict(pages=None), 0), (dict(kv_heads=0), {}, 0), (dict(kv_heads=0, weights=None, k_len=None), dict(start=P, pages=None), 0)])
+def test_evict_refusals(bad, cache, rc):
+    assert LIB.pcx_evict(C.byref(evict_args(cache, **bad)), None) == rc
+    assert LIB.pcx_evict(None, None) == -1
+
+
+def move_args(cache=None, base=P, token=128, head=64, size=2, dim=64, **kw):
+    a = fill(clear.MoveRowsArgs, **{**dict(moves=P, count=P, rows=200, tensors=1, seqs=2, kv_heads=2, most=4), **kw})
+    a.cache = cache_ref(**(cache or {}))
+    a.t[0] = clear.HeadsRef(base, token, head)
+    a.size[0], a.dim[0] = size, dim
+    return a
+
+
+@pytest.mark.parametrize("bad,cache,rc", [
+    (dict(seqs=-1), {}, -1), (dict(kv_heads=-1), {}, -1), (dict(most=-1), {}, -1), (dict(tensors=-1), {}, -1), (dict(tensors=5), {}, -1),
+    (dict(rows=-1), {}, -1), (dict(moves=None), {}, -1), (dict(count=None), {}, -1), (dict(moves=P + 4), {}, -1), (dict(base=None), {}, -1),
+    (dict(token=-1), {}, -1), (dict(size=1), {}, -2), (dict(size=3), {}, -2), (dict(dim=0), {}, -2), (dict(dim=2 ** 21), {}, -2),
+    (dict(base=P + 1), {}, -2), (dict(token=63), {}, -2), (dict(head=32), {}, -2), (dict(kv_heads=65536), {}, -2),
+    ({}, dict(pages=None), -1), ({}, dict(start=P), -1), ({}, dict(page_rows=8), -2), (dict(seqs=0), dict(pages=None), 0),
+    (dict(most=0, moves=None), {}, 0), (dict(tensors=0), {}, 0), (dict(kv_heads=0), {}, 0)])
+def test_move_rows_refusals(bad, cache, rc):
+    assert LIB.pcx_move_rows(C.byref(move_args(cache, **bad)), None) == rc
+    assert LIB.pcx_move_rows(None, None) == -1
+
+
+def test_evict_s_shapes_are_refused(ops):
+    w, n, mv, ct = Fake((96, 3), "f32"), Fake((2,), "i32"), Fake((2, 3, 4, 2), "i32"), Fake((2, 3), "i32")
+    good = dict(weights=w, k_len=n, keep=8, moves=mv, count=ct, pages=Fake((2, 5), "i32"), page_rows=16)
+    for bad in (dict(weights=Fake((96, 3))), dict(weights=Fake((96, 3, 1), "f32")), dict(places=Fake((96, 2), "i32")),
+                dict(places=Fake((96, 3), "f32")), dict(moves=Fake((2, 3, 4), "i32")), dict(moves=Fake((2, 2, 4, 2), "i32")),
+                dict(moves=Fake((2, 3, 4, 2), "i64")), dict(count=Fake((3, 3), "i32")), dict(k_len=Fake((2,), "i64")), dict(keep=-1),
+                dict(recent=5, first=4), dict(recent=-1), dict(next_place=Fake((3,), "i32")), dict(kept_len=Fake((3,), "i32")),
+                dict(k_start=Fake((2,), "i64")), dict(pages=None), dict(page_rows=None), dict(pages=None, page_rows=None),
+                dict(pages=Fake((3, 5), "i32")), dict(page_rows=20)):
+        with pytest.raises(ValueError):
+            ops.evict(**{**good, **bad})
+    k = Fake((96, 3, 64))
+    good = dict(moves=mv, count=ct, tensors=(k, w), pages=Fake((2, 5), "i32"), page_rows=16)
+    for bad in (dict(tensors=()), dict(tensors=(k,) * 5), dict(tensors=(k, Fake((95, 3), "f32"))), dict(tensors=(Fake((96, 2, 64)),)),
+                dict(tensors=(Fake((96, 3, 64), strides=(384, 128, 2)),)), dict(tensors=(Fake((96,), "f32"),)),
+                dict(moves=Fake((2, 3, 4, 1), "i32")), dict(moves=Fake((2, 3, 4, 2), "f32")), dict(count=Fake((2, 2), "i32")),
+                dict(k_start=Fake((2,), "i64"))):
+        with pytest.raises(ValueError):
+            ops.move_rows(**{**good, **bad})
