@@ -1218,6 +1218,39 @@ PC_STATIC_ASSERT(sizeof(AttentionPagedArgs) == 224, "AttentionPagedArgs layout")
 int pcx_attention_paged(const AttentionPagedArgs* args, pc_stream_t s);
 uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args); /* as pcx_attention_workspace */
 
+/* The weight that keys gather: for key j of sequence b and key head g, with the sequences, runs and `causal` of pcx_attention and
+ * rows as CacheRef says,
+ *     weights[row(j)][g] = decay before[row(j)][g] + sum exp(scale q . k_j - lse)
+ * over the queries that see j and the query heads of g. lse: what the attention of the same queries gave (f32
+ * [tokens][heads]); a query of -infinity, which sees no key, adds nothing. before (base NULL, or decay 0: not read, 0) may be
+ * weights itself. next_place (NULL: none): the last n_b keys of each sequence are its n_b queries' own and new: before is not
+ * read for them, and where places (base NULL: none) is given, theirs become next_place[b] - len + j (next_place[b]: the
+ * place after the sequence's last token). Rows of no sequence are left as they were; sequences may not share rows. Sums are f32 and have one order.
+ *
+ * weights, before: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). Keys on a page outside the pool have
+ * no row. Types, dim, scale and alignment as pcx_attention's; a query's row and head strides below 2^22 elements; kv_heads <
+ * 65536; decay >= 0 and finite. max_q and max_k are the longest runs expected: they choose the split of the rows, no result
+ * depends on them beyond the order of its sums. work (pcx_key_weights_workspace's bytes, less splits less; it may be attention's, whose
+ * counters it leaves alone) holds the parts' sums. */
+typedef struct KeyWeightsArgs {
+    HeadsRef q, k, weights, before, places;
+    CacheRef cache;
+    const float* lse;
+    const int32_t* q_start;
+    const int32_t* k_len;
+    const int32_t* next_place;
+    void* work;
+    uint64_t work_bytes;
+    int64_t kv_rows;
+    int32_t tokens, seqs, heads, kv_heads, dim;
+    int32_t type, causal, max_q, max_k;
+    float scale, decay;
+    int32_t pad;
+} KeyWeightsArgs;
+PC_STATIC_ASSERT(sizeof(KeyWeightsArgs) == 256, "KeyWeightsArgs layout");
+int pcx_key_weights(const KeyWeightsArgs* args, pc_stream_t s);
+uint64_t pcx_key_weights_workspace(const KeyWeightsArgs* args);
+
 /* Which keys leave a cache. Of sequence b's len = k_len[b] keys each key head keeps the min(keep, len) of largest weight, the lower
  * key of two alike (NaN weighs less than -infinity); before all others those are kept whose place is below `first` or at
  * least next_place[b] - recent (first + recent <= keep; places NULL: key j's place is j; next_place NULL: len). The kept keys j >= keep in rising order

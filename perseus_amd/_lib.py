@@ -136,6 +136,8 @@ _SIGS = {
     "pcx_attention_workspace": (C.c_uint64, [vp]),
     "pcx_attention_paged": (C.c_int, [vp, vp]),
     "pcx_attention_paged_workspace": (C.c_uint64, [vp]),
+    "pcx_key_weights": (C.c_int, [vp, vp]),
+    "pcx_key_weights_workspace": (C.c_uint64, [vp]),
     "pcx_evict": (C.c_int, [vp, vp]),
     "pcx_move_rows": (C.c_int, [vp, vp]),
 }

@@ -208,6 +208,14 @@ class AttentionPagedArgs(C.Structure):
     _fields_ = [("attention", AttentionArgs), ("cache", CacheRef)]
 
 
+class KeyWeightsArgs(C.Structure):
+    """include/pc_hip.h KeyWeightsArgs."""
+    _fields_ = [*_ref("q"), *_ref("k"), *_ref("weights"), *_ref("before"), *_ref("places"), ("cache", CacheRef), ("lse", _vp),
+                ("q_start", _vp), ("k_len", _vp), ("next_place", _vp), ("work", _vp), ("work_bytes", C.c_uint64), ("kv_rows", _i64),
+                ("tokens", _i32), ("seqs", _i32), ("heads", _i32), ("kv_heads", _i32), ("dim", _i32), ("type", _i32),
+                ("causal", _i32), ("max_q", _i32), ("max_k", _i32), ("scale", _f32), ("decay", _f32), ("pad", _i32)]
+
+
 class EvictArgs(C.Structure):
     """include/pc_hip.h EvictArgs."""
     _fields_ = [*_ref("weights"), *_ref("places"), ("cache", CacheRef), ("k_len", _vp), ("next_place", _vp), ("moves", _vp),
@@ -231,10 +239,12 @@ _ROTARY = struct.Struct("@" + "Pqq" * 2 + "PPq" + "i" * 8)
 _QK_NORM_ROTARY = struct.Struct("@" + "Pqq" * 6 + "P" * 5 + "qq" + "i" * 7 + "f")
 _ATTENTION = struct.Struct("@" + "Pqq" * 4 + "P" * 5 + "Qq" + "i" * 9 + "f")
 _CACHE = struct.Struct("@PPqii")
+_KEY_WEIGHTS = struct.Struct("@" + "Pqq" * 5 + "PPqii" + "P" * 5 + "Qq" + "i" * 9 + "ffi")
 _EVICT = struct.Struct("@" + "Pqq" * 2 + "PPqii" + "P" * 5 + "q" + "i" * 8)
 _MOVE_ROWS = struct.Struct("@" + "Pqq" * 4 + "PPqii" + "PPq" + "i" * 12)
 assert (_ROTARY.size, _QK_NORM_ROTARY.size, _ATTENTION.size) == (104, 232, 192)
 assert _CACHE.size == C.sizeof(CacheRef) == 32
+assert _KEY_WEIGHTS.size == C.sizeof(KeyWeightsArgs) == 256
 assert (_EVICT.size, C.sizeof(EvictArgs), _MOVE_ROWS.size, C.sizeof(MoveRowsArgs)) == (160, 160, 200, 200)
 assert (C.sizeof(RotaryArgs), C.sizeof(QkNormRotaryArgs), C.sizeof(AttentionArgs)) == (104, 232, 192)
 
@@ -427,6 +437,45 @@ class Clear:
         max_k = room if max_k is None else min(max_k, room)
         return self._attention(q, k, v, q_start, None, k_len, out, lse, scale, causal, max_q, max_k) + _CACHE.pack(
             0, ptr, step, width, page_rows)
+
+    def key_weights(self, q, k, lse, q_start, k_len, weights, k_start=None, pages=None, page_rows=None, before=None, decay=1.0,
+                    places=None, next_place=None, scale=None, causal=True, max_q=None, max_k=None):
+        """The weight that keys gather: weights (f32 [rows][kv heads], by any strides) = decay x before (the same shape, or None
+        for zeros; weights itself where they gather) + the sum of exp(scale q . k - lse) over the queries that see a key and the
+        heads of its group; q, k, lse and the runs as attention took and gave them, the keys' rows from k_start on or in pages.
+        next_place (i32 [sequences], the place after each sequence's last token): the last keys are the queries' own and new,
+        they begin at 0, and get their places (i32 [rows][kv heads], if given). Sequences may not share rows. max_q, max_k: the
+        longest runs expected; they only choose how rows are split."""
+        args = self._key_weights(q, k, lse, q_start, k_len, weights, k_start, pages, page_rows, before, decay, places, next_place, scale,
+                                 causal, max_q, max_k)
+        check(LIB.pcx_key_weights(args, self.stream.h), "key_weights")
+
+    def key_weights_args(self, *args, **kw):
+        """key_weights' checked arguments as the struct that pcx_key_weights and its workspace query take."""
+        return KeyWeightsArgs.from_buffer_copy(self._key_weights(*args, **kw))
+
+    def _key_weights(self, q, k, lse, q_start, k_len, weights, k_start=None, pages=None, page_rows=None, before=None, decay=1.0,
+                     places=None, next_place=None, scale=None, causal=True, max_q=None, max_k=None):
+        a, at, ah, qs, kind = _heads(q, "q")
+        b, bt, bh, ks, kkind = _heads(k, "k")
+        tokens, heads, dim = qs
+        rows, kv, kdim = ks
+        if kdim != dim or kind != kkind or kind not in TYPES:
+            raise ValueError("q and k: one dim, one floating type")
+        if places is not None and next_place is None:
+            raise ValueError("places: next_place says where they go on")
+        seqs = k_len.shape[0]
+        cache = _cache(k_start, pages, page_rows, seqs)
+        room = rows if pages is None else min(rows, cache[3] * page_rows)
+        none = (0, 0, 0)
+        return _KEY_WEIGHTS.pack(
+            a, at, ah, b, bt, bh, *_per_key(weights, "weights", "f32", (rows, kv)),
+            *(none if before is None else _per_key(before, "before", "f32", (rows, kv))),
+            *(none if places is None else _per_key(places, "places", "i32", (rows, kv))), *cache,
+            _flat(lse, "lse", "f32", tokens * heads), _flat(q_start, "q_start", "i32", seqs + 1), _flat(k_len, "k_len", "i32", seqs),
+            0 if next_place is None else _flat(next_place, "next_place", "i32", seqs), *self._work, rows, tokens, seqs, heads, kv, dim,
+            TYPES[kind], bool(causal), tokens if max_q is None else max_q, min(room if max_k is None else max_k, 0x7FFFFFFF),
+            dim ** -0.5 if scale is None else scale, decay, 0)
 
     def evict(self, weights, k_len, keep, moves, count, k_start=None, pages=None, page_rows=None, places=None, next_place=None,
               recent=0, first=0, kept_len=None, max_k=None):

@@ -1,0 +1,353 @@
+// What the queries of a call add to the weights of the keys that they see (pcx_key_weights).
+//
+// w_j = decay before_j + sum over the queries i that see j, and the heads h of the key's group, of exp(scale q_ih . k_j - lse_ih).
+// The products z = q k^T leave a key to a lane: lane (c, h) (c = lane mod 32, h = lane / 32) has the scores of key c with the rows
+// 8 i + 4 h + j (i, j < 4), so a key's sum grows inside its lane. The keys stay in registers, 64 to a wave; the rows go through LDS
+// once for the four waves of a workgroup, the next tile asked for while this one is used. Products, exponents and sums are f32; a
+// sum grows by the sum of 16 weights at a time. No two lanes add to the same word, so the sums have one order.
+#include <algorithm>
+
+#include "tiles.h"
+
+namespace pch {
+namespace clear {
+
+constexpr int BR = 64;   // rows of a tile: (query, head) pairs
+constexpr int BK = 256;  // keys of a workgroup
+
+struct Weigh {
+    HeadsRef q, k, weights, before, places;
+    const float* lse;
+    const int32_t *q_start, *k_len, *next_place;
+    const int64_t* k_start;  // null: pages
+    PagesRef pages;
+    float* work;  // [part][sequence][kv head][max_k] sums where rows are split
+    int64_t kv_rows;
+    int32_t tokens, seqs, heads, kv_heads, dim, causal, max_k;
+    int32_t group, hb, qt, blocks;  // heads of a key head; of a tile, queries of a tile, tiles of a query's heads
+    int32_t slots, parts;           // workgroups of a sequence's keys, parts of their rows
+    float scale, decay;
+};
+
+// a sequence's queries and keys, within the buffers
+struct Seq {
+    int q0, n, len;
+    int64_t k0;
+    __device__ __forceinline__ Seq(const Weigh& A, int b) {
+        const auto clamp = [](int x, int hi) { return x < 0 ? 0 : x > hi ? hi : x; };
+        q0 = clamp(A.q_start[b], A.tokens);
+        n = clamp(A.q_start[b + 1], A.tokens) - q0;
+        n = n < 0 ? 0 : n;
+        len = A.k_len[b];
+        len = len < 0 ? 0 : len;
+        int64_t room;
+        if (A.k_start) {
+            k0 = A.k_start[b];
+            room = k0 < 0 || k0 >= A.kv_rows ? 0 : A.kv_rows - k0;
+        } else {
+            k0 = (int64_t)b * A.pages.seq;
+            room = (int64_t)A.pages.width << A.pages.log;
+        }
+        if (len > room) len = (int)room;
+    }
+    // the cache's row of key j; -1: on a page that the pool does not have
+    __device__ __forceinline__ int64_t row(const Weigh& A, uint32_t j) const {
+        if (A.k_start) return k0 + j;
+        const int page = A.pages.table[k0 + (j >> A.pages.log)];
+        return (uint32_t)page < (uint32_t)A.pages.count ? ((int64_t)page << A.pages.log) + (j & ((1u << A.pages.log) - 1)) : -1;
+    }
+    // parts of the rows: lengths that the caller did not expect have no room for more than one
+    __device__ __forceinline__ int parts(const Weigh& A) const { return len <= A.max_k ? A.parts : 1; }
+};
+
+// key j's new weight from the sum that the queries add (row: its row, before: its weight so far, if any); a query's own key
+// begins at 0
+__device__ __forceinline__ bool fresh(const Weigh& A, const Seq& S, uint32_t j) {
+    return A.next_place && (int64_t)j >= (int64_t)S.len - S.n;
+}
+__device__ __forceinline__ float before(const Weigh& A, const Seq& S, int g, uint32_t j, int64_t row) {
+    if (row < 0 || !A.before.base || A.decay == 0.0f || fresh(A, S, j)) return 0;
+    return A.decay * *((const float*)A.before.base + row * A.before.token + g * A.before.head);
+}
+__device__ __forceinline__ void put(const Weigh& A, const Seq& S, int b, int g, uint32_t j, int64_t row, float w) {
+    if (row < 0) return;
+    *((float*)A.weights.base + row * A.weights.token + g * A.weights.head) = w;
+    if (A.places.base && fresh(A, S, j))
+        *((int32_t*)A.places.base + row * A.places.token + g * A.places.head) = A.next_place[b] - (S.len - (int)j);
+}
+__device__ __forceinline__ float* partial(const Weigh& A, int part, int b, int g) {
+    return A.work + (((int64_t)part * A.seqs + b) * A.kv_heads + g) * A.max_k;
+}
+
+template <class T, int DP, int DC>
+__global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
+    typedef typename Mat<T>::v8 v8;
+    constexpr int NW = 4, CPR = DP / 8, TB = BR * DP * 2, NL = BR * CPR / (64 * NW), STEPS = DC / 16;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * TB];
+    __shared__ __attribute__((aligned(16))) float nl[2][BR];  // less a row's log-sum-exp, in log2 units
+    __shared__ __attribute__((aligned(16))) int lim[2][BR];   // the keys that it sees
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const int g = blockIdx.x;
+    const int64_t item = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
+    const int b = (int)(item / (A.slots * A.parts));
+    if (b >= A.seqs) return;
+    const int rest = (int)(item - (int64_t)b * A.slots * A.parts), slot = rest / A.parts, part = rest - slot * A.parts;
+    const Seq S(A, b);
+    const int np = S.parts(A);
+    if (part >= np) return;
+    const float c2 = A.scale * 1.4426950408889634f;
+    const int tiles = (int)(((int64_t)S.n + A.qt - 1) / A.qt) * A.blocks;
+    // this lane's rows of a tile's loads (BR: none), and where they lie from the tile's first
+    uint32_t off[NL];
+    int row_of[NL];
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+        const int p = (n * NW + wave) * 64 + lane, x = p / CPR, qi = x / A.hb, hd = x - qi * A.hb;
+        const int ch = (p % CPR) ^ Tile<DP>::kswz(x);
+        row_of[n] = ch * 8 < A.dim && qi < A.qt ? x : BR;
+        off[n] = ((uint32_t)qi * (uint32_t)A.q.token + (uint32_t)hd * (uint32_t)A.q.head) * 2 + ch * 16;
+    }
+    const int xq = lane / A.hb, xh = lane - xq * A.hb;  // the row whose log-sum-exp this lane of the first wave brings
+    const uint32_t to = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 1024;
+    const T* const q = at<T>(A.q, S.q0, (int64_t)g * A.group);
+    const float* const lse = A.lse + (int64_t)S.q0 * A.heads + (int64_t)g * A.group;
+
+    // a tile's first query and head of the group, and its rows
+    struct Rows {
+        int i, hd, x;
+    };
+    const auto rows = [&](int t) {
+        const int qb = A.blocks == 1 ? t : t / A.blocks, i = qb * A.qt, hd = A.blocks == 1 ? 0 : (t - qb * A.blocks) * BR;
+        const int nq = S.n - i < A.qt ? S.n - i : A.qt, nh = A.group - hd < A.hb ? A.group - hd : A.hb;
+        return Rows{i, hd, nq * nh};
+    };
+    const auto load = [&](int t, int buf) {
+        const Rows r = rows(t);
+        const char* p = (const char*)(q + (int64_t)r.i * A.q.token + (int64_t)r.hd * A.q.head);
+        uint32_t own[NL];
+#pragma unroll
+        for (int n = 0; n < NL; ++n) own[n] = row_of[n] < r.x ? off[n] : 0x7ffffff0u;  // zeros
+        load_lds<NW * 1024>(__builtin_amdgcn_make_buffer_rsrc((void*)uniform64((uint64_t)p), 0, 0x40000000, 0x00020000), to + buf * TB, own);
+    };
+    const auto ask = [&](int t) {
+        const Rows r = rows(t);
+        return lane < r.x ? lse[(int64_t)(r.i + xq) * A.heads + r.hd + xh] : -INFINITY;
+    };
+    const auto bring = [&](int t, int buf, float x) {
+        const Rows r = rows(t);
+        nl[buf][lane] = x == -INFINITY ? x : x * -1.4426950408889634f;  // a row that sees no key adds nothing
+        const int64_t sees = (int64_t)S.len - S.n + r.i + xq + 1;
+        lim[buf][lane] = lane >= r.x || sees < 0 ? 0 : (int)sees;
+    };
+
+    for (int64_t k0 = (int64_t)slot * BK; k0 < S.len; k0 += (int64_t)A.slots * BK) {
+        const uint32_t j = (uint32_t)k0 + wave * 64 + c, len = (uint32_t)S.len;
+        int64_t key[2];
+        v8 kf[2][STEPS];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) key[kb] = j + 32 * kb < len ? S.row(A, j + 32 * kb) : -1;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            const T* x = at<T>(A.k, key[kb] < 0 ? 0 : key[kb], g);
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int d = 16 * s + 8 * h;
+                kf[kb][s] = key[kb] >= 0 && d < A.dim ? *(const v8*)(x + d) : (v8)(T)0.0f;
+            }
+        }
+        // after the loop lane (c, h) holds the sum of key j + 32 h
+        const uint32_t mine = j + 32 * h;
+        const int64_t row = h ? key[1] : key[0];
+        const float old = np == 1 ? before(A, S, g, mine, row) : 0;
+
+        // the tiles that see any of the keys, this part's of them; those from `whole` on see all of them
+        const int64_t end = k0 + BK < S.len ? k0 + BK : S.len;
+        const int64_t i0 = A.causal && k0 + S.n > S.len ? k0 + S.n - S.len : 0, i1 = A.causal && end - 1 + S.n > S.len ? end - 1 + S.n - S.len : 0;
+        const int begin = (int)(i0 / A.qt) * A.blocks, whole = (int)((i1 + A.qt - 1) / A.qt) * A.blocks;
+        const int t0 = begin + (int)((int64_t)(tiles - begin) * part / np), t1 = begin + (int)((int64_t)(tiles - begin) * (part + 1) / np);
+        float acc[2] = {0, 0};
+        const auto tile = [&](int buf, int x, bool masked) __attribute__((always_inline)) {
+            const char PCH_LDS* const l = (const char PCH_LDS*)lds + buf * TB + c * DP * 2;
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+                if (rb && x <= 32) break;
+                v16f z[2];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) z[kb] = (v16f)0.0f;
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) {
+                    const v8 a = *(const v8 PCH_LDS*)(l + rb * 32 * DP * 2 + (((2 * s + h) ^ Tile<DP>::kswz(c)) << 4));
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) z[kb] = Mat<T>::mul(a, kf[kb][s], z[kb]);
+                }
+                float part[2][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const v4f m = *(const v4f*)&nl[buf][32 * rb + 8 * i + 4 * h];
+                    typedef int v4i __attribute__((ext_vector_type(4)));
+                    v4i n;
+                    if (masked) n = *(const v4i*)&lim[buf][32 * rb + 8 * i + 4 * h];
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) {
+                        float w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w[e] = __builtin_amdgcn_exp2f(fmaf(z[kb][4 * i + e], c2, m[e]));
+                            if (masked && j + 32 * kb >= (uint32_t)n[e]) w[e] = 0;
+                        }
+                        part[kb][i] = (w[0] + w[1]) + (w[2] + w[3]);
+                    }
+                }
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) acc[kb] += (part[kb][0] + part[kb][1]) + (part[kb][2] + part[kb][3]);
+            }
+        };
+        if (t0 < t1) {
+            float raw = 0;
+            if (wave == 0) {
+                bring(t0, 0, ask(t0));
+                if (t0 + 1 < t1) raw = ask(t0 + 1);
+            }
+            load(t0, 0);
+            settled();
+            const auto step = [&](int t, bool masked) __attribute__((always_inline)) {
+                const int buf = (t - t0) & 1;
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (t + 1 < t1) {
+                    if (wave == 0) {
+                        bring(t + 1, buf ^ 1, raw);
+                        if (t + 2 < t1) raw = ask(t + 2);
+                    }
+                    load(t + 1, buf ^ 1);
+                }
+                tile(buf, rows(t).x, masked);
+            };
+            int t = t0;
+            for (; t < t1 && t < whole; ++t) step(t, true);
+            for (; t < t1; ++t) step(t, false);
+        }
+        const float both[2] = {acc[0] + other(acc[0]), acc[1] + other(acc[1])}, sum = h ? both[1] : both[0];
+        if (mine < len) {
+            if (np == 1)
+                put(A, S, b, g, mine, row, old + sum);
+            else
+                partial(A, part, b, g)[mine] = sum;
+        }
+        __syncthreads();  // the next keys' first tile takes the memory of these keys' last
+    }
+}
+
+// the parts of the rows joined, in their order: a lane a key
+__global__ void __launch_bounds__(256) weigh_join_k(Weigh A) {
+    const int g = blockIdx.y;
+    for (int b = blockIdx.z; b < A.seqs; b += gridDim.z) {
+        const Seq S(A, b);
+        const int np = S.parts(A);
+        const uint32_t j = blockIdx.x * 256 + threadIdx.x;
+        if (np == 1 || j >= (uint32_t)S.len) continue;
+        const int64_t row = S.row(A, j);
+        float sum = 0;
+        for (int p = 0; p < np; ++p) sum += partial(A, p, b, g)[j];
+        put(A, S, b, g, j, row, before(A, S, g, j, row) + sum);
+    }
+}
+
+static int checked(const KeyWeightsArgs* a, Weigh* w) {
+    if (!a || a->tokens < 0 || a->seqs < 0 || a->heads < 0 || a->kv_heads < 0 || a->kv_rows < 0 || a->max_q < 0 || a->max_k < 0) return -1;
+    if (a->type != PCX_BF16 && a->type != PCX_F16) return -2;
+    if (a->dim < 8 || a->dim > 256 || a->dim % 8) return -2;
+    if (!(a->scale > 0) || a->scale > 2.35e38f || !(a->decay >= 0) || a->decay > 3.4e38f) return -1;
+    if (a->heads && (a->kv_heads < 1 || a->heads % a->kv_heads)) return -1;
+    const bool any = a->seqs && a->kv_heads;
+    if (any && (!a->q_start || !a->k_len || (a->tokens && a->heads && !a->lse))) return -1;
+    if (a->cache.start && a->cache.pages) return -1;
+    if (a->places.base && !a->next_place) return -1;
+    *w = {};
+    if (!a->cache.start)
+        if (int e = pages_of(a->cache, any ? a->seqs : 0, a->kv_rows, &w->pages)) return any ? e : 0;
+    if (!usable(a->q, a->tokens, a->heads) || !usable(a->k, a->kv_rows, a->kv_heads)) return -1;
+    if (!usable(a->weights, any ? a->kv_rows : 0, a->kv_heads)) return -1;
+    for (const HeadsRef* r : {&a->before, &a->places})
+        if (r->token < 0 || r->head < 0) return -1;
+    for (const HeadsRef* r : {&a->weights, &a->before, &a->places})
+        if ((uintptr_t)r->base % 4) return -2;
+    w->q = settled(a->q, a->tokens, a->heads, a->dim), w->k = settled(a->k, a->kv_rows, a->kv_heads, a->dim);
+    w->weights = settled(a->weights, a->kv_rows, a->kv_heads, 1), w->before = settled(a->before, a->kv_rows, a->kv_heads, 1);
+    w->places = settled(a->places, a->kv_rows, a->kv_heads, 1);
+    for (const HeadsRef* r : {&w->q, &w->k})
+        if ((uintptr_t)r->base % 16 || r->token % 8 || r->head % 8) return -2;
+    if (!apart(w->weights, a->kv_rows, a->kv_heads, 1)) return -2;
+    if ((int64_t)a->tokens * a->heads > 0x7fffffff - 127 || a->kv_heads > 65535) return -2;
+    w->k_start = a->cache.start;
+    w->lse = a->lse, w->q_start = a->q_start, w->k_len = a->k_len, w->next_place = a->next_place;
+    w->kv_rows = a->kv_rows;
+    w->tokens = a->heads ? a->tokens : 0, w->seqs = a->seqs, w->heads = a->heads, w->kv_heads = a->kv_heads, w->dim = a->dim;
+    w->causal = a->causal, w->max_k = a->max_k, w->scale = a->scale, w->decay = a->decay;
+    w->group = a->heads && a->kv_heads ? a->heads / a->kv_heads : 1;
+    w->hb = w->group < BR ? w->group : BR;
+    w->qt = BR / w->hb;
+    w->blocks = (w->group + BR - 1) / BR;
+    // a tile's offsets: below 2^30 bytes
+    if (w->q.token > (1 << 28) / w->qt || w->q.head > (1 << 28) / w->hb) return -2;
+    return 0;
+}
+
+constexpr int64_t ITEMS = 0x7fffffff - 65535;
+
+// How the rows are split: keys alone give workgroups enough where there are 1024 (two waves a SIMD, twice over); where there are
+// fewer, parts of four tiles of rows and more. A workspace that is too small makes fewer of them.
+static uint64_t bytes_of(const Weigh& w, int parts) {
+    return parts > 1 ? PCX_ATTENTION_COUNTERS * 4 + (uint64_t)parts * w.seqs * w.kv_heads * w.max_k * 4 : 0;
+}
+static void choose(Weigh* w, int max_q, uint64_t room) {
+    const int64_t tiles = ((int64_t)max_q + w->qt - 1) / w->qt * w->blocks;
+    const int64_t keys = std::max<int64_t>(1, ((int64_t)w->max_k + BK - 1) / BK), most = std::max<int64_t>(1, (1 << 20) / ((int64_t)w->seqs * w->kv_heads));
+    w->slots = (int)std::min(keys, most);
+    const int64_t base = (int64_t)w->slots * w->seqs * w->kv_heads;
+    w->parts = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / base, tiles / 4));
+    while (w->parts > 1 && (bytes_of(*w, w->parts) > room || (int64_t)w->seqs * w->slots * w->parts > ITEMS)) w->parts /= 2;
+}
+
+template <class T>
+static int run(const Weigh& w, hipStream_t s) {
+    const int64_t items = (int64_t)w.seqs * w.slots * w.parts, high = std::min<int64_t>(items, 65535);
+    const dim3 grid((unsigned)w.kv_heads, (unsigned)high, (unsigned)((items + high - 1) / high)), block(256);
+    if (w.dim <= 64)
+        hipLaunchKernelGGL((weigh_k<T, 64, 64>), grid, block, 0, s, w);
+    else if (w.dim <= 96)
+        hipLaunchKernelGGL((weigh_k<T, 128, 96>), grid, block, 0, s, w);
+    else if (w.dim <= 128)
+        hipLaunchKernelGGL((weigh_k<T, 128, 128>), grid, block, 0, s, w);
+    else if (w.dim <= 192)
+        hipLaunchKernelGGL((weigh_k<T, 256, 192>), grid, block, 0, s, w);
+    else
+        hipLaunchKernelGGL((weigh_k<T, 256, 256>), grid, block, 0, s, w);
+    if (int e = launch_rc()) return e;
+    if (w.parts == 1) return 0;
+    const dim3 keys((unsigned)((w.max_k + 255) / 256), (unsigned)w.kv_heads, (unsigned)std::min(w.seqs, 65535));
+    hipLaunchKernelGGL(weigh_join_k, keys, block, 0, s, w);
+    return launch_rc();
+}
+
+}  // namespace clear
+}  // namespace pch
+
+using namespace pch;
+using namespace pch::clear;
+
+extern "C" uint64_t pcx_key_weights_workspace(const KeyWeightsArgs* args) {
+    Weigh w;
+    if (checked(args, &w) || !args->seqs || !args->kv_heads) return 0;
+    choose(&w, args->max_q, ~(uint64_t)0);
+    return bytes_of(w, w.parts);
+}
+
+extern "C" int pcx_key_weights(const KeyWeightsArgs* args, pc_stream_t s) {
+    Weigh w;
+    if (int e = checked(args, &w)) return e;
+    if ((uintptr_t)args->work % 16) return -2;
+    if (!args->seqs || !args->kv_heads) return 0;
+    choose(&w, args->max_q, args->work ? args->work_bytes : 0);
+    w.work = (float*)args->work + PCX_ATTENTION_COUNTERS;
+    return args->type == PCX_BF16 ? run<bf16>(w, (hipStream_t)s) : run<f16>(w, (hipStream_t)s);
+}

@@ -116,3 +116,25 @@ def kept(w, place, nxt, keep, recent, first):
     gone = np.ones(n, bool)
     gone[stay] = False
     return stay, list(zip(stay[stay >= keep], np.flatnonzero(gone[:keep])))
+
+
+def key_weights(q, k, lse, spans, group, scale, causal):
+    """spans: per sequence (query row, queries, key row, keys). (sums, bound): what each key of [rows][kv heads] gathers, 0 at rows
+    of no sequence, and how far f32 may be off: an exponent's D products and their sum, its scaling and the log-sum-exp's
+    (each a few roundings of their sizes), an exponential of 2 units, sums of 32 at a time that are added one after the other"""
+    R, KV, D = k.shape
+    out, bound = np.zeros((R, KV)), np.zeros((R, KV))
+    for q0, n, k0, m in spans:
+        for h in range(KV * group if n and m else 0):
+            g = h // group
+            Q, K = np.asarray(q[q0:q0 + n, h], np.float64), np.asarray(k[k0:k0 + m, g], np.float64)
+            L = np.asarray(lse[q0:q0 + n, h], np.float64)[:, None]
+            with np.errstate(invalid="ignore", over="ignore"):
+                z = scale * (Q @ K.T)
+                dz = scale * (np.abs(Q) @ np.abs(K).T)
+                sees = np.arange(m) <= m - n + np.arange(n)[:, None] if causal else np.ones((n, m), bool)
+                p = np.where(sees & (L > -np.inf) | sees & np.isnan(L), np.exp(z - L), 0)
+                d = (D + 4) * E * dz + 8 * E * (np.abs(z) + np.where(np.isfinite(L), np.abs(L), 0)) + 8 * E
+                out[k0:k0 + m, g] += p.sum(0)
+                bound[k0:k0 + m, g] += (p * d).sum(0) + (n * group / 16 + 32) * E * p.sum(0)
+    return out, bound

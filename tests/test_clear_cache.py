@@ -163,3 +163,63 @@ def test_evict_s_shapes_are_refused(ops):
                 dict(k_start=Fake((2,), "i64"))):
         with pytest.raises(ValueError):
             ops.move_rows(**{**good, **bad})
+
+
+def test_key_weights_s_struct():
+    assert [f for f, _ in clear.KeyWeightsArgs._fields_] == header_fields("KeyWeightsArgs")
+    names = [f for f, _ in clear.KeyWeightsArgs._fields_]
+    a = clear.KeyWeightsArgs.from_buffer_copy(clear._KEY_WEIGHTS.pack(*range(1, 40)))
+    got = []
+    for n in names:
+        got += [getattr(a.cache, x) for x, _ in clear.CacheRef._fields_] if n == "cache" else [getattr(a, n)]
+    assert got == list(range(1, 40))
+
+
+def weights_args(cache=None, **kw):
+    base = dict(lse=P, q_start=P, k_len=P, kv_rows=96, tokens=4, seqs=2, heads=4, kv_heads=2, dim=64, causal=1, max_q=2, max_k=50, scale=0.125,
+                decay=0.9)
+    for r, row, head in (("q", 256, 64), ("k", 128, 64), ("weights", 1, 96), ("before", 1, 96)):
+        base.update({r: P, r + "_token": row, r + "_head": head})
+    a = fill(clear.KeyWeightsArgs, **{**base, **kw})
+    a.cache = cache_ref(**(cache or {}))
+    return a
+
+
+@pytest.mark.parametrize("bad,cache,rc", [
+    (dict(tokens=-1), {}, -1), (dict(seqs=-1), {}, -1), (dict(heads=-1), {}, -1), (dict(kv_heads=-1), {}, -1), (dict(kv_rows=-1), {}, -1),
+    (dict(max_q=-1), {}, -1), (dict(max_k=-1), {}, -1), (dict(kv_heads=0), {}, -1), (dict(kv_heads=3), {}, -1), (dict(lse=None), {}, -1),
+    (dict(q_start=None), {}, -1), (dict(k_len=None), {}, -1), (dict(q=None), {}, -1), (dict(k=None), {}, -1), (dict(weights=None), {}, -1),
+    (dict(places=P), {}, -1), (dict(before_token=-1), {}, -1), (dict(places=P, next_place=P, places_head=-1), {}, -1),
+    (dict(scale=0.0), {}, -1), (dict(scale=float("nan")), {}, -1), (dict(scale=2.4e38), {}, -1), (dict(decay=-0.5), {}, -1),
+    (dict(decay=float("nan")), {}, -1), (dict(decay=float("inf")), {}, -1), ({}, dict(pages=None), -1), ({}, dict(start=P), -1),
+    ({}, dict(width=0), -1), ({}, dict(pages_seq=2), -1), ({}, dict(page_rows=8), -2), (dict(type=2), {}, -2), (dict(type=-1), {}, -2),
+    (dict(dim=60), {}, -2), (dict(dim=264), {}, -2), (dict(dim=0), {}, -2), (dict(q=P + 8), {}, -2), (dict(k_head=68), {}, -2),
+    (dict(q_token=1 << 27), {}, -2), (dict(q_head=1 << 28), {}, -2), (dict(weights=P + 2), {}, -2), (dict(before=P + 1), {}, -2),
+    (dict(weights_token=0), {}, -2), (dict(work=P + 4, work_bytes=1 << 20), {}, -2), (dict(heads=65536, kv_heads=65536), {}, -2),
+    (dict(tokens=2 ** 30), {}, -2), (dict(seqs=0), dict(pages=None), 0), (dict(heads=0, kv_heads=0), {}, 0)])
+def test_key_weights_refusals(bad, cache, rc):
+    a = weights_args(cache, **bad)
+    assert LIB.pcx_key_weights(C.byref(a), None) == rc
+    if rc:
+        b = weights_args(cache, **{n: v for n, v in bad.items() if n != "work"})
+        assert "work" in bad or LIB.pcx_key_weights_workspace(C.byref(b)) == 0
+    assert LIB.pcx_key_weights(None, None) == -1 and LIB.pcx_key_weights_workspace(None) == 0
+
+
+def test_key_weights_s_workspace():
+    """none for a token; the parts' sums for a prompt, whatever work says"""
+    assert LIB.pcx_key_weights_workspace(C.byref(weights_args(max_q=1))) == 0
+    a = weights_args(tokens=8192, seqs=1, max_q=8192, max_k=4096, kv_rows=8192, work=3, work_bytes=1)
+    n = LIB.pcx_key_weights_workspace(C.byref(a))
+    assert n > 4 * 4096 and (n - 4 * 4096) % (2 * 4096 * 4) == 0
+
+
+def test_key_weights_shapes_are_refused(ops):
+    q, k, lse, w, n = Fake((4, 4, 64)), Fake((96, 2, 64)), Fake((4, 4), "f32"), Fake((96, 2), "f32"), Fake((2,), "i32")
+    good = dict(q=q, k=k, lse=lse, q_start=Fake((3,), "i32"), k_len=n, weights=w, pages=Fake((2, 5), "i32"), page_rows=16)
+    for bad in (dict(k=Fake((96, 2, 32))), dict(k=Fake((96, 2, 64), "f16")), dict(q=Fake((4, 4, 64), "i32")), dict(lse=Fake((4, 2), "f32")),
+                dict(lse=Fake((4, 4))), dict(weights=Fake((95, 2), "f32")), dict(weights=Fake((96, 2))), dict(before=Fake((96, 4), "f32")),
+                dict(places=Fake((96, 2), "i32")), dict(places=Fake((96, 2), "f32"), next_place=n), dict(next_place=Fake((3,), "i32")),
+                dict(q_start=n), dict(k_len=Fake((2,), "i64")), dict(k_start=Fake((2,), "i64")), dict(pages=None), dict(page_rows=20)):
+        with pytest.raises(ValueError):
+            ops.key_weights(**{**good, **bad})
