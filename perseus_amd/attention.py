@@ -175,3 +175,144 @@ class ClearBlock:
     def keys(self):
         """The cached keys on the host, float32 [length][kv_heads dim]: what key_slots packs for encryption."""
         return self.k.numpy(self.ops.stream)[:self.length].reshape(self.length, -1)
+
+
+class PagedBlock:
+    """One attention block's clear side for several sequences that share a pool of pages, and for sequences longer than an encrypted
+    scoring holds: each key's attention weight is gathered as queries see it, and `evict` cuts a sequence to its `keep` keys of
+    largest weight (per key head), its last `recent` places and its first `first` among them. A key's place is its token's number
+    in the sequence, which it is rotated by and keeps.
+
+    `rows` are the block's projected rows of several sequences one after the other, an Array (or another library's device tensor)
+    [tokens][heads + 2 kv_heads][dim]: queries, then keys, then values. A call uploads where its tokens go and waits for that (so for
+    the stream's work before it); nothing is allocated after the constructor. tokens: the most of one call."""
+
+    def __init__(self, ops, heads, kv_heads, dim, seqs, pages, page_rows=16, keep=TOKENS, recent=32, first=4, tokens=TOKENS,
+                 dtype="bf16", table=None, layout="half", q_weight=None, k_weight=None, eps=1e-6, decay=1.0):
+        from .clear import Array, block_checked
+        from .engine import DevBuf
+
+        block_checked(heads, kv_heads, dim, 1, dtype, table, layout, q_weight, k_weight)
+        if min(seqs, pages, tokens, keep) < 1 or min(recent, first) < 0 or first + recent > keep or not decay >= 0:
+            raise ValueError("sequences, pages, tokens and keep: one or more; recent and first at most keep together; decay 0 or more")
+        if page_rows < 16 or page_rows & (page_rows - 1):
+            raise ValueError(f"page_rows {page_rows}: a power of two, 16 or more")
+        self.ops, self.heads, self.kv_heads, self.dim, self.page_rows = ops, heads, kv_heads, dim, page_rows
+        self.keep, self.recent, self.first, self.decay, self.tokens = keep, recent, first, decay, tokens
+        self.table, self.layout, self.q_weight, self.k_weight, self.eps = table, layout, q_weight, k_weight, eps
+        rows = pages * page_rows
+        self.k, self.v = (Array((rows, kv_heads, dim), dtype) for _ in range(2))
+        self.q, self.out = (Array((tokens, heads, dim), dtype) for _ in range(2))
+        self.lse = Array((tokens, heads), "f32")
+        # a head's rows one after the other, as both of their operators read them
+        self.weights, self.places = (Array((rows, kv_heads), kind, strides=(1, rows)) for kind in ("f32", "i32"))
+        self.moves = Array((seqs, kv_heads, keep, 2), "i32")
+        self.count = Array((seqs, kv_heads), "i32")
+        self._free = list(range(pages))
+        self._pages = [[] for _ in range(seqs)]
+        self.lengths, self.next_places = [0] * seqs, [0] * seqs
+        # what a call uploads, in one buffer: [slots i64][positions][q_start][k_len][next_place][tables]
+        self._words = [2 * tokens, tokens, seqs + 1, seqs, seqs, seqs * pages]
+        self._at = [sum(self._words[:i]) for i in range(len(self._words) + 1)]
+        self._host = np.zeros(self._at[-1], np.int32)
+        self._plan = DevBuf(self._at[-1])
+
+    def _put(self, i, values, kind=np.int32):
+        values = np.ascontiguousarray(values, kind).reshape(-1).view(np.int32)
+        self._host[self._at[i]:self._at[i] + values.size] = values
+
+    def _array(self, i, shape, kind="i32", strides=None):
+        from .clear import Array
+
+        return Array(shape, kind, self._plan, self._at[i], strides)
+
+    def _upload(self, lengths, next_places, longest):
+        """the sequences' lengths, places and pages as the next calls find them"""
+        n, width = len(lengths), -(-longest // self.page_rows)
+        table = np.full((n, width), -1, np.int32)
+        for b, p in enumerate(self._pages):
+            table[b, :len(p[:width])] = p[:width]
+        self._put(3, lengths)
+        self._put(4, next_places)
+        self._put(5, table)
+        self._plan.upload(self._host.view(np.uint32), self.ops.stream)
+        return dict(pages=self._array(5, (n, width)), page_rows=self.page_rows)
+
+    def append(self, rows, counts, causal=True):
+        """The next counts[b] tokens of each sequence b (0: none) into its cache, and their attention over all of it: (q, out, lse) of
+        these tokens, views of the block's buffers until the next call. Their weights are gathered by the keys that they see."""
+        from .clear import Array
+
+        counts = [int(c) for c in counts]
+        T, H, KV, P = rows.shape[0], self.heads, self.kv_heads, self.page_rows
+        if len(counts) != len(self.lengths) or min(counts) < 0 or sum(counts) != T or not 1 <= T <= self.tokens:
+            raise ValueError(f"{T} rows, {counts} tokens: 1 to {self.tokens} in all, a number for each of {len(self.lengths)} sequences")
+        if rows.shape[1] != H + 2 * KV or rows.shape[2] != self.dim:
+            raise ValueError("rows: [tokens][heads + 2 kv_heads][dim]")
+        if self.table is not None and any(c and at + c > self.table.shape[0] for at, c in zip(self.next_places, counts)):
+            raise ValueError(f"the rotation's table has {self.table.shape[0]} places")
+        lengths = [n + c for n, c in zip(self.lengths, counts)]
+        need = [max(0, -(-n // P) - len(p)) for n, p in zip(lengths, self._pages)]
+        if sum(need) > len(self._free):
+            raise ValueError(f"{sum(need)} more pages wanted, {len(self._free)} are free: evict, or a larger pool")
+        for p, n in zip(self._pages, need):
+            p += [self._free.pop() for _ in range(n)]
+        at = [np.arange(n, m) for n, m in zip(self.lengths, lengths)]
+        self._put(0, np.concatenate([self._rows(b, j) for b, j in enumerate(at)]), np.int64)
+        self._put(1, np.concatenate([np.arange(n, n + c) for n, c in zip(self.next_places, counts)]))
+        self._put(2, np.concatenate([[0], np.cumsum(counts)]))
+        next_places = [n + c for n, c in zip(self.next_places, counts)]
+        seqs, longest = len(counts), max(n for n, c in zip(lengths, counts) if c)
+        # sequences without new tokens are of length 0 to this call: their weights stay
+        where = self._upload([n if c else 0 for n, c in zip(lengths, counts)], next_places, longest)
+        q, out, lse = (Array((T,) + x.shape[1:], x.dtype, x.buf, 0, x.stride()) for x in (self.q, self.out, self.lse))
+        part = rows.heads if isinstance(rows, Array) else lambda a, c: rows[:, a:a + c]
+        q_start, k_len = self._array(2, (seqs + 1,)), self._array(3, (seqs,))
+        expect = dict(max_q=max(counts), max_k=longest)
+        self.ops.qk_norm_rotary(part(0, H), part(H, KV), self.q_weight, self.k_weight,
+                                None if self.table is None else self._array(1, (T,)), self.table, q, self.k, eps=self.eps,
+                                layout=self.layout, v=part(H + KV, KV), v_out=self.v, slots=self._array(0, (T,), "i64"))
+        self.ops.attention_paged(q, self.k, self.v, q_start, where["pages"], P, k_len, out, lse, causal=causal, **expect)
+        self.ops.key_weights(q, self.k, lse, q_start, k_len, self.weights, before=self.weights, decay=self.decay, places=self.places,
+                             next_place=self._array(4, (seqs,)), causal=causal, **expect, **where)
+        self.lengths, self.next_places = lengths, next_places  # only now: tokens that failed are appended again at the same places
+        return q, out, lse
+
+    def evict(self):
+        """Cuts each sequence longer than `keep` to that many keys; their pages go back to the pool. Returns the (moves, count) of
+        move_rows, for a copy of the cache elsewhere (encrypted keys, say) that is to be kept alike: row moves[b][g][i][0] of
+        sequence b and key head g went to row [i][1], i < count[b][g]; (None, None) where no sequence is longer."""
+        P, longest = self.page_rows, max(self.lengths)
+        if longest <= self.keep:
+            return None, None
+        where = self._upload(self.lengths, self.next_places, longest)
+        seqs = len(self.lengths)
+        self.ops.evict(self.weights, self._array(3, (seqs,)), self.keep, self.moves, self.count, places=self.places,
+                       next_place=self._array(4, (seqs,)), recent=self.recent, first=self.first, max_k=longest, **where)
+        self.ops.move_rows(self.moves, self.count, (self.k, self.v, self.weights, self.places), **where)
+        self.lengths = [min(n, self.keep) for n in self.lengths]
+        for n, p in zip(self.lengths, self._pages):
+            while len(p) > -(-n // P):
+                self._free.append(p.pop())
+        return self.moves, self.count
+
+    def drop(self, seq):
+        """Ends a sequence: its pages go back to the pool, its number is free for another."""
+        self._free += self._pages[seq]
+        self._pages[seq], self.lengths[seq], self.next_places[seq] = [], 0, 0
+
+    def _rows(self, seq, j):
+        return np.array(self._pages[seq] or [0], np.int64)[j // self.page_rows] * self.page_rows + j % self.page_rows
+
+    def rows_of(self, seq):
+        """The pool's rows of a sequence's keys, in the order of its cache (of k, v, weights and places)."""
+        return self._rows(seq, np.arange(self.lengths[seq]))
+
+    def keys(self, seq):
+        """A sequence's cached keys on the host, float32 [length][kv_heads dim]: what key_slots packs for encryption."""
+        from .clear import Array, SIZES
+
+        n, step = self.lengths[seq], self.page_rows * self.kv_heads * self.dim * SIZES[self.k.dtype] // 4
+        pages = [Array((self.page_rows, self.kv_heads * self.dim), self.k.dtype, self.k.buf, p * step).numpy(self.ops.stream)
+                 for p in self._pages[seq]]
+        return np.concatenate(pages)[:n] if n else np.zeros((0, self.kv_heads * self.dim), np.float32)
