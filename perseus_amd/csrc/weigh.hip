@@ -26,7 +26,10 @@ struct Weigh {
     int32_t tokens, seqs, heads, kv_heads, dim, causal, max_k;
     int32_t group, hb, qt, blocks;  // heads of a key head; of a tile, queries of a tile, tiles of a query's heads
     int32_t slots, parts;           // workgroups of a sequence's keys, parts of their rows
+    uint32_t per_hb;                // 2^16 / hb, rounded up
     float scale, decay;
+    // the query of a tile's row (below 64)
+    __device__ __forceinline__ int query(int x) const { return (int)(((uint32_t)x * per_hb) >> 16); }
 };
 
 // a sequence's queries and keys, within the buffers
@@ -46,7 +49,7 @@ struct Seq {
             room = k0 < 0 || k0 >= A.kv_rows ? 0 : A.kv_rows - k0;
         } else {
             k0 = (int64_t)b * A.pages.seq;
-            room = (int64_t)A.pages.width << A.pages.log;
+            room = A.pages.count ? (int64_t)A.pages.width << A.pages.log : 0;  // an empty pool has no rows
         }
         if (len > room) len = (int)room;
     }
@@ -55,6 +58,19 @@ struct Seq {
         if (A.k_start) return k0 + j;
         const int page = A.pages.table[k0 + (j >> A.pages.log)];
         return (uint32_t)page < (uint32_t)A.pages.count ? ((int64_t)page << A.pages.log) + (j & ((1u << A.pages.log) - 1)) : -1;
+    }
+    // the rows of two keys, their pages asked for at once
+    __device__ __forceinline__ void two_rows(const Weigh& A, uint32_t j0, uint32_t j1, int64_t (&r)[2]) const {
+        if (A.k_start) {
+            r[0] = k0 + j0, r[1] = k0 + j1;
+            return;
+        }
+        const int32_t* const table = A.pages.table + k0;
+        const int page[2] = {table[j0 >> A.pages.log], table[j1 >> A.pages.log]};
+        const uint32_t low = (1u << A.pages.log) - 1, j[2] = {j0, j1};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            r[i] = (uint32_t)page[i] < (uint32_t)A.pages.count ? ((int64_t)page[i] << A.pages.log) + (j[i] & low) : -1;
     }
     // parts of the rows: lengths that the caller did not expect have no room for more than one
     __device__ __forceinline__ int parts(const Weigh& A) const { return len <= A.max_k ? A.parts : 1; }
@@ -67,7 +83,7 @@ __device__ __forceinline__ bool fresh(const Weigh& A, const Seq& S, uint32_t j) 
 }
 __device__ __forceinline__ float before(const Weigh& A, const Seq& S, int g, uint32_t j, int64_t row) {
     if (row < 0 || !A.before.base || A.decay == 0.0f || fresh(A, S, j)) return 0;
-    return A.decay * *((const float*)A.before.base + row * A.before.token + g * A.before.head);
+    return *((const float*)A.before.base + row * A.before.token + g * A.before.head);
 }
 __device__ __forceinline__ void put(const Weigh& A, const Seq& S, int b, int g, uint32_t j, int64_t row, float w) {
     if (row < 0) return;
@@ -82,32 +98,30 @@ __device__ __forceinline__ float* partial(const Weigh& A, int part, int b, int g
 template <class T, int DP, int DC>
 __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
     typedef typename Mat<T>::v8 v8;
+    typedef int v4i __attribute__((ext_vector_type(4)));
     constexpr int NW = 4, CPR = DP / 8, TB = BR * DP * 2, NL = BR * CPR / (64 * NW), STEPS = DC / 16;
     __shared__ __attribute__((aligned(1024))) char lds[2 * TB];
     __shared__ __attribute__((aligned(16))) float nl[2][BR];  // less a row's log-sum-exp, in log2 units
     __shared__ __attribute__((aligned(16))) int lim[2][BR];   // the keys that it sees
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
-    const int g = blockIdx.x;
-    const int64_t item = blockIdx.y + (int64_t)gridDim.y * blockIdx.z;
-    const int b = (int)(item / (A.slots * A.parts));
-    if (b >= A.seqs) return;
-    const int rest = (int)(item - (int64_t)b * A.slots * A.parts), slot = rest / A.parts, part = rest - slot * A.parts;
+    const int g = blockIdx.x, slot = A.parts == 1 ? blockIdx.y : blockIdx.y / A.parts, part = blockIdx.y - slot * A.parts;
+    const int b = blockIdx.z;
     const Seq S(A, b);
     const int np = S.parts(A);
-    if (part >= np) return;
+    if (part >= np || (int64_t)slot * BK >= S.len) return;
     const float c2 = A.scale * 1.4426950408889634f;
-    const int tiles = (int)(((int64_t)S.n + A.qt - 1) / A.qt) * A.blocks;
+    const int tiles = (int)(((uint32_t)S.n + A.qt - 1) / A.qt) * A.blocks;
     // this lane's rows of a tile's loads (BR: none), and where they lie from the tile's first
     uint32_t off[NL];
     int row_of[NL];
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-        const int p = (n * NW + wave) * 64 + lane, x = p / CPR, qi = x / A.hb, hd = x - qi * A.hb;
+        const int p = (n * NW + wave) * 64 + lane, x = p / CPR, qi = A.query(x), hd = x - qi * A.hb;
         const int ch = (p % CPR) ^ Tile<DP>::kswz(x);
         row_of[n] = ch * 8 < A.dim && qi < A.qt ? x : BR;
         off[n] = ((uint32_t)qi * (uint32_t)A.q.token + (uint32_t)hd * (uint32_t)A.q.head) * 2 + ch * 16;
     }
-    const int xq = lane / A.hb, xh = lane - xq * A.hb;  // the row whose log-sum-exp this lane of the first wave brings
+    const int xq = A.query(lane), xh = lane - xq * A.hb;  // the row whose log-sum-exp this lane of the first wave brings
     const uint32_t to = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 1024;
     const T* const q = at<T>(A.q, S.q0, (int64_t)g * A.group);
     const float* const lse = A.lse + (int64_t)S.q0 * A.heads + (int64_t)g * A.group;
@@ -141,30 +155,39 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
     };
 
     for (int64_t k0 = (int64_t)slot * BK; k0 < S.len; k0 += (int64_t)A.slots * BK) {
+        // the tiles that see any of the keys, this part's of them; those from `whole` on see all of them
+        const int64_t end = k0 + BK < S.len ? k0 + BK : S.len;
+        const uint32_t i0 = A.causal && k0 + S.n > S.len ? k0 + S.n - S.len : 0, i1 = A.causal && end - 1 + S.n > S.len ? end - 1 + S.n - S.len : 0;
+        const int begin = (int)(i0 / A.qt) * A.blocks, whole = (int)((i1 + A.qt - 1) / A.qt) * A.blocks;
+        int t0 = begin, t1 = tiles;
+        if (np > 1) {
+            t0 = begin + (int)((double)(tiles - begin) * part / np);  // exact for the last part's end, one value for both neighbours
+            t1 = begin + (int)((double)(tiles - begin) * (part + 1) / np);
+        }
+        float raw = 0;
+        if (t0 < t1) {
+            load(t0, 0);
+            if (wave == 0) raw = ask(t0);
+        }
+        // the keys of this wave, in registers; what the last tile has no key for is some row's, and not kept
         const uint32_t j = (uint32_t)k0 + wave * 64 + c, len = (uint32_t)S.len;
         int64_t key[2];
+        S.two_rows(A, j < len ? j : len - 1, j + 32 < len ? j + 32 : len - 1, key);
         v8 kf[2][STEPS];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) key[kb] = j + 32 * kb < len ? S.row(A, j + 32 * kb) : -1;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             const T* x = at<T>(A.k, key[kb] < 0 ? 0 : key[kb], g);
 #pragma unroll
-            for (int s = 0; s < STEPS; ++s) {
-                const int d = 16 * s + 8 * h;
-                kf[kb][s] = key[kb] >= 0 && d < A.dim ? *(const v8*)(x + d) : (v8)(T)0.0f;
-            }
+            for (int s = 0; s < STEPS; ++s) kf[kb][s] = *(const v8*)(x + std::min(16 * s + 8 * h, A.dim - 8));
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+                if (16 * s + 16 > A.dim && 16 * s + 8 * h >= A.dim) kf[kb][s] = (v8)(T)0.0f;
         }
         // after the loop lane (c, h) holds the sum of key j + 32 h
         const uint32_t mine = j + 32 * h;
         const int64_t row = h ? key[1] : key[0];
-        const float old = np == 1 ? before(A, S, g, mine, row) : 0;
+        const float old = np == 1 && mine < len ? before(A, S, g, mine, row) : 0;
 
-        // the tiles that see any of the keys, this part's of them; those from `whole` on see all of them
-        const int64_t end = k0 + BK < S.len ? k0 + BK : S.len;
-        const int64_t i0 = A.causal && k0 + S.n > S.len ? k0 + S.n - S.len : 0, i1 = A.causal && end - 1 + S.n > S.len ? end - 1 + S.n - S.len : 0;
-        const int begin = (int)(i0 / A.qt) * A.blocks, whole = (int)((i1 + A.qt - 1) / A.qt) * A.blocks;
-        const int t0 = begin + (int)((int64_t)(tiles - begin) * part / np), t1 = begin + (int)((int64_t)(tiles - begin) * (part + 1) / np);
         float acc[2] = {0, 0};
         const auto tile = [&](int buf, int x, bool masked) __attribute__((always_inline)) {
             const char PCH_LDS* const l = (const char PCH_LDS*)lds + buf * TB + c * DP * 2;
@@ -184,7 +207,6 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const v4f m = *(const v4f*)&nl[buf][32 * rb + 8 * i + 4 * h];
-                    typedef int v4i __attribute__((ext_vector_type(4)));
                     v4i n;
                     if (masked) n = *(const v4i*)&lim[buf][32 * rb + 8 * i + 4 * h];
 #pragma unroll
@@ -202,14 +224,12 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
                 for (int kb = 0; kb < 2; ++kb) acc[kb] += (part[kb][0] + part[kb][1]) + (part[kb][2] + part[kb][3]);
             }
         };
+        settled();
         if (t0 < t1) {
-            float raw = 0;
             if (wave == 0) {
-                bring(t0, 0, ask(t0));
+                bring(t0, 0, raw);
                 if (t0 + 1 < t1) raw = ask(t0 + 1);
             }
-            load(t0, 0);
-            settled();
             const auto step = [&](int t, bool masked) __attribute__((always_inline)) {
                 const int buf = (t - t0) & 1;
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -229,27 +249,25 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
         const float both[2] = {acc[0] + other(acc[0]), acc[1] + other(acc[1])}, sum = h ? both[1] : both[0];
         if (mine < len) {
             if (np == 1)
-                put(A, S, b, g, mine, row, old + sum);
+                put(A, S, b, g, mine, row, fmaf(A.decay, old, sum));
             else
                 partial(A, part, b, g)[mine] = sum;
         }
-        __syncthreads();  // the next keys' first tile takes the memory of these keys' last
+        if (k0 + (int64_t)A.slots * BK < S.len) __syncthreads();  // the next keys' first tile takes the memory of these keys' last
     }
 }
 
 // the parts of the rows joined, in their order: a lane a key
 __global__ void __launch_bounds__(256) weigh_join_k(Weigh A) {
-    const int g = blockIdx.y;
-    for (int b = blockIdx.z; b < A.seqs; b += gridDim.z) {
-        const Seq S(A, b);
-        const int np = S.parts(A);
-        const uint32_t j = blockIdx.x * 256 + threadIdx.x;
-        if (np == 1 || j >= (uint32_t)S.len) continue;
-        const int64_t row = S.row(A, j);
-        float sum = 0;
-        for (int p = 0; p < np; ++p) sum += partial(A, p, b, g)[j];
-        put(A, S, b, g, j, row, before(A, S, g, j, row) + sum);
-    }
+    const int g = blockIdx.y, b = blockIdx.z;
+    const Seq S(A, b);
+    const int np = S.parts(A);
+    const uint32_t j = blockIdx.x * 256 + threadIdx.x;
+    if (np == 1 || j >= (uint32_t)S.len) return;
+    const int64_t row = S.row(A, j);
+    float sum = 0;
+    for (int p = 0; p < np; ++p) sum += partial(A, p, b, g)[j];
+    put(A, S, b, g, j, row, fmaf(A.decay, before(A, S, g, j, row), sum));
 }
 
 static int checked(const KeyWeightsArgs* a, Weigh* w) {
@@ -277,7 +295,7 @@ static int checked(const KeyWeightsArgs* a, Weigh* w) {
     for (const HeadsRef* r : {&w->q, &w->k})
         if ((uintptr_t)r->base % 16 || r->token % 8 || r->head % 8) return -2;
     if (!apart(w->weights, a->kv_rows, a->kv_heads, 1)) return -2;
-    if ((int64_t)a->tokens * a->heads > 0x7fffffff - 127 || a->kv_heads > 65535) return -2;
+    if ((int64_t)a->tokens * a->heads > 0x7fffffff - 127 || a->kv_heads > 65535 || a->seqs > 65535) return -2;
     w->k_start = a->cache.start;
     w->lse = a->lse, w->q_start = a->q_start, w->k_len = a->k_len, w->next_place = a->next_place;
     w->kv_rows = a->kv_rows;
@@ -285,14 +303,13 @@ static int checked(const KeyWeightsArgs* a, Weigh* w) {
     w->causal = a->causal, w->max_k = a->max_k, w->scale = a->scale, w->decay = a->decay;
     w->group = a->heads && a->kv_heads ? a->heads / a->kv_heads : 1;
     w->hb = w->group < BR ? w->group : BR;
+    w->per_hb = (65536 + w->hb - 1) / w->hb;
     w->qt = BR / w->hb;
     w->blocks = (w->group + BR - 1) / BR;
     // a tile's offsets: below 2^30 bytes
     if (w->q.token > (1 << 28) / w->qt || w->q.head > (1 << 28) / w->hb) return -2;
     return 0;
 }
-
-constexpr int64_t ITEMS = 0x7fffffff - 65535;
 
 // How the rows are split: keys alone give workgroups enough where there are 1024 (two waves a SIMD, twice over); where there are
 // fewer, parts of four tiles of rows and more. A workspace that is too small makes fewer of them.
@@ -301,17 +318,16 @@ static uint64_t bytes_of(const Weigh& w, int parts) {
 }
 static void choose(Weigh* w, int max_q, uint64_t room) {
     const int64_t tiles = ((int64_t)max_q + w->qt - 1) / w->qt * w->blocks;
-    const int64_t keys = std::max<int64_t>(1, ((int64_t)w->max_k + BK - 1) / BK), most = std::max<int64_t>(1, (1 << 20) / ((int64_t)w->seqs * w->kv_heads));
+    const int64_t keys = std::max<int64_t>(1, ((int64_t)w->max_k + BK - 1) / BK), most = std::max<int64_t>(1, std::min<int64_t>(65535, (1 << 20) / ((int64_t)w->seqs * w->kv_heads)));
     w->slots = (int)std::min(keys, most);
     const int64_t base = (int64_t)w->slots * w->seqs * w->kv_heads;
     w->parts = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / base, tiles / 4));
-    while (w->parts > 1 && (bytes_of(*w, w->parts) > room || (int64_t)w->seqs * w->slots * w->parts > ITEMS)) w->parts /= 2;
+    while (w->parts > 1 && (bytes_of(*w, w->parts) > room || w->slots * w->parts > 65535)) w->parts /= 2;
 }
 
 template <class T>
 static int run(const Weigh& w, hipStream_t s) {
-    const int64_t items = (int64_t)w.seqs * w.slots * w.parts, high = std::min<int64_t>(items, 65535);
-    const dim3 grid((unsigned)w.kv_heads, (unsigned)high, (unsigned)((items + high - 1) / high)), block(256);
+    const dim3 grid((unsigned)w.kv_heads, (unsigned)(w.slots * w.parts), (unsigned)w.seqs), block(256);
     if (w.dim <= 64)
         hipLaunchKernelGGL((weigh_k<T, 64, 64>), grid, block, 0, s, w);
     else if (w.dim <= 96)
@@ -324,7 +340,7 @@ static int run(const Weigh& w, hipStream_t s) {
         hipLaunchKernelGGL((weigh_k<T, 256, 256>), grid, block, 0, s, w);
     if (int e = launch_rc()) return e;
     if (w.parts == 1) return 0;
-    const dim3 keys((unsigned)((w.max_k + 255) / 256), (unsigned)w.kv_heads, (unsigned)std::min(w.seqs, 65535));
+    const dim3 keys((unsigned)((w.max_k + 255) / 256), (unsigned)w.kv_heads, (unsigned)w.seqs);
     hipLaunchKernelGGL(weigh_join_k, keys, block, 0, s, w);
     return launch_rc();
 }
