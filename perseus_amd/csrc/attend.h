@@ -78,85 +78,14 @@ __device__ __forceinline__ int keys_of(int tiles, int most) {
     return (int)min((uint32_t)tiles * KT, (uint32_t)most);
 }
 
-// inclusive sums over the lanes of a wave, and the largest value (by data-parallel moves: no trip through LDS)
-template <int CTRL, int ROWS>
-__device__ __forceinline__ int moved(int x) {
-    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ int lane_sums(int x) {
-    x += moved<0x111, 0xf>(x);  // from 1, 2, 4 and 8 lanes below in a row of 16
-    x += moved<0x112, 0xf>(x);
-    x += moved<0x114, 0xf>(x);
-    x += moved<0x118, 0xf>(x);
-    x += moved<0x142, 0xa>(x);  // the last lane of rows 0 and 2 into rows 1 and 3
-    x += moved<0x143, 0xc>(x);  // lane 31 into rows 2 and 3
-    return x;
-}
-__device__ __forceinline__ int total(int x) { return __builtin_amdgcn_readlane(lane_sums(x), 63); }
-__device__ __forceinline__ int largest(int x) {  // of values not negative
-    x = max(x, moved<0x111, 0xf>(x));
-    x = max(x, moved<0x112, 0xf>(x));
-    x = max(x, moved<0x114, 0xf>(x));
-    x = max(x, moved<0x118, 0xf>(x));
-    x = max(x, moved<0x142, 0xa>(x));
-    x = max(x, moved<0x143, 0xc>(x));
-    return __builtin_amdgcn_readlane(x, 63);
-}
-
 // ------------------------------------------------------------------------------------------------ keys in pages
-// PAGED: a sequence's key j lies in row page[j / rows] rows + j mod rows of the pool (rows: a power of two, 16 at least; whole
-// pages). Tiles of keys are loaded in runs of 16 rows, each in one page: a run has a buffer of its own, whose base the scalar unit
-// makes while the wave works on the tile before, and the lanes' offsets are within the run. Page numbers are read by scalar loads
-// a tile ahead, so that no tile waits for its table. A run past the sequence's end, or on a page that the pool does not have, is
-// an empty buffer: it reads as zeros.
-constexpr int RUN = 16;
-typedef const int32_t __attribute__((address_space(4))) page_t;
-
-template <int NL, int NW, int CPR>
-struct Runs {
-    static constexpr int PER = 64 / CPR;                                       // rows of a load
-    static constexpr int E = PER * NW >= RUN ? NL : NL * PER * NW / RUN;       // runs that a wave takes a part of
-    static constexpr int N = NL / E;                                           // its loads of one
-    static_assert(E * N == NL && (N == 1 || N * PER * NW == RUN));
-    int page[E];
-    // the tile's run that the wave's loads e N .. e N + N - 1 take
-    static __device__ __forceinline__ int run(int e, int wave) { return (e * N * NW + wave) * PER / RUN; }
-    template <int KT>
-    __device__ __forceinline__ void fetch(const PagesRef& P, page_t* table, int t, int wave) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t row = (uint32_t)t * KT + run(e, wave) * RUN;
-            page[e] = table[min(row >> P.log, (uint32_t)P.width - 1)];
-        }
-    }
-    template <int KT, int STEP>
-    __device__ __forceinline__ void load(const PagesRef& P, const char* base, int token, int dim, int len, int t, int wave,
-                                         uint32_t lds, const uint32_t (&off)[NL]) const {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t row = (uint32_t)t * KT + run(e, wave) * RUN;
-            const int left = (int)((uint32_t)len - row), nr = left < RUN ? left : RUN;
-            const bool there = (uint32_t)page[e] < (uint32_t)P.count && nr > 0;
-            const int64_t at = ((int64_t)(there ? page[e] : 0) << P.log) + (row & ((1u << P.log) - 1));
-            int bytes = there ? ((nr - 1) * token + dim) * 2 : 0;
-            asm("" : "+s"(bytes));  // a select, where the compiler would make a branch around each run
-            const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + at * token * 2), 0, bytes, 0x00020000);
-            uint32_t own[N];
-#pragma unroll
-            for (int n = 0; n < N; ++n) own[n] = off[e * N + n];
-            load_lds<STEP>(r, lds + e * N * STEP, own);
-        }
-    }
-};
-
 // the pool's row of a sequence's key j; -1: on a page that it does not have
 template <bool PAGED>
 __device__ __forceinline__ int64_t row_of(const PagesRef& P, const Work& w, uint32_t j) {
     if constexpr (!PAGED) {
         return w.k0 + j;
     } else {
-        const int page = P.table[w.seq * P.seq + (j >> P.log)];
-        return (uint32_t)page < (uint32_t)P.count ? ((int64_t)page << P.log) + (j & ((1u << P.log) - 1)) : -1;
+        return P.row(P.table[w.seq * P.seq + (j >> P.log)], j);
     }
 }
 

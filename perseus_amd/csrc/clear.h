@@ -31,6 +31,10 @@ struct PagesRef {
     const int32_t* table;
     int64_t seq;
     int32_t width, count, log;
+    // the pool's row of key j, which lies on `page`; -1: on one that the pool does not have
+    __device__ __forceinline__ int64_t row(int page, uint32_t j) const {
+        return (uint32_t)page < (uint32_t)count ? ((int64_t)page << log) + (j & ((1u << log) - 1)) : -1;
+    }
 };
 // the pages of a cache of `rows` rows: 0, or the error
 inline int pages_of(const CacheRef& c, int64_t seqs, int64_t rows, PagesRef* p) {

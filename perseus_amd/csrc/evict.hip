@@ -29,8 +29,7 @@ struct Rows {
     }
     __device__ __forceinline__ int64_t row(int64_t at, uint32_t j) const {
         if (start) return at + j;
-        const int page = p.table[at + (j >> p.log)];
-        return (uint32_t)page < (uint32_t)p.count ? ((int64_t)page << p.log) + (j & ((1u << p.log) - 1)) : -1;
+        return p.row(p.table[at + (j >> p.log)], j);
     }
 };
 
