@@ -262,9 +262,11 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
 
 // ------------------------------------------------------------------------------------------------ few rows
 // 32 rows and fewer (tokens): the rows stay in registers, and each wave streams tiles of 32 keys past them through LDS of its own,
-// two tiles of it: the next on its way while it works on this one. The tiles of all sequences and key heads are numbered in a
-// row, and every wave on the chip takes as many of them: lengths far apart leave none idle. The sums of eight tiles wait in LDS until
-// they are added to the weights before.
+// two tiles of it: the next on its way while it works on this one. What bounds it is the reading of the keys. The tiles of all
+// sequences are numbered in a row and cut into as many parts as the chip's waves hold of all key heads, so that lengths far apart leave
+// none idle; neighbouring waves read neighbouring heads of the same keys (each its own part of all heads' tiles: 95 us, so 85: a
+// row's heads lie together in memory). The sums of eight tiles wait in LDS until they are added to the weights before. A token each
+// of 48 caches of 89 to 8000 keys x 8 heads of 128: 85 us, 5.0 TB/s (a large copy: 5.6).
 constexpr int WINDOW = 8;
 
 // the sequences' tiles of 32 keys, a lane per sequence, 64 sequences at a time
@@ -293,16 +295,12 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
     int* const lim = limits[wave];
     float* const sums = window[wave];
     const float c2 = A.scale * 1.4426950408889634f;
-    // this wave's tiles of all: of sequence 0's heads, then of sequence 1's, ...
     int64_t total = 0;
     for (int b0 = 0; b0 < A.seqs; b0 += 64) {
         const Tiles t = tiles_of(Seq(A, std::min(b0 + lane, A.seqs - 1)), b0 + lane < A.seqs);
         total += t.upto(63);
     }
-    total *= A.kv_heads;
-    const int waves = gridDim.x * NW, me = blockIdx.x * NW + wave;
-    int64_t now = (int64_t)((double)total * me / waves);
-    const int64_t stop = me + 1 == waves ? total : (int64_t)((double)total * (me + 1) / waves);
+    const int waves = gridDim.x * NW, parts = std::max(1, waves / A.kv_heads);
     uint32_t off[NL];
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
@@ -310,130 +308,135 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
         off[n] = ch * 8 < A.dim ? (PAGED ? key % RUN : key) * (uint32_t)A.k.token * 2 + ch * 16 : 0x7ffffff0u;
     }
     const uint32_t base = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 2 * TB;
-    int b = -1;
-    Seq S;
-    int64_t start = 0, end = 0;  // the numbers of the sequence's tiles
-    while (now < stop) {
-        if (now >= end) {  // the sequence of this tile
-            int64_t past = 0;
-            b = -1;
-            for (int b0 = 0; b0 < A.seqs && b < 0; b0 += 64) {
-                const Seq own(A, std::min(b0 + lane, A.seqs - 1));
-                const Tiles t = tiles_of(own, b0 + lane < A.seqs);
-                const uint64_t here = __ballot(past + t.mine() * A.kv_heads > now);
-                if (here) {
-                    const int l = __builtin_ctzll(here);
-                    b = b0 + l;
-                    S = Seq(own, l);
-                    start = past + (l ? t.upto(l - 1) * A.kv_heads : 0);
-                    end = past + t.upto(l) * A.kv_heads;
-                }
-                past += t.upto(63) * A.kv_heads;
-            }
-            if (b < 0) return;
-        }
-        const int tiles = (int)(((uint32_t)S.len + KT - 1) / KT);
-        const int g = (int)((double)(now - start) / tiles), first = (int)(now - start - (int64_t)g * tiles);
-        const int last = (int)std::min<int64_t>(tiles, first + (stop - now));  // one past this wave's
-        now += last - first;
-        const char* const kp = (const char*)uniform64((uint64_t)at<T>(A.k, PAGED ? 0 : S.k0, g));
-        page_t* const table = PAGED ? (page_t*)uniform64((uint64_t)(A.pages.table + S.k0)) : nullptr;
-        Runs<NL, 1, CPR> pages;
-        const auto load = [&](int t, int buf) __attribute__((always_inline)) {
-            if constexpr (PAGED) {
-                pages.template load<KT, 1024>(A.pages, kp, (int)A.k.token, A.dim, S.len, t, 0, base + buf * TB, off);
-            } else {
-                const int left = S.len - t * KT, nr = (left < KT ? left : KT) - 1;
-                const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)t * KT * A.k.token * 2), 0,
-                                                                 (nr * (int)A.k.token + A.dim) * 2, 0x00020000);
-                load_lds<1024>(r, base + buf * TB, off);
-            }
-        };
-        // 32 rows, query * group + head of the group; more only where more queries came than were expected: each 32 add to the last's
-        const int64_t all = (int64_t)S.n * A.group;
-        for (int64_t r0 = 0; r0 == 0 || r0 < all; r0 += 32) {
-            if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, first, 0);
-            load(first, 0);
-            if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, first + 1, 0);
-            const int R = all - r0 < 32 ? (int)(all - r0) : 32;
-            const uint32_t r = (uint32_t)r0 + (c < R ? c : 0), i = A.group == 1 ? r : r / (uint32_t)A.group;
-            const int64_t head = (int64_t)g * A.group + (r - i * A.group);
-            v8 q[STEPS];
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s) q[s] = (v8)(T)0.0f;
-            if (c < R) {
-                const T* x = at<T>(A.q, S.q0 + (int64_t)i, head);
-#pragma unroll
-                for (int s = 0; s < STEPS; ++s) q[s] = *(const v8*)(x + std::min(16 * s + 8 * h, A.dim - 8));
-                const float x2 = A.lse[(S.q0 + (int64_t)i) * A.heads + head];
-                nl[c] = x2 == -INFINITY ? x2 : x2 * -1.4426950408889634f;  // a row that sees no key adds nothing
-                const int64_t sees = A.causal ? (int64_t)S.len - S.n + i + 1 : S.len;
-                lim[c] = sees < 0 ? 0 : (int)sees;
-            } else {
-                nl[c] = -INFINITY;
-                lim[c] = 0;
-            }
-#pragma unroll
-            for (int s = 0; s < STEPS; ++s)
-                if (16 * s + 16 > A.dim && 16 * s + 8 * h >= A.dim) q[s] = (v8)(T)0.0f;
-            // the weights before: on later rows, those that the earlier ones have written
-            const bool begin = r0 == 0, kept = !begin || (A.before.base && A.decay != 0.0f), given = begin && kept;
-            const float decay = begin ? A.decay : 1.0f;
-            const float* const from = (const float*)(given ? A.before.base : A.weights.base) + g * (given ? A.before.head : A.weights.head);
-            const int64_t step = given ? A.before.token : A.weights.token;
-            // the keys that every row sees
-            const int64_t whole = A.causal && S.n > 1 ? (int64_t)S.len - S.n + 1 + (A.group == 1 ? r0 : r0 / A.group) : (int64_t)S.len + KT;
-            settled();
-            int buf = 0;
-            for (int t0 = first; t0 < last; t0 += WINDOW) {
-                const int t1 = std::min(t0 + WINDOW, last);
-                for (int t = t0; t < t1; ++t, buf ^= 1) {
-                    if (t + 1 < last) {
-                        load(t + 1, buf ^ 1);
-                        if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, t + 2, 0);
-                        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
-                    } else {
-                        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (int unit = blockIdx.x * NW + wave; unit < parts * A.kv_heads; unit += waves) {
+        const int part = unit / A.kv_heads, g = unit - part * A.kv_heads;
+        int64_t now = (int64_t)((double)total * part / parts);
+        const int64_t stop = (int64_t)((double)total * (part + 1) / parts);
+        int b = -1;
+        Seq S;
+        int64_t start = 0, end = 0;  // the numbers of the sequence's tiles
+        while (now < stop) {
+            if (now >= end) {  // the sequence of this tile
+                int64_t past = 0;
+                b = -1;
+                for (int b0 = 0; b0 < A.seqs && b < 0; b0 += 64) {
+                    const Seq own(A, std::min(b0 + lane, A.seqs - 1));
+                    const Tiles t = tiles_of(own, b0 + lane < A.seqs);
+                    const uint64_t here = __ballot(past + t.mine() > now);
+                    if (here) {
+                        const int l = __builtin_ctzll(here);
+                        b = b0 + l;
+                        S = Seq(own, l);
+                        start = past + (l ? t.upto(l - 1) : 0);
+                        end = past + t.upto(l);
                     }
-                    const char PCH_LDS* const l = (const char PCH_LDS*)lds + (wave * 2 + buf) * TB + c * DP * 2;
-                    v16f z = (v16f)0.0f;
+                    past += t.upto(63);
+                }
+                if (b < 0) return;
+            }
+            const int tiles = (int)(((uint32_t)S.len + KT - 1) / KT);
+            const int first = (int)(now - start);
+            const int last = (int)std::min<int64_t>(tiles, first + (stop - now));  // one past this wave's
+            now += last - first;
+            const char* const kp = (const char*)uniform64((uint64_t)at<T>(A.k, PAGED ? 0 : S.k0, g));
+            page_t* const table = PAGED ? (page_t*)uniform64((uint64_t)(A.pages.table + S.k0)) : nullptr;
+            Runs<NL, 1, CPR> pages;
+            const auto load = [&](int t, int buf) __attribute__((always_inline)) {
+                if constexpr (PAGED) {
+                    pages.template load<KT, 1024>(A.pages, kp, (int)A.k.token, A.dim, S.len, t, 0, base + buf * TB, off);
+                } else {
+                    const int left = S.len - t * KT, nr = (left < KT ? left : KT) - 1;
+                    const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)t * KT * A.k.token * 2), 0,
+                                                                     (nr * (int)A.k.token + A.dim) * 2, 0x00020000);
+                    load_lds<1024>(r, base + buf * TB, off);
+                }
+            };
+            // 32 rows, query * group + head of the group; more only where more queries came than were expected: each 32 add to the last's
+            const int64_t all = (int64_t)S.n * A.group;
+            for (int64_t r0 = 0; r0 == 0 || r0 < all; r0 += 32) {
+                if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, first, 0);
+                load(first, 0);
+                if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, first + 1, 0);
+                const int R = all - r0 < 32 ? (int)(all - r0) : 32;
+                const uint32_t r = (uint32_t)r0 + (c < R ? c : 0), i = A.group == 1 ? r : r / (uint32_t)A.group;
+                const int64_t head = (int64_t)g * A.group + (r - i * A.group);
+                v8 q[STEPS];
 #pragma unroll
-                    for (int s = 0; s < STEPS; ++s) z = Mat<T>::mul(q[s], *(const v8 PCH_LDS*)(l + (((2 * s + h) ^ Tile<DP>::kswz(c)) << 4)), z);
+                for (int s = 0; s < STEPS; ++s) q[s] = (v8)(T)0.0f;
+                if (c < R) {
+                    const T* x = at<T>(A.q, S.q0 + (int64_t)i, head);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const v4f m = *(const v4f*)&nl[8 * e + 4 * h];
+                    for (int s = 0; s < STEPS; ++s) q[s] = *(const v8*)(x + std::min(16 * s + 8 * h, A.dim - 8));
+                    const float x2 = A.lse[(S.q0 + (int64_t)i) * A.heads + head];
+                    nl[c] = x2 == -INFINITY ? x2 : x2 * -1.4426950408889634f;  // a row that sees no key adds nothing
+                    const int64_t sees = A.causal ? (int64_t)S.len - S.n + i + 1 : S.len;
+                    lim[c] = sees < 0 ? 0 : (int)sees;
+                } else {
+                    nl[c] = -INFINITY;
+                    lim[c] = 0;
+                }
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) z[4 * e + u] = __builtin_amdgcn_exp2f(fmaf(z[4 * e + u], c2, m[u]));
+                for (int s = 0; s < STEPS; ++s)
+                    if (16 * s + 16 > A.dim && 16 * s + 8 * h >= A.dim) q[s] = (v8)(T)0.0f;
+                // the weights before: on later rows, those that the earlier ones have written
+                const bool begin = r0 == 0, kept = !begin || (A.before.base && A.decay != 0.0f), given = begin && kept;
+                const float decay = begin ? A.decay : 1.0f;
+                const float* const from = (const float*)(given ? A.before.base : A.weights.base) + g * (given ? A.before.head : A.weights.head);
+                const int64_t step = given ? A.before.token : A.weights.token;
+                // the keys that every row sees
+                const int64_t whole = A.causal && S.n > 1 ? (int64_t)S.len - S.n + 1 + (A.group == 1 ? r0 : r0 / A.group) : (int64_t)S.len + KT;
+                settled();
+                int buf = 0;
+                for (int t0 = first; t0 < last; t0 += WINDOW) {
+                    const int t1 = std::min(t0 + WINDOW, last);
+                    for (int t = t0; t < t1; ++t, buf ^= 1) {
+                        if (t + 1 < last) {
+                            load(t + 1, buf ^ 1);
+                            if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, t + 2, 0);
+                            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
+                        } else {
+                            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                        }
+                        const char PCH_LDS* const l = (const char PCH_LDS*)lds + (wave * 2 + buf) * TB + c * DP * 2;
+                        v16f z = (v16f)0.0f;
+#pragma unroll
+                        for (int s = 0; s < STEPS; ++s) z = Mat<T>::mul(q[s], *(const v8 PCH_LDS*)(l + (((2 * s + h) ^ Tile<DP>::kswz(c)) << 4)), z);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const v4f m = *(const v4f*)&nl[8 * e + 4 * h];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) z[4 * e + u] = __builtin_amdgcn_exp2f(fmaf(z[4 * e + u], c2, m[u]));
+                        }
+                        if ((int64_t)t * KT + KT > whole)
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if ((int64_t)t * KT + c >= lim[8 * (e >> 2) + 4 * h + (e & 3)]) z[e] = 0;
+                        float sum = ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
+                        sum += ((z[8] + z[9]) + (z[10] + z[11])) + ((z[12] + z[13]) + (z[14] + z[15]));
+                        sum += other(sum);
+                        if (h == 0) sums[(t - t0) * KT + c] = sum;
                     }
-                    if ((int64_t)t * KT + KT > whole)
+                    // loads on every path, all of them waited for here: one that the compiler took to be on its way at the next tile would
+                    // make it wait there for that tile's keys too
+                    const uint32_t j0 = (uint32_t)t0 * KT + lane, j1 = std::min((uint32_t)t1 * KT, (uint32_t)S.len);
+                    int64_t row[WINDOW / 2];
+                    float old[WINDOW / 2];
 #pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if ((int64_t)t * KT + c >= lim[8 * (e >> 2) + 4 * h + (e & 3)]) z[e] = 0;
-                    float sum = ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
-                    sum += ((z[8] + z[9]) + (z[10] + z[11])) + ((z[12] + z[13]) + (z[14] + z[15]));
-                    sum += other(sum);
-                    if (h == 0) sums[(t - t0) * KT + c] = sum;
-                }
-                // loads on every path, all of them waited for here: one that the compiler took to be on its way at the next tile would
-                // make it wait there for that tile's keys too
-                const uint32_t j0 = (uint32_t)t0 * KT + lane, j1 = std::min((uint32_t)t1 * KT, (uint32_t)S.len);
-                int64_t row[WINDOW / 2];
-                float old[WINDOW / 2];
+                    for (int e = 0; e < WINDOW / 2; ++e) row[e] = PAGED ? A.pages.table[S.k0 + (std::min(j0 + e * 64, j1 - 1) >> A.pages.log)] : 0;
 #pragma unroll
-                for (int e = 0; e < WINDOW / 2; ++e) row[e] = PAGED ? A.pages.table[S.k0 + (std::min(j0 + e * 64, j1 - 1) >> A.pages.log)] : 0;
+                    for (int e = 0; e < WINDOW / 2; ++e) {
+                        const uint32_t j = std::min(j0 + e * 64, j1 - 1);
+                        row[e] = PAGED ? A.pages.row((int)row[e], j) : S.k0 + j;
+                        old[e] = from[(row[e] < 0 ? 0 : row[e]) * step];
+                    }
 #pragma unroll
-                for (int e = 0; e < WINDOW / 2; ++e) {
-                    const uint32_t j = std::min(j0 + e * 64, j1 - 1);
-                    row[e] = PAGED ? A.pages.row((int)row[e], j) : S.k0 + j;
-                    old[e] = from[(row[e] < 0 ? 0 : row[e]) * step];
-                }
+                    for (int e = 0; e < WINDOW / 2; ++e) asm volatile("" : "+v"(old[e]));
 #pragma unroll
-                for (int e = 0; e < WINDOW / 2; ++e) asm volatile("" : "+v"(old[e]));
-#pragma unroll
-                for (int e = 0; e < WINDOW / 2; ++e) {
-                    const uint32_t j = j0 + e * 64;
-                    const float sum = sums[e * 64 + lane];
-                    if (j < j1) put(A, S, b, g, j, row[e], kept && !(begin && fresh(A, S, j)) ? fmaf(decay, old[e], sum) : sum);
+                    for (int e = 0; e < WINDOW / 2; ++e) {
+                        const uint32_t j = j0 + e * 64;
+                        const float sum = sums[e * 64 + lane];
+                        if (j < j1) put(A, S, b, g, j, row[e], kept && !(begin && fresh(A, S, j)) ? fmaf(decay, old[e], sum) : sum);
+                    }
                 }
             }
         }
