@@ -2,9 +2,16 @@
 //
 // w_j = decay before_j + sum over the queries i that see j, and the heads h of the key's group, of exp(scale q_ih . k_j - lse_ih).
 // The products z = q k^T leave a key to a lane: lane (c, h) (c = lane mod 32, h = lane / 32) has the scores of key c with the rows
-// 8 i + 4 h + j (i, j < 4), so a key's sum grows inside its lane. The keys stay in registers, 64 to a wave; the rows go through LDS
-// once for the four waves of a workgroup, the next tile asked for while this one is used. Products, exponents and sums are f32; a
-// sum grows by the sum of 16 weights at a time. No two lanes add to the same word, so the sums have one order.
+// 8 i + 4 h + j (i, j < 4), so a key's sum grows inside its lane. Products, exponents and sums are f32; a sum grows by the sum of 16
+// weights at a time. No two lanes add to the same word, so the sums have one order.
+//
+// weigh_k (prompts and chunks): the keys stay in registers, 64 to a wave; the rows go through LDS once for the four waves of a
+// workgroup, the next tile asked for while this one is used; rows are split over workgroups and joined where the keys are few.
+// weigh_few_k (up to 32 rows): the rows stay in registers and the keys are streamed.
+//
+// 8192 tokens x 32/8 heads of 128, causal, f16: 309 us, 890 TFLOP/s (a 16384^3 product: 1280). Power bounds it: with queries or
+// keys of zeros, whose products switch nothing, the same instructions take 234 us. Without the exponentials 292, without the
+// products 149. One product after the other, then its exponentials: 329; deeper buffers, other interleavings, three waves a SIMD: within 2%.
 #include <algorithm>
 
 #include "tiles.h"
@@ -12,7 +19,7 @@
 namespace pch {
 namespace clear {
 
-constexpr int BR = 64;   // rows of a tile: (query, head) pairs
+constexpr int rows_of(int dim) { return dim <= 128 ? 128 : 64; }  // rows of a tile: (query, head) pairs
 constexpr int BK = 256;  // keys of a workgroup
 
 struct Weigh {
@@ -102,7 +109,7 @@ template <class T, int DP, int DC>
 __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
     typedef typename Mat<T>::v8 v8;
     typedef int v4i __attribute__((ext_vector_type(4)));
-    constexpr int NW = 4, CPR = DP / 8, TB = BR * DP * 2, NL = BR * CPR / (64 * NW), STEPS = DC / 16;
+    constexpr int NW = 4, CPR = DP / 8, BR = rows_of(DP), TB = BR * DP * 2, NL = BR * CPR / (64 * NW), STEPS = DC / 16;
     __shared__ __attribute__((aligned(1024))) char lds[2 * TB];
     __shared__ __attribute__((aligned(16))) float nl[2][BR];  // less a row's log-sum-exp, in log2 units
     __shared__ __attribute__((aligned(16))) int lim[2][BR];   // the keys that it sees
@@ -124,7 +131,7 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
         row_of[n] = ch * 8 < A.dim && qi < A.qt ? x : BR;
         off[n] = ((uint32_t)qi * (uint32_t)A.q.token + (uint32_t)hd * (uint32_t)A.q.head) * 2 + ch * 16;
     }
-    const int xq = A.query(lane), xh = lane - xq * A.hb;  // the row whose log-sum-exp this lane of the first wave brings
+    const int x0 = threadIdx.x, xq = A.query(x0), xh = x0 - xq * A.hb;  // the row whose log-sum-exp this lane of the first waves brings
     const uint32_t to = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 1024;
     const T* const q = at<T>(A.q, S.q0, (int64_t)g * A.group);
     const float* const lse = A.lse + (int64_t)S.q0 * A.heads + (int64_t)g * A.group;
@@ -134,7 +141,7 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
         int i, hd, x;
     };
     const auto rows = [&](int t) {
-        const int qb = A.blocks == 1 ? t : t / A.blocks, i = qb * A.qt, hd = A.blocks == 1 ? 0 : (t - qb * A.blocks) * BR;
+        const int qb = A.blocks == 1 ? t : t / A.blocks, i = qb * A.qt, hd = A.blocks == 1 ? 0 : (t - qb * A.blocks) * A.hb;
         const int nq = S.n - i < A.qt ? S.n - i : A.qt, nh = A.group - hd < A.hb ? A.group - hd : A.hb;
         return Rows{i, hd, nq * nh};
     };
@@ -148,13 +155,13 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
     };
     const auto ask = [&](int t) {
         const Rows r = rows(t);
-        return lane < r.x ? lse[(int64_t)(r.i + xq) * A.heads + r.hd + xh] : -INFINITY;
+        return x0 < r.x ? lse[(int64_t)(r.i + xq) * A.heads + r.hd + xh] : -INFINITY;
     };
     const auto bring = [&](int t, int buf, float x) {
         const Rows r = rows(t);
-        nl[buf][lane] = x == -INFINITY ? x : x * -1.4426950408889634f;  // a row that sees no key adds nothing
+        nl[buf][x0] = x == -INFINITY ? x : x * -1.4426950408889634f;  // a row that sees no key adds nothing
         const int64_t sees = (int64_t)S.len - S.n + r.i + xq + 1;
-        lim[buf][lane] = lane >= r.x || sees < 0 ? 0 : (int)sees;
+        lim[buf][x0] = x0 >= r.x || sees < 0 ? 0 : (int)sees;
     };
 
     for (int64_t k0 = (int64_t)slot * BK; k0 < S.len; k0 += (int64_t)A.slots * BK) {
@@ -170,7 +177,7 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
         float raw = 0;
         if (t0 < t1) {
             load(t0, 0);
-            if (wave == 0) raw = ask(t0);
+            if (wave < BR / 64) raw = ask(t0);
         }
         // the keys of this wave, in registers; what the last tile has no key for is some row's, and not kept
         const uint32_t j = (uint32_t)k0 + wave * 64 + c, len = (uint32_t)S.len;
@@ -195,8 +202,8 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
         const auto tile = [&](int buf, int x, bool masked) __attribute__((always_inline)) {
             const char PCH_LDS* const l = (const char PCH_LDS*)lds + buf * TB + c * DP * 2;
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                if (rb && x <= 32) break;
+            for (int rb = 0; rb < BR / 32; ++rb) {
+                if (x <= 32 * rb) break;
                 v16f z[2];
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb) z[kb] = (v16f)0.0f;
@@ -227,9 +234,50 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
                 for (int kb = 0; kb < 2; ++kb) acc[kb] += (part[kb][0] + part[kb][1]) + (part[kb][2] + part[kb][3]);
             }
         };
+        // Rows that see all of the keys, up to 128 dimensions (above, the registers do not hold it): 32 rows' products beside the
+        // exponentials of the 32 before, across tiles; the last ones' scores z1 and their rows' m1 wait for the next products (at the
+        // beginning: none, weights of 0)
+        v16f z0[2], z1[2];
+        v4f m1[4];
+        const auto products = [&](int buf, int rb, v16f (&z)[2]) __attribute__((always_inline)) {
+            const char PCH_LDS* const l = (const char PCH_LDS*)lds + buf * TB + (32 * rb + c) * DP * 2;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) z[kb] = (v16f)0.0f;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const v8 a = *(const v8 PCH_LDS*)(l + (((2 * s + h) ^ Tile<DP>::kswz(c)) << 4));
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) z[kb] = Mat<T>::mul(a, kf[kb][s], z[kb]);
+            }
+        };
+        const auto weights = [&](const v16f (&z)[2], const v4f (&m)[4]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                float part[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(fmaf(z[kb][4 * i + e], c2, m[i][e]));
+                    part[i] = (w[0] + w[1]) + (w[2] + w[3]);
+                }
+                acc[kb] += (part[0] + part[1]) + (part[2] + part[3]);
+            }
+        };
+        const auto pair = [&](int buf, int rb) __attribute__((always_inline)) {
+            products(buf, 2 * rb, z0);
+            weights(z1, m1);
+            __builtin_amdgcn_sched_barrier(0);
+            v4f m0[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m0[i] = *(const v4f*)&nl[buf][64 * rb + 8 * i + 4 * h], m1[i] = *(const v4f*)&nl[buf][64 * rb + 32 + 8 * i + 4 * h];
+            products(buf, 2 * rb + 1, z1);
+            weights(z0, m0);
+            __builtin_amdgcn_sched_barrier(0);
+        };
         settled();
         if (t0 < t1) {
-            if (wave == 0) {
+            if (wave < BR / 64) {
                 bring(t0, 0, raw);
                 if (t0 + 1 < t1) raw = ask(t0 + 1);
             }
@@ -237,17 +285,27 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
                 const int buf = (t - t0) & 1;
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if (t + 1 < t1) {
-                    if (wave == 0) {
+                    if (wave < BR / 64) {
                         bring(t + 1, buf ^ 1, raw);
                         if (t + 2 < t1) raw = ask(t + 2);
                     }
                     load(t + 1, buf ^ 1);
                 }
+                if constexpr (DP <= 128)
+                    if (!masked) {
+#pragma unroll
+                        for (int rb = 0; rb < BR / 64; ++rb)
+                            if (64 * rb < rows(t).x) pair(buf, rb);
+                        return;
+                    }
                 tile(buf, rows(t).x, masked);
             };
             int t = t0;
             for (; t < t1 && t < whole; ++t) step(t, true);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z1[i & 1] = (v16f)0.0f, m1[i] = (v4f)-INFINITY;
             for (; t < t1; ++t) step(t, false);
+            if constexpr (DP <= 128) weights(z1, m1);
         }
         const float both[2] = {acc[0] + other(acc[0]), acc[1] + other(acc[1])}, sum = h ? both[1] : both[0];
         if (mine < len) {
@@ -488,6 +546,7 @@ static int checked(const KeyWeightsArgs* a, Weigh* w) {
     w->tokens = a->heads ? a->tokens : 0, w->seqs = a->seqs, w->heads = a->heads, w->kv_heads = a->kv_heads, w->dim = a->dim;
     w->causal = a->causal, w->max_k = a->max_k, w->scale = a->scale, w->decay = a->decay;
     w->group = a->heads && a->kv_heads ? a->heads / a->kv_heads : 1;
+    const int BR = rows_of(w->dim);
     w->hb = w->group < BR ? w->group : BR;
     w->per_hb = (65536 + w->hb - 1) / w->hb;
     w->qt = BR / w->hb;
@@ -497,8 +556,8 @@ static int checked(const KeyWeightsArgs* a, Weigh* w) {
     return 0;
 }
 
-// How the rows are split: keys alone give workgroups enough where there are 1024 (two waves a SIMD, twice over); where there are
-// fewer, parts of four tiles of rows and more. A workspace that is too small makes fewer of them.
+// How the rows are split: into workgroups for two a CU if they have a tile each, and up to 2048 where they have four tiles and more
+// (8192 tokens x 32 heads: 1024 workgroups 329 us, 2048 317, 4096 323, 8192 354). A workspace that is too small makes fewer.
 static uint64_t bytes_of(const Weigh& w, int parts) {
     return parts > 1 ? PCX_ATTENTION_COUNTERS * 4 + (uint64_t)parts * w.seqs * w.kv_heads * w.max_k * 4 : 0;
 }
@@ -507,7 +566,7 @@ static void choose(Weigh* w, int max_q, uint64_t room) {
     const int64_t keys = std::max<int64_t>(1, ((int64_t)w->max_k + BK - 1) / BK), most = std::max<int64_t>(1, std::min<int64_t>(65535, (1 << 20) / ((int64_t)w->seqs * w->kv_heads)));
     w->slots = (int)std::min(keys, most);
     const int64_t base = (int64_t)w->slots * w->seqs * w->kv_heads;
-    w->parts = (int)std::max<int64_t>(1, std::min<int64_t>(1024 / base, tiles / 4));
+    w->parts = (int)std::max<int64_t>({1, std::min<int64_t>(512 / base, tiles), std::min<int64_t>(2048 / base, tiles / 4)});
     while (w->parts > 1 && (bytes_of(*w, w->parts) > room || w->slots * w->parts > 65535)) w->parts /= 2;
 }
 
