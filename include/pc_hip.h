@@ -1257,7 +1257,9 @@ uint64_t pcx_key_weights_workspace(const KeyWeightsArgs* args);
  * are to go where the evicted ones j < keep lie, in rising order: moves[b][g][i] = (from, to), i < count[b][g], for pcx_move_rows.
  * At most `most` are written (count is what there are: at most keep, and at most len - keep); entries past them are left
  * as they were. kept_len (NULL: none; not k_len itself): min(keep, len), what the sequence's length is once its rows have moved.
- * Keys on a page outside the pool are evicted first. max_k: the longest run expected; it only chooses a kernel.
+ * Keys on a page outside the pool are evicted first. max_k: the longest run expected; it only chooses a kernel. work
+ * (pcx_evict_workspace's bytes, 0 but for few long runs, which take longer without; 16-byte aligned; it may be attention's, whose
+ * counters it leaves alone).
  * weights: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). */
 typedef struct EvictArgs {
     HeadsRef weights, places;
@@ -1267,11 +1269,14 @@ typedef struct EvictArgs {
     int32_t* moves;            /* [seqs][kv_heads][most][2] */
     int32_t* count;            /* [seqs][kv_heads] */
     int32_t* kept_len;         /* [seqs] */
+    void* work;
+    uint64_t work_bytes;
     int64_t rows;
     int32_t seqs, kv_heads, keep, recent, first, most, max_k, pad;
 } EvictArgs;
-PC_STATIC_ASSERT(sizeof(EvictArgs) == 160, "EvictArgs layout");
+PC_STATIC_ASSERT(sizeof(EvictArgs) == 176, "EvictArgs layout");
 int pcx_evict(const EvictArgs* args, pc_stream_t s);
+uint64_t pcx_evict_workspace(const EvictArgs* args);
 
 /* The moves of pcx_evict, in up to four tensors [rows][kv_heads][dim[i]] at once (keys, values, weights, places), elements of
  * size[i] = 2, 4 or 8 bytes: row `to` of sequence b and key head g becomes row `from`, i < min(count[b][g], most). Moves that leave

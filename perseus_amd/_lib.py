@@ -139,6 +139,7 @@ _SIGS = {
     "pcx_key_weights": (C.c_int, [vp, vp]),
     "pcx_key_weights_workspace": (C.c_uint64, [vp]),
     "pcx_evict": (C.c_int, [vp, vp]),
+    "pcx_evict_workspace": (C.c_uint64, [vp]),
     "pcx_move_rows": (C.c_int, [vp, vp]),
 }
 for _name, (_res, _args) in _SIGS.items():

@@ -219,7 +219,7 @@ class KeyWeightsArgs(C.Structure):
 class EvictArgs(C.Structure):
     """include/pc_hip.h EvictArgs."""
     _fields_ = [*_ref("weights"), *_ref("places"), ("cache", CacheRef), ("k_len", _vp), ("next_place", _vp), ("moves", _vp),
-                ("count", _vp), ("kept_len", _vp), ("rows", _i64), ("seqs", _i32), ("kv_heads", _i32), ("keep", _i32),
+                ("count", _vp), ("kept_len", _vp), ("work", _vp), ("work_bytes", C.c_uint64), ("rows", _i64), ("seqs", _i32), ("kv_heads", _i32), ("keep", _i32),
                 ("recent", _i32), ("first", _i32), ("most", _i32), ("max_k", _i32), ("pad", _i32)]
 
 
@@ -240,12 +240,12 @@ _QK_NORM_ROTARY = struct.Struct("@" + "Pqq" * 6 + "P" * 5 + "qq" + "i" * 7 + "f"
 _ATTENTION = struct.Struct("@" + "Pqq" * 4 + "P" * 5 + "Qq" + "i" * 9 + "f")
 _CACHE = struct.Struct("@PPqii")
 _KEY_WEIGHTS = struct.Struct("@" + "Pqq" * 5 + "PPqii" + "P" * 5 + "Qq" + "i" * 9 + "ffi")
-_EVICT = struct.Struct("@" + "Pqq" * 2 + "PPqii" + "P" * 5 + "q" + "i" * 8)
+_EVICT = struct.Struct("@" + "Pqq" * 2 + "PPqii" + "P" * 6 + "Qq" + "i" * 8)
 _MOVE_ROWS = struct.Struct("@" + "Pqq" * 4 + "PPqii" + "PPq" + "i" * 12)
 assert (_ROTARY.size, _QK_NORM_ROTARY.size, _ATTENTION.size) == (104, 232, 192)
 assert _CACHE.size == C.sizeof(CacheRef) == 32
 assert _KEY_WEIGHTS.size == C.sizeof(KeyWeightsArgs) == 256
-assert (_EVICT.size, C.sizeof(EvictArgs), _MOVE_ROWS.size, C.sizeof(MoveRowsArgs)) == (160, 160, 200, 200)
+assert (_EVICT.size, C.sizeof(EvictArgs), _MOVE_ROWS.size, C.sizeof(MoveRowsArgs)) == (176, 176, 200, 200)
 assert (C.sizeof(RotaryArgs), C.sizeof(QkNormRotaryArgs), C.sizeof(AttentionArgs)) == (104, 232, 192)
 
 
@@ -499,7 +499,7 @@ class Clear:
             *w, *p, *cache, _flat(k_len, "k_len", "i32", seqs),
             0 if next_place is None else _flat(next_place, "next_place", "i32", seqs),
             _flat(moves, "moves", "i32", None), _flat(count, "count", "i32", seqs * kv),
-            0 if kept_len is None else _flat(kept_len, "kept_len", "i32", seqs), rows, seqs, kv, keep, recent, first, moves.shape[2],
+            0 if kept_len is None else _flat(kept_len, "kept_len", "i32", seqs), *self._work, rows, seqs, kv, keep, recent, first, moves.shape[2],
             min(room if max_k is None else max_k, 0x7FFFFFFF), 0)
         check(LIB.pcx_evict(args, self.stream.h), "evict")
 

@@ -3,7 +3,9 @@
 // Kept are the `keep` keys of a (sequence, key head) whose weights are largest, protected ones before all others, the lower key
 // of two alike. The kept rows behind `keep` go to the gaps before it, both in rising order: as few moves as there are gaps, and
 // none of them reads what another writes, so that they all run at once, in place.
-#include "clear.h"
+#include <algorithm>
+
+#include "tiles.h"
 
 namespace pch {
 namespace clear {
@@ -40,11 +42,21 @@ static int rows_of(const CacheRef& c, int64_t seqs, int64_t rows, Rows* r) {
 }
 
 // ------------------------------------------------------------------------------------------------ the choice
+// A key's worth is a word of 64 bits, no two alike: the weight's bits in their order (protected keys above all), then the key's
+// number from the top down. Kept are the keys from the keep-th largest word on. That word is found by its digits from the top: the
+// words with the digits found so far are counted by their next one, 11 bits, in 2048 bins in LDS, until the bin that the last kept
+// word is in is kept whole or holds few enough to rank each against all. Weights spread over orders of magnitude take one digit.
+//
+// What bounds it are latencies: the loads of weights, places and pages, the counting's atomics, the barriers between.
+constexpr int WAVES = 16, THREADS = 64 * WAVES, BINS = 2048, RANKED = 1024;
+constexpr int SLICES = 16, GATHERED = 8192, LONG = 16384;
+
 struct Choice {
     HeadsRef weights, places;
     Rows cache;
     const int32_t *k_len, *next_place;
     int32_t *moves, *count, *kept_len;
+    char* work;
     int32_t seqs, keep, recent, first, most;
 };
 
@@ -55,162 +67,298 @@ __device__ __forceinline__ uint32_t ordered(float w) {
     const uint32_t u = __float_as_uint(w + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ uint64_t word(uint32_t key, uint32_t j) { return (uint64_t)key << 32 | ~j; }
 
-constexpr int WAVES = 16, BINS = 2048;
-
-// the sum over the lanes below and this one
-__device__ __forceinline__ uint32_t upto(uint32_t x) {
-    const int lane = threadIdx.x & 63;
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-
-// A workgroup takes a (sequence, key head). The smallest word kept is found digit by digit, 11, 11 and 10 bits from the top, by
-// counting the words with the digits found so far in 2048 bins; then ranks are counted by ballots, a wave a run of keys. A chunk
-// of 1024 E words stays in registers; of more keys than that the words are made again for each digit.
-struct Counts {
-    uint32_t hist[BINS], sums[3][WAVES], found[2];
+struct Shared {
+    uint32_t hist[BINS], sums[2][WAVES], found[3], n;
+    uint64_t ranked[RANKED], least;
 };
 
-template <int E>
-__device__ __forceinline__ void choose(const Choice& A, int b, Counts& S) {
-    constexpr int CHUNK = 64 * WAVES * E, BATCH = E > 16 ? 8 : 16;  // rows whose loads are on their way at once
-    auto& hist = S.hist;
-    auto& sums = S.sums;
-    auto& found = S.found;
-    const int g = blockIdx.x, kv = gridDim.x;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int len = A.k_len[b];
-    const int64_t at = A.cache.begin(b, &len);
-    int32_t* const count = A.count + (int64_t)b * kv + g;
-    if (A.kept_len && g == 0 && threadIdx.x == 0) A.kept_len[b] = len < A.keep ? len : A.keep;
-    if (len <= A.keep || A.keep == 0) {
-        if (threadIdx.x == 0) *count = 0;
-        return;
+// the sum over the lanes of the waves before this one, and over all, of what each wave brings (the same to all its lanes)
+__device__ __forceinline__ uint32_t waves_before(uint32_t (&sums)[WAVES], uint32_t mine, uint32_t* all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (lane == 0) sums[wave] = mine;
+    __syncthreads();
+    const int in = lane_sums(lane < WAVES ? (int)sums[lane] : 0);
+    *all = __builtin_amdgcn_readlane(in, WAVES - 1);
+    return wave ? __builtin_amdgcn_readlane(in, wave - 1) : 0;
+}
+
+// the bin that the need-th largest is in: (bin, how many of its words are among them, its words), in found; x and y are the counts of
+// bins BINS - 1 - 2 thread and the one below
+__device__ __forceinline__ void find(Shared& S, uint32_t x, uint32_t y, uint32_t need) {
+    const uint32_t in = lane_sums(x + y);
+    uint32_t all;
+    if (threadIdx.x < 3) S.found[threadIdx.x] = 0;  // of fewer words than that: none
+    const uint32_t before = waves_before(S.sums[0], __builtin_amdgcn_readlane(in, 63), &all) + in - x - y;
+    if (before < need && need <= before + x + y) {
+        const bool second = need > before + x;
+        S.found[0] = BINS - 1 - 2 * threadIdx.x - second;
+        S.found[1] = need - before - (second ? x : 0);
+        S.found[2] = second ? y : x;
     }
-    const int64_t next = A.next_place ? A.next_place[b] : len;
-    const float* const w = (const float*)A.weights.base + g * A.weights.head;
-    const int32_t* const places = A.places.base ? (const int32_t*)A.places.base + g * A.places.head : nullptr;
-    uint32_t key[E];
-    int c0, seg;  // the chunk in registers: its first key, the keys of a wave's run
-    const auto load = [&](int from) {
-        c0 = from;
-        const int n = len - from < CHUNK ? len - from : CHUNK;
-        seg = 64 * ((n + 64 * WAVES - 1) / (64 * WAVES));
-#pragma unroll
-        for (int e0 = 0; e0 < E; e0 += BATCH) {
-            if (e0 * 64 >= seg) break;
-            int64_t row[BATCH];
-#pragma unroll
-            for (int e = 0; e < BATCH; ++e) {
-                const int j = from + wave * seg + (e0 + e) * 64 + lane;
-                row[e] = (e0 + e) * 64 < seg && j < len ? A.cache.row(at, j) : -1;
-            }
-            float x[BATCH];
-            int place[BATCH];
-#pragma unroll
-            for (int e = 0; e < BATCH; ++e) {
-                x[e] = row[e] < 0 ? 0 : w[row[e] * A.weights.token];
-                place[e] = row[e] < 0 ? 0 : places ? places[row[e] * A.places.token] : from + wave * seg + (e0 + e) * 64 + lane;
-            }
-#pragma unroll
-            for (int e = 0; e < BATCH; ++e)
-                key[e0 + e] = row[e] < 0 ? 0 : place[e] >= next - A.recent || place[e] < A.first ? PROTECTED : ordered(x[e]);
+    __syncthreads();
+}
+
+// The need-th largest (need >= 1) of the words that each(f) calls f with, on the lanes that have them.
+template <class Each>
+__device__ __forceinline__ uint64_t select(Shared& S, uint32_t need, Each each) {
+    uint64_t prefix = 0;
+    for (int low = 53;; low = low == 32 ? 21 : low > 32 ? std::max(low - 11, 32) : std::max(low - 11, 0)) {
+        const int bits = low == 32 || low == 0 ? 10 : 11, above = low + bits;
+        S.hist[threadIdx.x] = S.hist[threadIdx.x + THREADS] = 0;
+        if (threadIdx.x == 0) S.n = 0;
+        __syncthreads();
+        each([&](uint64_t w) {
+            if (above == 64 || w >> above == prefix) atomicAdd(&S.hist[(w >> low) & ((1u << bits) - 1)], 1);
+        });
+        __syncthreads();
+        find(S, S.hist[BINS - 1 - 2 * threadIdx.x], S.hist[BINS - 2 - 2 * threadIdx.x], need);
+        prefix = prefix << bits | S.found[0];
+        need = S.found[1];
+        const uint32_t n = S.found[2];
+        if (n == need || low == 0) return prefix << low;
+        if (n > RANKED) continue;
+        each([&](uint64_t w) {
+            if (w >> low == prefix) S.ranked[atomicAdd(&S.n, 1) % RANKED] = w;  // (n of them, unless weights change meanwhile)
+        });
+        __syncthreads();
+        if (threadIdx.x < n) {
+            const uint64_t mine = S.ranked[threadIdx.x];
+            uint32_t larger = 0;
+            for (uint32_t i = 0; i < n; ++i) larger += S.ranked[i] > mine;
+            if (larger == need - 1) S.least = mine;
         }
-    };
-    // f(e, j, key) for the chunk's keys of this lane, in the order of e
-    const auto each = [&](auto f) {
+        __syncthreads();
+        return S.least;
+    }
+}
+
+// the words of a (sequence, key head)'s keys, E in the registers of each lane: a wave's lanes hold runs of 64 keys, its runs one
+// after the other
+template <int E>
+struct Words {
+    const Choice& A;
+    const int g, len;
+    const int64_t at, next;
+    uint32_t key[E];
+    int from, seg;  // the chunk in registers: its first key, the keys of a wave's run
+    static constexpr int CHUNK = THREADS * E;
+
+    __device__ __forceinline__ Words(const Choice& a, int g, int b, int len, int64_t at)
+        : A(a), g(g), len(len), at(at), next(a.next_place ? a.next_place[b] : len), from(0), seg(0) {}
+    __device__ __forceinline__ int first() const { return from + (int)(threadIdx.x >> 6) * seg + (int)(threadIdx.x & 63); }
+    // the chunk of keys lo .. hi - 1, E loads of each kind on their way at once
+    __device__ __forceinline__ void load(int lo, int hi) {
+        const float* const w = (const float*)A.weights.base + g * A.weights.head;
+        const int32_t* const places = A.places.base ? (const int32_t*)A.places.base + g * A.places.head : nullptr;
+        from = lo;
+        seg = 64 * ((hi - lo + THREADS - 1) / THREADS);
+        int64_t row[E];
+        float x[E];
+        int place[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) row[e] = e * 64 < seg && first() + e * 64 < hi ? A.cache.row(at, first() + e * 64) : -1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            x[e] = row[e] < 0 ? 0 : w[row[e] * A.weights.token];
+            place[e] = row[e] < 0 ? 0 : places ? places[row[e] * A.places.token] : first() + e * 64;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) key[e] = row[e] < 0 ? 0 : place[e] >= next - A.recent || place[e] < A.first ? PROTECTED : ordered(x[e]);
+    }
+    // f(e, j, word, whether there is one) in the order of e
+    template <class F>
+    __device__ __forceinline__ void each(int hi, F f) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             if (e * 64 >= seg) break;
-            const int j = c0 + wave * seg + e * 64 + lane;
-            f(e, j, key[e], j < len);
+            const int j = first() + e * 64;
+            f(e, j, word(key[e], j), j < hi);
         }
-    };
-    const bool once = len <= CHUNK;
-    if (once) load(0);
-    uint32_t prefix = 0, need = A.keep;
-    for (int p = 0; p < 3; ++p) {
-        const int low = p == 0 ? 21 : p == 1 ? 10 : 0, above = p == 0 ? 0 : p == 1 ? 21 : 10;
-        const uint32_t mask = p == 2 ? 1023 : 2047;
-        hist[threadIdx.x] = hist[threadIdx.x + 1024] = 0;
-        __syncthreads();
-        for (int from = 0; from < len; from += CHUNK) {
-            if (!once) load(from);
-            each([&](int, int, uint32_t k, bool in) {
-                if (in && (p == 0 || k >> above == prefix)) atomicAdd(&hist[(k >> low) & mask], 1);
+    }
+    // f(word) for the keys lo .. hi - 1; loaded: they are in registers
+    template <class F>
+    __device__ __forceinline__ void all(int lo, int hi, bool loaded, F f) {
+        for (int c = lo; c < hi; c += std::min(CHUNK, hi - c)) {
+            const int end = c + std::min(CHUNK, hi - c);
+            if (!loaded) load(c, end);
+            each(end, [&](int, int, uint64_t w, bool in) {
+                if (in) f(w);
             });
         }
-        __syncthreads();
-        // bins from the top, two to a thread: the one where the words kept begin
-        const uint32_t x = hist[BINS - 1 - 2 * threadIdx.x], y = hist[BINS - 2 - 2 * threadIdx.x], in = upto(x + y);
-        if (lane == 63) sums[0][wave] = in;
-        __syncthreads();
-        uint32_t before = in - x - y;
-        for (int v = 0; v < wave; ++v) before += sums[0][v];
-        if (before < need && need <= before + x + y) {
-            const bool second = need > before + x;
-            found[0] = BINS - 1 - 2 * threadIdx.x - second;
-            found[1] = need - before - (second ? x : 0);
-        }
-        __syncthreads();
-        prefix = p == 0 ? found[0] : prefix << (p == 1 ? 11 : 10) | found[0];
-        need = found[1];  // of the words with these digits
     }
-    // prefix: the smallest word kept; need: how many of those alike stay, the lowest
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    int32_t* const moves = A.moves + ((int64_t)b * kv + g) * A.most * 2;
-    uint32_t ties = 0, movers = 0, holes = 0;  // of the chunks before
-    for (int from = 0; from < len; from += CHUNK) {
-        if (!once) load(from);
-        uint32_t n = 0;
-        each([&](int, int, uint32_t k, bool in) { n += __popcll(__ballot(in && k == prefix)); });
-        if (lane == 0) sums[0][wave] = n;
-        __syncthreads();
-        uint32_t tie = ties, m = 0, h = 0;
-        for (int v = 0; v < WAVES; ++v) {
-            tie += v < wave ? sums[0][v] : 0;
-            ties += sums[0][v];
+    // The moves of the keys lo .. hi - 1, least: the smallest word kept; movers, holes: of the keys before (each counts only from or to
+    // `keep`), added to.
+    __device__ __forceinline__ void emit(Shared& S, int lo, int hi, bool loaded, uint64_t least, int32_t* moves, uint32_t& movers, uint32_t& holes) {
+        const uint64_t below = ((uint64_t)1 << (threadIdx.x & 63)) - 1;
+        for (int c = lo; c < hi; c += std::min(CHUNK, hi - c)) {
+            const int end = c + std::min(CHUNK, hi - c);
+            if (!loaded) load(c, end);
+            uint32_t m = 0, h = 0, all_m, all_h;
+            each(end, [&](int, int j, uint64_t w, bool in) {
+                m += __popcll(__ballot(in && w >= least && j >= A.keep));
+                h += __popcll(__ballot(in && w < least && j < A.keep));
+            });
+            m = movers + waves_before(S.sums[0], m, &all_m);
+            h = holes + waves_before(S.sums[1], h, &all_h);
+            movers += all_m;
+            holes += all_h;
+            each(end, [&](int, int j, uint64_t w, bool in) {
+                const bool mover = in && w >= least && j >= A.keep, hole = in && w < least && j < A.keep;
+                const uint64_t ms = __ballot(mover), hs = __ballot(hole);
+                const uint32_t to = m + __popcll(ms & below), gap = h + __popcll(hs & below);
+                if (mover && to < (uint32_t)A.most) moves[2 * (int64_t)to] = j;
+                if (hole && gap < (uint32_t)A.most) moves[2 * (int64_t)gap + 1] = j;
+                m += __popcll(ms);
+                h += __popcll(hs);
+            });
+            __syncthreads();
         }
-        uint64_t kept = 0;
-        each([&](int e, int j, uint32_t k, bool in) {
-            const uint64_t alike = __ballot(in && k == prefix);
-            const bool stays = in && (k > prefix || (k == prefix && tie + __popcll(alike & below) < need));
-            tie += __popcll(alike);
-            kept |= (uint64_t)stays << e;
-            m += __popcll(__ballot(stays && j >= A.keep));
-            h += __popcll(__ballot(in && !stays && j < A.keep));
-        });
-        if (lane == 0) sums[1][wave] = m, sums[2][wave] = h;
-        __syncthreads();
-        m = movers, h = holes;
-        for (int v = 0; v < WAVES; ++v) {
-            m += v < wave ? sums[1][v] : 0;
-            h += v < wave ? sums[2][v] : 0;
-            movers += sums[1][v];
-            holes += sums[2][v];
-        }
-        each([&](int e, int j, uint32_t, bool in) {
-            const bool stays = kept >> e & 1;
-            const uint64_t mover = __ballot(stays && j >= A.keep), hole = __ballot(in && !stays && j < A.keep);
-            const uint32_t to = m + __popcll(mover & below), gap = h + __popcll(hole & below);
-            if (stays && j >= A.keep && to < (uint32_t)A.most) moves[2 * (int64_t)to] = j;
-            if (in && !stays && j < A.keep && gap < (uint32_t)A.most) moves[2 * (int64_t)gap + 1] = j;
-            m += __popcll(mover);
-            h += __popcll(hole);
-        });
-        __syncthreads();
     }
-    if (threadIdx.x == 0) *count = (int32_t)holes;
+};
+
+// a workgroup for each (sequence, key head)
+template <int E>
+__global__ void __launch_bounds__(THREADS) evict_k(Choice A) {
+    __shared__ Shared S;
+    const int g = blockIdx.x, kv = gridDim.x;
+    for (int b = blockIdx.y; b < A.seqs; b += gridDim.y) {
+        int len = A.k_len[b];
+        const int64_t at = A.cache.begin(b, &len), pair = (int64_t)b * kv + g;
+        if (A.kept_len && g == 0 && threadIdx.x == 0) A.kept_len[b] = len < A.keep ? len : A.keep;
+        uint32_t movers = 0, holes = 0;
+        if (len > A.keep && A.keep) {
+            Words<E> W(A, g, b, len, at);
+            const bool once = len <= W.CHUNK;
+            if (once) W.load(0, len);
+            const uint64_t least = select(S, A.keep, [&](auto f) { W.all(0, len, once, f); });
+            W.emit(S, 0, len, once, least, A.moves + pair * A.most * 2, movers, holes);
+        }
+        if (threadIdx.x == 0) A.count[pair] = (int32_t)holes;
+    }
 }
 
-template <int E>
-__global__ void __launch_bounds__(64 * WAVES) evict_k(Choice A) {
-    __shared__ Counts S;
-    for (int b = blockIdx.y; b < A.seqs; b += gridDim.y) choose<E>(A, b, S);
+// ------------------------------------------------------------------------------------------------ long caches
+// Few pairs of long runs: 16 workgroups to each, a slice of its keys each (no slice on both sides of `keep`), in three launches. The
+// slices' counts of the first digit; the words of the bin that is kept in part, gathered (8192 at most: of more, a few weights shared
+// by thousands of keys, each workgroup goes through all words by itself); the smallest word kept, and the slices' moves.
+struct Pair {
+    uint32_t hist[SLICES][BINS];
+    uint64_t gathered[GATHERED];
+    uint32_t found[3], kept[SLICES], some[SLICES];  // kept for certain, of the bin
+};
+static_assert(sizeof(Pair) % 8 == 0, "the gathered words stay aligned");
+
+struct Slice {
+    int lo, hi, before;  // its keys; the slices on its side of `keep` begin with this one
+};
+__device__ __forceinline__ Slice slice_of(int s, int len, int keep) {
+    int left = (int)((int64_t)SLICES * keep / len);
+    left = left < 1 ? 1 : left > SLICES - 1 ? SLICES - 1 : left;
+    const auto cut = [](int n, int i, int of) { return (int)((int64_t)n * i / of); };
+    if (s < left) return {cut(keep, s, left), cut(keep, s + 1, left), 0};
+    const int n = len - keep, of = SLICES - left;
+    return {keep + cut(n, s - left, of), keep + cut(n, s - left + 1, of), left};
+}
+
+template <int STAGE>
+__global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
+    __shared__ Shared S;
+    constexpr int E = 8;
+    const int g = blockIdx.x, kv = gridDim.x, s = blockIdx.y, b = blockIdx.z;
+    int len = A.k_len[b];
+    const int64_t at = A.cache.begin(b, &len), pair = (int64_t)b * kv + g;
+    if (STAGE == 2 && A.kept_len && g == 0 && s == 0 && threadIdx.x == 0) A.kept_len[b] = len < A.keep ? len : A.keep;
+    if (len <= A.keep || A.keep == 0) {
+        if (STAGE == 2 && s == 0 && threadIdx.x == 0) A.count[pair] = 0;
+        return;
+    }
+    Pair& P = ((Pair*)A.work)[pair];
+    const Slice mine = slice_of(s, len, A.keep);
+    Words<E> W(A, g, b, len, at);
+    if constexpr (STAGE == 0) {
+        S.hist[threadIdx.x] = S.hist[threadIdx.x + THREADS] = 0;
+        __syncthreads();
+        W.all(mine.lo, mine.hi, false, [&](uint64_t w) { atomicAdd(&S.hist[w >> 53], 1); });
+        __syncthreads();
+        *(uint2*)&P.hist[s][2 * threadIdx.x] = *(const uint2*)&S.hist[2 * threadIdx.x];
+    } else if constexpr (STAGE == 1) {
+        if (threadIdx.x == 0) S.n = 0;
+        const int at2 = BINS - 2 - 2 * threadIdx.x;
+        uint32_t x = 0, y = 0;
+        uint2 own = make_uint2(0, 0);
+#pragma unroll
+        for (int i = 0; i < SLICES; ++i) {
+            const uint2 c = *(const uint2*)&P.hist[i][at2];
+            x += c.y, y += c.x;
+            if (i == s) own = c;
+        }
+        find(S, x, y, A.keep);
+        const uint32_t bin = S.found[0], n = S.found[2];
+        // the words of this slice above the bin, and of the slices before in it
+        uint32_t above;
+        const uint32_t sum = lane_sums((uint32_t)at2 > bin ? own.x + own.y : (uint32_t)at2 + 1 > bin ? own.y : 0);
+        waves_before(S.sums[1], __builtin_amdgcn_readlane(sum, 63), &above);
+        if (threadIdx.x == 0) {
+            P.kept[s] = above;
+            P.some[s] = P.hist[s][bin];
+            if (s == 0) P.found[0] = bin, P.found[1] = S.found[1], P.found[2] = n;
+        }
+        if (n > GATHERED || n == S.found[1]) return;
+        uint32_t to = 0;
+        for (int i = 0; i < s; ++i) to += P.hist[i][bin];
+        W.all(mine.lo, mine.hi, false, [&](uint64_t w) {
+            if (w >> 53 == bin) P.gathered[(to + atomicAdd(&S.n, 1)) % GATHERED] = w;
+        });
+    } else {
+        const uint32_t bin = P.found[0], need = P.found[1], n = P.found[2];
+        uint64_t least = (uint64_t)bin << 53;
+        uint32_t movers = 0, holes = 0, before = 0;  // kept of the slices on this side before this one
+        if (n > GATHERED) {
+            least = select(S, A.keep, [&](auto f) { W.all(0, len, false, f); });
+            const int from = mine.before ? A.keep : 0;
+            uint32_t kept = 0;
+            W.all(from, mine.lo, false, [&](uint64_t w) { kept += w >= least; });
+            __syncthreads();
+            waves_before(S.sums[0], __builtin_amdgcn_readlane(lane_sums(kept), 63), &before);
+            __syncthreads();
+        } else {
+            uint32_t some = 0, to = 0, from = 0;  // the bin's words before this slice, and before its side
+            for (int i = 0; i < s; ++i) {
+                if (i < mine.before) from += P.some[i];
+                to += P.some[i];
+                if (i >= mine.before) before += P.kept[i];
+            }
+            if (n == need) {
+                before += to - from;
+            } else {
+                uint64_t w[GATHERED / THREADS];
+#pragma unroll
+                for (int i = 0; i < GATHERED / THREADS; ++i) w[i] = threadIdx.x + i * THREADS < n ? P.gathered[threadIdx.x + i * THREADS] : 0;
+                least = select(S, need, [&](auto f) {
+#pragma unroll
+                    for (int i = 0; i < GATHERED / THREADS; ++i)
+                        if (threadIdx.x + i * THREADS < n) f(w[i]);
+                });
+#pragma unroll
+                for (int i = 0; i < GATHERED / THREADS; ++i) {
+                    const uint32_t k = threadIdx.x + i * THREADS;
+                    some += k >= from && k < to && w[i] >= least;
+                }
+                uint32_t all;
+                waves_before(S.sums[1], __builtin_amdgcn_readlane(lane_sums(some), 63), &all);
+                before += all;
+                __syncthreads();
+            }
+        }
+        if (mine.before)
+            movers = before;
+        else
+            holes = mine.lo - before;
+        W.emit(S, mine.lo, mine.hi, false, least, A.moves + pair * A.most * 2, movers, holes);
+        if (!mine.before && mine.hi == A.keep && threadIdx.x == 0) A.count[pair] = (int32_t)holes;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ the moves
@@ -273,6 +421,14 @@ __global__ void __launch_bounds__(256) move_k(Moves A) {
 using namespace pch;
 using namespace pch::clear;
 
+// Few pairs of long runs: their workgroups alone do not fill the chip, and one takes long (65536 keys x 8 heads: FIGURES).
+static bool is_long(const EvictArgs& a) { return a.max_k > LONG && (int64_t)a.seqs * a.kv_heads < 256; }
+static uint64_t work_bytes(const EvictArgs& a) { return PCX_ATTENTION_COUNTERS * 4 + (uint64_t)a.seqs * a.kv_heads * sizeof(Pair); }
+
+extern "C" uint64_t pcx_evict_workspace(const EvictArgs* a) {
+    return a && a->seqs > 0 && a->kv_heads > 0 && is_long(*a) ? work_bytes(*a) : 0;
+}
+
 extern "C" int pcx_evict(const EvictArgs* a, pc_stream_t s) {
     if (!a || a->seqs < 0 || a->kv_heads < 0 || a->keep < 0 || a->recent < 0 || a->first < 0 || a->most < 0 || a->max_k < 0) return -1;
     if ((int64_t)a->recent + a->first > a->keep) return -1;
@@ -281,14 +437,28 @@ extern "C" int pcx_evict(const EvictArgs* a, pc_stream_t s) {
     const bool any = a->seqs && a->kv_heads;
     if (any && (!a->k_len || !a->count || (a->most && !a->moves) || a->kept_len == a->k_len)) return -1;
     if (!usable(a->weights, any ? a->rows : 0, a->kv_heads) || a->places.token < 0 || a->places.head < 0) return -1;
-    if (((uintptr_t)a->weights.base | (uintptr_t)a->places.base) % 4 || a->kv_heads > 65535) return -2;
+    if (((uintptr_t)a->weights.base | (uintptr_t)a->places.base) % 4 || (uintptr_t)a->work % 16 || a->kv_heads > 65535) return -2;
     if (!any) return 0;
     c.weights = settled(a->weights, a->rows, a->kv_heads, 1), c.places = settled(a->places, a->rows, a->kv_heads, 1);
     c.k_len = a->k_len, c.next_place = a->next_place;
     c.moves = a->moves, c.count = a->count, c.kept_len = a->kept_len;
     c.seqs = a->seqs, c.keep = a->keep, c.recent = a->recent, c.first = a->first, c.most = a->most;
-    const dim3 grid(a->kv_heads, a->seqs < 65535 ? a->seqs : 65535);
-    hipLaunchKernelGGL((evict_k<16>), grid, dim3(64 * WAVES), 0, (hipStream_t)s, c);
+    const hipStream_t st = (hipStream_t)s;
+    if (is_long(*a) && a->work && a->work_bytes >= work_bytes(*a)) {
+        c.work = (char*)a->work + PCX_ATTENTION_COUNTERS * 4;
+        const dim3 grid(a->kv_heads, SLICES, a->seqs), block(THREADS);
+        hipLaunchKernelGGL((evict_long_k<0>), grid, block, 0, st, c);
+        if (int e = launch_rc()) return e;
+        hipLaunchKernelGGL((evict_long_k<1>), grid, block, 0, st, c);
+        if (int e = launch_rc()) return e;
+        hipLaunchKernelGGL((evict_long_k<2>), grid, block, 0, st, c);
+        return launch_rc();
+    }
+    const dim3 grid(a->kv_heads, std::min(a->seqs, 65535)), block(THREADS);
+    if (a->max_k <= 8 * THREADS)
+        hipLaunchKernelGGL((evict_k<8>), grid, block, 0, st, c);
+    else
+        hipLaunchKernelGGL((evict_k<16>), grid, block, 0, st, c);
     return launch_rc();
 }
 
