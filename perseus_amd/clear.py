@@ -321,7 +321,7 @@ def _per_key(x, name, dtype, shape=None):
         raise ValueError(f"{name}: not on the device")
     if (_known.get(x.dtype) or _type(x.dtype)) != dtype or len(x.shape) != 2:
         raise ValueError(f"{name}: {dtype} [rows][kv heads] is wanted, got {x.dtype} {tuple(x.shape)}")
-    if shape is not None and tuple(x.shape) != tuple(shape):
+    if shape is not None and x.shape != shape:
         raise ValueError(f"{name}: {tuple(shape)} is wanted, got {tuple(x.shape)}")
     return (x.data_ptr(), *x.stride())
 
@@ -487,8 +487,9 @@ class Clear:
         are never more than keep, or than the longest run less keep). max_k: the longest run expected; it only chooses a kernel."""
         seqs = k_len.shape[0]
         rows, kv = weights.shape if len(weights.shape) == 2 else (0, 0)
-        if len(moves.shape) != 4 or tuple(moves.shape[:2]) != (seqs, kv) or moves.shape[3] != 2:
-            raise ValueError(f"moves: [{seqs}][{kv}][most][2] is wanted, got {tuple(moves.shape)}")
+        shape = moves.shape
+        if len(shape) != 4 or shape[0] != seqs or shape[1] != kv or shape[3] != 2:
+            raise ValueError(f"moves: [{seqs}][{kv}][most][2] is wanted, got {tuple(shape)}")
         if min(keep, recent, first) < 0 or first + recent > keep:
             raise ValueError(f"keep {keep}, recent {recent}, first {first}: none negative, no more protected than kept")
         w = _per_key(weights, "weights", "f32")
@@ -499,29 +500,30 @@ class Clear:
             *w, *p, *cache, _flat(k_len, "k_len", "i32", seqs),
             0 if next_place is None else _flat(next_place, "next_place", "i32", seqs),
             _flat(moves, "moves", "i32", None), _flat(count, "count", "i32", seqs * kv),
-            0 if kept_len is None else _flat(kept_len, "kept_len", "i32", seqs), *self._work, rows, seqs, kv, keep, recent, first, moves.shape[2],
+            0 if kept_len is None else _flat(kept_len, "kept_len", "i32", seqs), *self._work, rows, seqs, kv, keep, recent, first, shape[2],
             min(room if max_k is None else max_k, 0x7FFFFFFF), 0)
         check(LIB.pcx_evict(args, self.stream.h), "evict")
 
     def move_rows(self, moves, count, tensors, k_start=None, pages=None, page_rows=None):
         """The moves that evict chose, in up to four tensors [rows][kv heads][dim] or [rows][kv heads] of any types at once, by any
         strides of rows and heads: keys, values, their weights and places. Rows move in place, all moves at once."""
-        if len(moves.shape) != 4 or moves.shape[3] != 2 or not 1 <= len(tensors) <= 4:
+        shape = moves.shape
+        if len(shape) != 4 or shape[3] != 2 or not 1 <= len(tensors) <= 4:
             raise ValueError("moves [sequences][kv heads][most][2], and one to four tensors")
-        seqs, kv, most, _ = moves.shape
+        seqs, kv, most, _ = shape
         refs, sizes, dims, rows = [], [], [], None
         for x in tensors:
-            if len(x.shape) == 3:
-                at, row, head, shape, kind = _heads(x, "tensors")
-                dims.append(shape[2])
+            kind = _known.get(x.dtype) or _type(x.dtype)
+            if len(x.shape) == 2:
+                refs += _per_key(x, "tensors", kind)
+                (r, heads), dim = x.shape, 1
             else:
-                kind = _known.get(x.dtype) or _type(x.dtype)
-                at, row, head = _per_key(x, "tensors", kind)
-                dims.append(1)
-            if x.shape[1] != kv or rows not in (None, x.shape[0]):
+                at, row, head, (r, heads, dim), _ = _heads(x, "tensors")
+                refs += at, row, head
+            if heads != kv or rows not in (None, r):
                 raise ValueError(f"tensors: the same rows and {kv} key heads each")
-            rows = x.shape[0]
-            refs += at, row, head
+            rows = r
+            dims.append(dim)
             sizes.append(SIZES[kind])
         n = 4 - len(tensors)
         args = _MOVE_ROWS.pack(*refs, *[0] * 3 * n, *_cache(k_start, pages, page_rows, seqs), _flat(moves, "moves", "i32", None),

@@ -220,7 +220,7 @@ struct Words {
 
 // a workgroup for each (sequence, key head)
 template <int E>
-__global__ void __launch_bounds__(THREADS) evict_k(Choice A) {
+__global__ void __launch_bounds__(THREADS, E > 8 ? 4 : 8) evict_k(Choice A) {
     __shared__ Shared S;
     const int g = blockIdx.x, kv = gridDim.x;
     for (int b = blockIdx.y; b < A.seqs; b += gridDim.y) {
@@ -277,10 +277,12 @@ __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
     Pair& P = ((Pair*)A.work)[pair];
     const Slice mine = slice_of(s, len, A.keep);
     Words<E> W(A, g, b, len, at);
+    const bool once = mine.hi - mine.lo <= W.CHUNK;
+    if (once) W.load(mine.lo, mine.hi);
     if constexpr (STAGE == 0) {
         S.hist[threadIdx.x] = S.hist[threadIdx.x + THREADS] = 0;
         __syncthreads();
-        W.all(mine.lo, mine.hi, false, [&](uint64_t w) { atomicAdd(&S.hist[w >> 53], 1); });
+        W.all(mine.lo, mine.hi, once, [&](uint64_t w) { atomicAdd(&S.hist[w >> 53], 1); });
         __syncthreads();
         *(uint2*)&P.hist[s][2 * threadIdx.x] = *(const uint2*)&S.hist[2 * threadIdx.x];
     } else if constexpr (STAGE == 1) {
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
         if (n > GATHERED || n == S.found[1]) return;
         uint32_t to = 0;
         for (int i = 0; i < s; ++i) to += P.hist[i][bin];
-        W.all(mine.lo, mine.hi, false, [&](uint64_t w) {
+        W.all(mine.lo, mine.hi, once, [&](uint64_t w) {
             if (w >> 53 == bin) P.gathered[(to + atomicAdd(&S.n, 1)) % GATHERED] = w;
         });
     } else {
@@ -320,6 +322,7 @@ __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
             const int from = mine.before ? A.keep : 0;
             uint32_t kept = 0;
             W.all(from, mine.lo, false, [&](uint64_t w) { kept += w >= least; });
+            if (once) W.load(mine.lo, mine.hi);
             __syncthreads();
             waves_before(S.sums[0], __builtin_amdgcn_readlane(lane_sums(kept), 63), &before);
             __syncthreads();
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
             movers = before;
         else
             holes = mine.lo - before;
-        W.emit(S, mine.lo, mine.hi, false, least, A.moves + pair * A.most * 2, movers, holes);
+        W.emit(S, mine.lo, mine.hi, once, least, A.moves + pair * A.most * 2, movers, holes);
         if (!mine.before && mine.hi == A.keep && threadIdx.x == 0) A.count[pair] = (int32_t)holes;
     }
 }
