@@ -1208,8 +1208,8 @@ PC_STATIC_ASSERT(sizeof(CacheRef) == 32, "CacheRef layout");
 
 /* pcx_attention over keys and values in pages (cache.start is NULL; attention.k_start is not read): sequence b has the first
  * k_len[b] keys of its pages, what lies past width page_rows is cut off. Sequences may share pages (a prefix that they have in
- * common). Keys and values on a page outside the pool read as zeros: such a key's score is 0 and counts. All else is
- * pcx_attention's, its workspace and counters too; max_k is at most width page_rows. */
+ * common). Keys and values on a page outside the pool read as zeros: such a key's score is 0 and counts. page_rows times a key or
+ * value row's stride is below 2^31. All else is pcx_attention's, its workspace and counters too; max_k is at most width page_rows. */
 typedef struct AttentionPagedArgs {
     AttentionArgs attention;
     CacheRef cache;
@@ -1228,8 +1228,8 @@ uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args); /* as pc
  * place after the sequence's last token). Rows of no sequence are left as they were; sequences may not share rows. Sums are f32 and have one order.
  *
  * weights, before: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). Keys on a page outside the pool have
- * no row. Types, dim, scale and alignment as pcx_attention's; a query's row and head strides below 2^22 elements; seqs and
- * kv_heads below 65536; decay >= 0 and finite. max_q and max_k are the longest runs expected: they choose the split of the rows, no result
+ * no row. Types, dim, scale and alignment as pcx_attention's; a query's row and head strides below 2^22 elements, page_rows
+ * times a key row's below 2^31; seqs and kv_heads below 65536; decay >= 0 and finite. max_q and max_k are the longest runs expected: they choose the split of the rows, no result
  * depends on them beyond the order of its sums. work (pcx_key_weights_workspace's bytes, less splits less; it may be attention's, whose
  * counters it leaves alone) holds the parts' sums. */
 typedef struct KeyWeightsArgs {

@@ -499,14 +499,14 @@ __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArg
     const auto load_k = [&](int t, const Runs<NL, NW, CPR>& r) {
         if (t < first) return;
         if constexpr (PAGED)
-            r.template load<KT, NW * 1024>(P, kp, (int)A.k.token, A.dim, w.len, t, wave, base + (t & 1) * TB, ko);
+            r.template load<KT, NW * 1024>(P, kp, (uint32_t)A.k.token * 2, A.dim, w.len, t, wave, base + (t & 1) * TB, ko);
         else
             load(kp, A.k.token, t, base + (t & 1) * TB, ko);
     };
     const auto load_v = [&](int t, const Runs<NL, NW, CPR>& r) {
         if (t < first) return;
         if constexpr (PAGED)
-            r.template load<KT, NW * 1024>(P, vp, (int)A.v.token, A.dim, w.len, t, wave, base + (2 + (t & 1)) * TB, vo);
+            r.template load<KT, NW * 1024>(P, vp, (uint32_t)A.v.token * 2, A.dim, w.len, t, wave, base + (2 + (t & 1)) * TB, vo);
         else
             load(vp, A.v.token, t, base + (2 + (t & 1)) * TB, vo);
     };
@@ -694,13 +694,13 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     page_t* const table = PAGED ? (page_t*)uniform64((uint64_t)(P.table + w.seq * P.seq)) : nullptr;
     const auto load_k = [&](int t) {
         if constexpr (PAGED)
-            pages.template load<KT, 1024>(P, kp, (int)A.k.token, A.dim, w.len, t, 0, base, ko);
+            pages.template load<KT, 1024>(P, kp, (uint32_t)A.k.token * 2, A.dim, w.len, t, 0, base, ko);
         else
             load(kp, A.k.token, t, base, ko);
     };
     const auto load_v = [&](int t) {
         if constexpr (PAGED) {
-            pages.template load<KT, 1024>(P, vp, (int)A.v.token, A.dim, w.len, t, 0, base + TB, vo);
+            pages.template load<KT, 1024>(P, vp, (uint32_t)A.v.token * 2, A.dim, w.len, t, 0, base + TB, vo);
             if (t >= first + NW) pages.template fetch<KT>(P, table, t - NW, 0);
         } else {
             load(vp, A.v.token, t, base + TB, vo);

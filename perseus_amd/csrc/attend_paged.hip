@@ -9,7 +9,8 @@ static int checked_paged(const AttentionPagedArgs* given, AttentionArgs* a, Page
     if (!given) return -1;
     if (int e = checked(&given->attention, a, true)) return e;
     if (given->cache.start) return -1;
-    return pages_of(given->cache, a->seqs, a->kv_rows, p);
+    if (int e = pages_of(given->cache, a->seqs, a->kv_rows, p)) return e;
+    return (a->k.token << p->log) > PAGE_MAX || (a->v.token << p->log) > PAGE_MAX ? -2 : 0;
 }
 
 extern "C" uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args) {

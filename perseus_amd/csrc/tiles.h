@@ -135,6 +135,7 @@ __device__ __forceinline__ void settled() { __builtin_amdgcn_s_waitcnt(0x0f70); 
 // a tile ahead, so that no tile waits for its table. A run past the sequence's end, or on a page that the pool does not have, is
 // an empty buffer: it reads as zeros.
 constexpr int RUN = 16;
+constexpr int64_t PAGE_MAX = 0x7fffffff;  // elements from a page to the next
 typedef const int32_t __attribute__((address_space(4))) page_t;
 
 template <int NL, int NW, int CPR>
@@ -146,26 +147,30 @@ struct Runs {
     int page[E];
     // the tile's run that the wave's loads e N .. e N + N - 1 take
     static __device__ __forceinline__ int run(int e, int wave) { return (e * N * NW + wave) * PER / RUN; }
+    // page numbers; a tile begins at a page or lies in one
     template <int KT>
     __device__ __forceinline__ void fetch(const PagesRef& P, page_t* table, int t, int wave) {
+        const uint32_t first = ((uint32_t)t * KT) >> P.log;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t row = (uint32_t)t * KT + run(e, wave) * RUN;
-            page[e] = table[min(row >> P.log, (uint32_t)P.width - 1)];
-        }
+        for (int e = 0; e < E; ++e) page[e] = table[min(first + ((uint32_t)(run(e, wave) * RUN) >> P.log), (uint32_t)P.width - 1)];
     }
+    // The scalar unit's instructions are in the way of the wave's others, so they are few for each run: what the tile alone decides
+    // is made once (6 chunks of up to 512 queries over up to 6000 keys 169 -> FIGURE us). token: a row's distance in bytes; a page's
+    // bytes stay in 32 bits.
     template <int KT, int STEP>
-    __device__ __forceinline__ void load(const PagesRef& P, const char* base, int token, int dim, int len, int t, int wave,
+    __device__ __forceinline__ void load(const PagesRef& P, const char* base, uint32_t token, int dim, int len, int t, int wave,
                                          uint32_t lds, const uint32_t (&off)[NL]) const {
+        const uint32_t row = (uint32_t)t * KT, mask = (1u << P.log) - 1, step = token << P.log;
+        const int left = min(len - (int)row, KT), last = (left - 1) * (int)token + dim * 2, full = (RUN - 1) * (int)token + dim * 2;
+        const char* const tile = base + (row & mask) * token;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const uint32_t row = (uint32_t)t * KT + run(e, wave) * RUN;
-            const int left = (int)((uint32_t)len - row), nr = left < RUN ? left : RUN;
-            const bool there = (uint32_t)page[e] < (uint32_t)P.count && nr > 0;
-            const int64_t at = ((int64_t)(there ? page[e] : 0) << P.log) + (row & ((1u << P.log) - 1));
-            int bytes = there ? ((nr - 1) * token + dim) * 2 : 0;
-            asm("" : "+s"(bytes));  // a select, where the compiler would make a branch around each run
-            const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + at * token * 2), 0, bytes, 0x00020000);
+            const uint32_t at = run(e, wave) * RUN;
+            const bool there = (uint32_t)page[e] < (uint32_t)P.count;
+            int bytes = there ? max(min(last - (int)(at * token), full), 0) : 0;
+            uint32_t id = there ? page[e] : 0;
+            asm("" : "+s"(bytes), "+s"(id));  // selects, where the compiler would make a branch around each run
+            const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(tile + (uint64_t)id * step + (at & mask) * token), 0, bytes, 0x00020000);
             uint32_t own[N];
 #pragma unroll
             for (int n = 0; n < N; ++n) own[n] = off[e * N + n];

@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
             Runs<NL, 1, CPR> pages;
             const auto load = [&](int t, int buf) __attribute__((always_inline)) {
                 if constexpr (PAGED) {
-                    pages.template load<KT, 1024>(A.pages, kp, (int)A.k.token, A.dim, S.len, t, 0, base + buf * TB, off);
+                    pages.template load<KT, 1024>(A.pages, kp, (uint32_t)A.k.token * 2, A.dim, S.len, t, 0, base + buf * TB, off);
                 } else {
                     const int left = S.len - t * KT, nr = (left < KT ? left : KT) - 1;
                     const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(kp + (int64_t)t * KT * A.k.token * 2), 0,
@@ -552,7 +552,7 @@ static int checked(const KeyWeightsArgs* a, Weigh* w) {
     w->qt = BR / w->hb;
     w->blocks = (w->group + BR - 1) / BR;
     // a tile's offsets: below 2^30 bytes
-    if (w->k.token > 1 << 22 || w->q.token > (1 << 28) / w->qt || w->q.head > (1 << 28) / w->hb) return -2;
+    if (w->k.token > 1 << 22 || (!w->k_start && (w->k.token << w->pages.log) > PAGE_MAX) || w->q.token > (1 << 28) / w->qt || w->q.head > (1 << 28) / w->hb) return -2;
     return 0;
 }
 
