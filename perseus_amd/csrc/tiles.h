@@ -155,8 +155,11 @@ struct Runs {
         for (int e = 0; e < E; ++e) page[e] = table[min(first + ((uint32_t)(run(e, wave) * RUN) >> P.log), (uint32_t)P.width - 1)];
     }
     // The scalar unit's instructions are in the way of the wave's others, so they are few for each run: what the tile alone decides
-    // is made once (6 chunks of up to 512 queries over up to 6000 keys 169 -> FIGURE us). token: a row's distance in bytes; a page's
-    // bytes stay in 32 bits.
+    // is made once (6 chunks of up to 512 queries over up to 6000 keys 169 -> 156 us; over one run of rows 128, the same for pages of
+    // 16 to 1024 rows in any order). Nearer to it came neither one buffer for a tile of one page (165), nor one for the whole pool with a
+    // run as the scalar offset (33% behind), nor page numbers through LDS (157): what is left is not the number of these instructions
+    // but the scalar registers, whose spilling takes vector registers that the products' addresses had. token: a row's distance in
+    // bytes; a page's bytes stay in 32 bits.
     template <int KT, int STEP>
     __device__ __forceinline__ void load(const PagesRef& P, const char* base, uint32_t token, int dim, int len, int t, int wave,
                                          uint32_t lds, const uint32_t (&off)[NL]) const {
