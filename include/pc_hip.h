@@ -1228,8 +1228,8 @@ uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args); /* as pc
  * place after the sequence's last token). Rows of no sequence are left as they were; sequences may not share rows. Sums are f32 and have one order.
  *
  * weights, before: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). Keys on a page outside the pool have
- * no row. Types, dim, scale and alignment as pcx_attention's; a query's row and head strides below 2^22 elements, page_rows
- * times a key row's below 2^31; seqs and kv_heads below 65536; decay >= 0 and finite. max_q and max_k are the longest runs expected: they choose the split of the rows, no result
+ * no row. Types, dim, scale and alignment as pcx_attention's; a query's row and head strides up to 2^21 elements, a key
+ * row's up to 2^22, page_rows times it below 2^31; seqs and kv_heads below 65536; decay >= 0 and finite. max_q and max_k are the longest runs expected: they choose the split of the rows, no result
  * depends on them beyond the order of its sums. work (pcx_key_weights_workspace's bytes, less splits less; it may be attention's, whose
  * counters it leaves alone) holds the parts' sums. */
 typedef struct KeyWeightsArgs {

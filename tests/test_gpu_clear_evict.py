@@ -112,6 +112,15 @@ def test_evict_of_long_caches(ops, lens, page):
     run_evict(ops, lens, 2, 60000, 500, 4, page, spread, max_k=100)
 
 
+@pytest.mark.parametrize("page", [0, 16])
+def test_evict_of_short_runs_beside_long_ones(ops, page):
+    """slices of no key, of one key, and sequences that keep all, where the longest is shared out to many workgroups"""
+    say(f"[clear] evict of lengths from 0 to 20000 together, pages of {page}")
+    for keep in (1, 2, 3, 15, 16, 17, 100):
+        run_evict(ops, [20000, keep + 1, keep, 0, keep + 2, 2 * keep + 31, 2000], 3, keep, 0, 0, page, spread)
+    run_evict(ops, [16385, 5000], 2, 4999, 40, 4, page, spread)
+
+
 @pytest.mark.parametrize("what", ["alike", "few", "zeros", "signs", "bits"])
 @pytest.mark.parametrize("n,keep", [(900, 300), (20000, 15000), (130, 65)])
 def test_evict_of_ties_and_strange_weights(ops, what, n, keep):
@@ -257,3 +266,39 @@ def test_evict_and_moves_far_into_a_pool(ops):
             k[d, g] = k[s, g]
     got = buf.download(stream=ops.stream, offset=first * kv * dim // 2).view(np.uint16)
     assert (clear.from_bf16(got).reshape(k.shape) == k).all()
+
+
+def test_evict_of_long_caches_replays_as_a_graph(ops):
+    """the launches of a long cache's choice captured once: replays with eager calls between them equal the eager lists"""
+    say("[clear] evict of 30000 keys as a graph, 3 replays")
+    st, n, kv, keep = ops.stream, 30000, 2, 9000
+    rng = np.random.default_rng(7)
+    w = [spread(rng, n * kv).reshape(kv, n).astype(np.float32) for _ in range(3)]
+    dw, k0, dn = pa.Array((n, kv), "f32", strides=(1, n)), pa.Array.of(np.zeros(1, np.int64)), pa.Array((1,), "i32")
+    moves, count = pa.Array((1, kv, keep, 2), "i32"), pa.Array((1, kv), "i32")
+
+    def load(i):
+        dw.buf.upload(w[i].reshape(-1).view(np.uint32), st)
+        dn.buf.upload(np.array([n - 37 * i], np.uint32), st)
+        moves.buf.upload(np.zeros(moves.buf.words, np.uint32), st)
+
+    def step():
+        ops.evict(dw, dn, keep, moves, count, k_start=k0, recent=50, first=4)
+
+    eager = []
+    for i in range(3):
+        load(i)
+        step()
+        eager.append((moves.numpy(st), count.numpy(st)))
+        for g in range(kv):
+            mv = co.kept(w[i][g, :n - 37 * i], np.arange(n - 37 * i), n - 37 * i, keep, 50, 4)[1]
+            assert (eager[i][0][0, g, :len(mv)] == np.array(mv)).all() and eager[i][1][0, g] == len(mv)
+    load(0)
+    graph = pa.Graph(st, step)
+    for i in range(3):
+        load((i + 1) % 3)
+        step()
+        st.sync()
+        load(i)
+        graph.launch(st)
+        assert (moves.numpy(st) == eager[i][0]).all() and (count.numpy(st) == eager[i][1]).all()

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import perseus_amd as pa
+from perseus_amd import clear
 from tests import clear_oracle as co
 from tests.test_gpu_clear import placed
 from tests.test_gpu_clear_evict import per_key
@@ -203,6 +204,51 @@ def test_key_weights_many_sequences(ops):
     spans = [(int(rng.integers(0, 4)), int(rng.integers(0, 50))) for _ in range(300)]
     run_weights(ops, "bf16", 64, 2, 1, spans, True, 16, new=True)
     run_weights(ops, "f16", 64, 2, 2, [(5 * n, 2 * m) for n, m in spans[:130]], True, 0)
+
+
+def test_key_weights_of_many_key_heads(ops):
+    """more key heads than waves take at once"""
+    say("[clear] key_weights of 5000 key heads")
+    run_weights(ops, "f16", 8, 5000, 5000, [(1, 40), (2, 9)], True, 16, new=True)
+    run_weights(ops, "bf16", 8, 600, 300, [(40, 50), (0, 3)], True, 0)
+
+
+def test_key_weights_replay_as_a_graph(ops):
+    """rows split and joined, and a token's, captured: replays with eager calls between them equal the eager sums"""
+    say("[clear] key_weights as a graph, 3 replays")
+    st, H, KV, D, n = ops.stream, 8, 2, 64, 700
+    rng = np.random.default_rng(2)
+    q, k = pa.Array((n, H, D), "bf16"), pa.Array((n, KV, D), "bf16")
+    lse, w, q0 = pa.Array((n, H), "f32"), pa.Array((n, KV), "f32", strides=(1, n)), pa.Array((2,), "i32")
+    k0, kl = pa.Array.of(np.zeros(1, np.int64)), pa.Array((1,), "i32")
+    cases = [(rng.normal(size=(n, H, D)), rng.normal(size=(n, KV, D)), rng.random((n, H)) + 6, m) for m in (700, 500, 123)]
+
+    def load(c):
+        for x, y in ((q, c[0]), (k, c[1])):
+            x.buf.upload(clear.to_bf16(y).view(np.uint32), st)
+        lse.buf.upload(c[2].astype(np.float32).view(np.uint32), st)
+        w.buf.upload(np.zeros(w.buf.words, np.uint32), st)
+        q0.buf.upload(np.array([0, c[3]], np.uint32), st)
+        kl.buf.upload(np.array([c[3]], np.uint32), st)
+
+    def step():
+        ops.key_weights(q, k, lse, q0, kl, w, k_start=k0, before=w, max_q=n, max_k=n)
+        ops.key_weights(q, k, lse, q0, kl, w, k_start=k0, before=w, decay=0.5, max_q=1, max_k=n)
+
+    eager = []
+    for c in cases:
+        load(c)
+        step()
+        eager.append(w.numpy(st))
+    load(cases[0])
+    graph = pa.Graph(st, step)
+    for i, c in enumerate(cases):
+        load(cases[(i + 1) % 3])
+        step()
+        st.sync()
+        load(c)
+        graph.launch(st)
+        assert (w.numpy(st) == eager[i]).all(), i
 
 
 def test_key_weights_cuts_and_bad_pages(ops):
