@@ -4,6 +4,7 @@
 // of two alike. The kept rows behind `keep` go to the gaps before it, both in rising order: as few moves as there are gaps, and
 // none of them reads what another writes, so that they all run at once, in place.
 #include <algorithm>
+#include <type_traits>
 
 #include "tiles.h"
 
@@ -23,7 +24,7 @@ struct Rows {
             room = at < 0 || at >= rows ? 0 : rows - at;
         } else {
             at = (int64_t)b * p.seq;
-            room = (int64_t)p.width << p.log;
+            room = p.count ? (int64_t)p.width << p.log : 0;  // an empty pool has no rows
         }
         if (*len < 0) *len = 0;
         if (*len > room) *len = (int)room;
@@ -47,7 +48,9 @@ static int rows_of(const CacheRef& c, int64_t seqs, int64_t rows, Rows* r) {
 // words with the digits found so far are counted by their next one, 11 bits, in 2048 bins in LDS, until the bin that the last kept
 // word is in is kept whole or holds few enough to rank each against all. Weights spread over orders of magnitude take one digit.
 //
-// What bounds it are latencies: the loads of weights, places and pages, the counting's atomics, the barriers between.
+// What bounds it are latencies: the loads of pages, weights and places, the counting's atomics, the barriers between. 528 keys x 12
+// heads 5.7 us; 48 caches of 4160 keys x 8 heads 18; 65536 keys x 8 heads 31 in three launches. Three digits of every word in place of
+// one and a ranking: 12, 32 and 168.
 constexpr int WAVES = 16, THREADS = 64 * WAVES, BINS = 2048, RANKED = 1024;
 constexpr int SLICES = 16, GATHERED = 8192, LONG = 16384;
 
@@ -136,7 +139,7 @@ __device__ __forceinline__ uint64_t select(Shared& S, uint32_t need, Each each) 
 
 // the words of a (sequence, key head)'s keys, E in the registers of each lane: a wave's lanes hold runs of 64 keys, its runs one
 // after the other
-template <int E>
+template <int E, bool SMALL>
 struct Words {
     const Choice& A;
     const int g, len;
@@ -148,24 +151,41 @@ struct Words {
     __device__ __forceinline__ Words(const Choice& a, int g, int b, int len, int64_t at)
         : A(a), g(g), len(len), at(at), next(a.next_place ? a.next_place[b] : len), from(0), seg(0) {}
     __device__ __forceinline__ int first() const { return from + (int)(threadIdx.x >> 6) * seg + (int)(threadIdx.x & 63); }
-    // the chunk of keys lo .. hi - 1, E loads of each kind on their way at once
+    // The chunk of keys lo .. hi - 1, E loads of each kind on their way at once; those past the end read the last key again (loads under
+    // a condition each: 48 caches of 4160 keys 25.6 us, so 23.7). SMALL: rows and their offsets in 32 bits.
     __device__ __forceinline__ void load(int lo, int hi) {
-        const float* const w = (const float*)A.weights.base + g * A.weights.head;
-        const int32_t* const places = A.places.base ? (const int32_t*)A.places.base + g * A.places.head : nullptr;
+        typedef typename std::conditional<SMALL, uint32_t, int64_t>::type index;
+        const char* const w = (const char*)A.weights.base + g * A.weights.head * 4;
+        const char* const places = A.places.base ? (const char*)A.places.base + g * A.places.head * 4 : nullptr;
+        const index w_row = (index)A.weights.token * 4, p_row = (index)A.places.token * 4;
+        const bool paged = !A.cache.start;
+        const int32_t* const table = A.cache.p.table + (paged ? at : 0);
+        const uint32_t low = (1u << A.cache.p.log) - 1;
         from = lo;
         seg = 64 * ((hi - lo + THREADS - 1) / THREADS);
-        int64_t row[E];
+        if (lo >= hi) return;  // a slice of no key: there is no last one to read again
+        int page[E], place[E];
         float x[E];
-        int place[E];
+        const auto key_of = [&](int e) { return (uint32_t)std::min(first() + e * 64, hi - 1); };
+        if (paged)
 #pragma unroll
-        for (int e = 0; e < E; ++e) row[e] = e * 64 < seg && first() + e * 64 < hi ? A.cache.row(at, first() + e * 64) : -1;
+            for (int e = 0; e < E; ++e) page[e] = table[key_of(e) >> A.cache.p.log];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            x[e] = row[e] < 0 ? 0 : w[row[e] * A.weights.token];
-            place[e] = row[e] < 0 ? 0 : places ? places[row[e] * A.places.token] : first() + e * 64;
+            const uint32_t j = key_of(e);
+            index row = (index)at + j;
+            if (paged) {
+                page[e] = (uint32_t)page[e] < (uint32_t)A.cache.p.count ? page[e] : -1;
+                row = ((index)(page[e] < 0 ? 0 : page[e]) << A.cache.p.log) + (j & low);
+            }
+            x[e] = *(const float*)(w + row * w_row);
+            if (places) place[e] = *(const int32_t*)(places + row * p_row);
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) key[e] = row[e] < 0 ? 0 : place[e] >= next - A.recent || place[e] < A.first ? PROTECTED : ordered(x[e]);
+        for (int e = 0; e < E; ++e) {
+            const int64_t p = places ? place[e] : (int)key_of(e);
+            key[e] = paged && page[e] < 0 ? 0 : p >= next - A.recent || p < A.first ? PROTECTED : ordered(x[e]);
+        }
     }
     // f(e, j, word, whether there is one) in the order of e
     template <class F>
@@ -219,7 +239,7 @@ struct Words {
 };
 
 // a workgroup for each (sequence, key head)
-template <int E>
+template <int E, bool SMALL>
 __global__ void __launch_bounds__(THREADS, E > 8 ? 4 : 8) evict_k(Choice A) {
     __shared__ Shared S;
     const int g = blockIdx.x, kv = gridDim.x;
@@ -229,7 +249,7 @@ __global__ void __launch_bounds__(THREADS, E > 8 ? 4 : 8) evict_k(Choice A) {
         if (A.kept_len && g == 0 && threadIdx.x == 0) A.kept_len[b] = len < A.keep ? len : A.keep;
         uint32_t movers = 0, holes = 0;
         if (len > A.keep && A.keep) {
-            Words<E> W(A, g, b, len, at);
+            Words<E, SMALL> W(A, g, b, len, at);
             const bool once = len <= W.CHUNK;
             if (once) W.load(0, len);
             const uint64_t least = select(S, A.keep, [&](auto f) { W.all(0, len, once, f); });
@@ -262,7 +282,7 @@ __device__ __forceinline__ Slice slice_of(int s, int len, int keep) {
     return {keep + cut(n, s - left, of), keep + cut(n, s - left + 1, of), left};
 }
 
-template <int STAGE>
+template <int STAGE, bool SMALL>
 __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
     __shared__ Shared S;
     constexpr int E = 8;
@@ -276,7 +296,7 @@ __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
     }
     Pair& P = ((Pair*)A.work)[pair];
     const Slice mine = slice_of(s, len, A.keep);
-    Words<E> W(A, g, b, len, at);
+    Words<E, SMALL> W(A, g, b, len, at);
     const bool once = mine.hi - mine.lo <= W.CHUNK;
     if (once) W.load(mine.lo, mine.hi);
     if constexpr (STAGE == 0) {
@@ -390,7 +410,9 @@ struct Moves {
     }
 };
 
-// A power of two of lanes takes a move, 16 bytes of a row each where addresses allow: the loads of all tensors, then the stores.
+// A power of two of lanes takes a move, 16 bytes of a row each where addresses allow: the loads of all tensors, then the stores. It
+// is bound by the memory, rows of one head a few hundred bytes each, out of order: 12480 moves x 8 heads of keys and values of 256
+// bytes, weights and places, 104 MB: 23.5 us, 4.4 TB/s (a large copy: 5.6).
 __global__ void __launch_bounds__(256) move_k(Moves A) {
     const int g = blockIdx.y, kv = gridDim.y, l = threadIdx.x & ((1 << A.lanes_log) - 1), each = 256 >> A.lanes_log;
     for (int b = blockIdx.z; b < A.seqs; b += gridDim.z) {
@@ -424,7 +446,30 @@ __global__ void __launch_bounds__(256) move_k(Moves A) {
 using namespace pch;
 using namespace pch::clear;
 
-// Few pairs of long runs: their workgroups alone do not fill the chip, and one takes long (65536 -> 16384 keys x 8 heads with the moves: a workgroup each 219 us, so 61).
+template <bool SMALL>
+static int run(const Choice& c, int kv_heads, int max_k, bool shared, hipStream_t s) {
+    const dim3 block(THREADS);
+    if (shared) {
+        const dim3 grid(kv_heads, SLICES, c.seqs);
+        hipLaunchKernelGGL((evict_long_k<0, SMALL>), grid, block, 0, s, c);
+        if (int e = launch_rc()) return e;
+        hipLaunchKernelGGL((evict_long_k<1, SMALL>), grid, block, 0, s, c);
+        if (int e = launch_rc()) return e;
+        hipLaunchKernelGGL((evict_long_k<2, SMALL>), grid, block, 0, s, c);
+        return launch_rc();
+    }
+    const dim3 grid(kv_heads, std::min(c.seqs, 65535));
+    // 5 words a lane take 64 registers, so that two workgroups share a CU (48 caches of 4160 keys x 8 heads, a word's registers not
+    // bounded: 32.4 us, so 25.6); of longer runs 16, read again for each digit past 16384
+    if (max_k <= 5 * THREADS)
+        hipLaunchKernelGGL((evict_k<5, SMALL>), grid, block, 0, s, c);
+    else
+        hipLaunchKernelGGL((evict_k<16, SMALL>), grid, block, 0, s, c);
+    return launch_rc();
+}
+
+// Few pairs of long runs: their workgroups alone do not fill the chip, and one takes long (65536 -> 16384 keys x 8 heads with the
+// moves: a workgroup each 219 us, so 61).
 static bool is_long(const EvictArgs& a) { return a.max_k > LONG && (int64_t)a.seqs * a.kv_heads < 256; }
 static uint64_t work_bytes(const EvictArgs& a) { return PCX_ATTENTION_COUNTERS * 4 + (uint64_t)a.seqs * a.kv_heads * sizeof(Pair); }
 
@@ -446,23 +491,11 @@ extern "C" int pcx_evict(const EvictArgs* a, pc_stream_t s) {
     c.k_len = a->k_len, c.next_place = a->next_place;
     c.moves = a->moves, c.count = a->count, c.kept_len = a->kept_len;
     c.seqs = a->seqs, c.keep = a->keep, c.recent = a->recent, c.first = a->first, c.most = a->most;
-    const hipStream_t st = (hipStream_t)s;
-    if (is_long(*a) && a->work && a->work_bytes >= work_bytes(*a)) {
-        c.work = (char*)a->work + PCX_ATTENTION_COUNTERS * 4;
-        const dim3 grid(a->kv_heads, SLICES, a->seqs), block(THREADS);
-        hipLaunchKernelGGL((evict_long_k<0>), grid, block, 0, st, c);
-        if (int e = launch_rc()) return e;
-        hipLaunchKernelGGL((evict_long_k<1>), grid, block, 0, st, c);
-        if (int e = launch_rc()) return e;
-        hipLaunchKernelGGL((evict_long_k<2>), grid, block, 0, st, c);
-        return launch_rc();
-    }
-    const dim3 grid(a->kv_heads, std::min(a->seqs, 65535)), block(THREADS);
-    if (a->max_k <= 8 * THREADS)
-        hipLaunchKernelGGL((evict_k<8>), grid, block, 0, st, c);
-    else
-        hipLaunchKernelGGL((evict_k<16>), grid, block, 0, st, c);
-    return launch_rc();
+    // offsets of 4-byte elements in 32 bits
+    const bool small = a->rows < 0x3fffffff / std::max<int64_t>({1, c.weights.token, c.places.base ? c.places.token : 0});
+    const bool shared = is_long(*a) && a->work && a->work_bytes >= work_bytes(*a);
+    c.work = (char*)a->work + PCX_ATTENTION_COUNTERS * 4;
+    return small ? run<true>(c, a->kv_heads, a->max_k, shared, (hipStream_t)s) : run<false>(c, a->kv_heads, a->max_k, shared, (hipStream_t)s);
 }
 
 extern "C" int pcx_move_rows(const MoveRowsArgs* a, pc_stream_t s) {
