@@ -459,9 +459,12 @@ static int run(const Choice& c, int kv_heads, int max_k, bool shared, hipStream_
         return launch_rc();
     }
     const dim3 grid(kv_heads, std::min(c.seqs, 65535));
-    // 5 words a lane take 64 registers, so that two workgroups share a CU (48 caches of 4160 keys x 8 heads, a word's registers not
-    // bounded: 32.4 us, so 25.6); of longer runs 16, read again for each digit past 16384
-    if (max_k <= 5 * THREADS)
+    // A word a lane where that is all (528 keys x 12 heads, five: 6.6 us, so 5.7). 5 take 64 registers, so that two workgroups share a
+    // CU (48 caches of 4160 keys x 8 heads, registers not bounded: 32.4 us, so 25.6); of longer runs 16, read again for each digit
+    // past 16384.
+    if (max_k <= THREADS)
+        hipLaunchKernelGGL((evict_k<1, SMALL>), grid, block, 0, s, c);
+    else if (max_k <= 5 * THREADS)
         hipLaunchKernelGGL((evict_k<5, SMALL>), grid, block, 0, s, c);
     else
         hipLaunchKernelGGL((evict_k<16, SMALL>), grid, block, 0, s, c);
