@@ -121,8 +121,9 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
     if (part >= np || (int64_t)slot * BK >= S.len) return;
     const float c2 = A.scale * 1.4426950408889634f;
     const int tiles = (int)(((uint32_t)S.n + A.qt - 1) / A.qt) * A.blocks;
-    // this lane's rows of a tile's loads (BR: none), and where they lie from the tile's first
-    uint32_t off[NL];
+    // This lane's rows of a tile's loads (BR: none), and where they lie from the tile's first. In place of rows that the tile does not
+    // have it takes the first again: of zeros, an infinity in a key would make a NaN where all rows' scores of it are -infinity.
+    uint32_t off[NL], first[NL];
     int row_of[NL];
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
@@ -130,6 +131,7 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
         const int ch = (p % CPR) ^ Tile<DP>::kswz(x);
         row_of[n] = ch * 8 < A.dim && qi < A.qt ? x : BR;
         off[n] = ((uint32_t)qi * (uint32_t)A.q.token + (uint32_t)hd * (uint32_t)A.q.head) * 2 + ch * 16;
+        first[n] = ch * 8 < A.dim ? ch * 16 : 0x7ffffff0u;  // past the dimensions: zeros
     }
     const int x0 = threadIdx.x, xq = A.query(x0), xh = x0 - xq * A.hb;  // the row whose log-sum-exp this lane of the first waves brings
     const uint32_t to = (uint32_t)(uintptr_t)(char PCH_LDS*)lds + wave * 1024;
@@ -150,7 +152,7 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
         const char* p = (const char*)(q + (int64_t)r.i * A.q.token + (int64_t)r.hd * A.q.head);
         uint32_t own[NL];
 #pragma unroll
-        for (int n = 0; n < NL; ++n) own[n] = row_of[n] < r.x ? off[n] : 0x7ffffff0u;  // zeros
+        for (int n = 0; n < NL; ++n) own[n] = row_of[n] < r.x ? off[n] : first[n];
         load_lds<NW * 1024>(__builtin_amdgcn_make_buffer_rsrc((void*)uniform64((uint64_t)p), 0, 0x40000000, 0x00020000), to + buf * TB, own);
     };
     const auto ask = [&](int t) {
@@ -421,10 +423,12 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
                 v8 q[STEPS];
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) q[s] = (v8)(T)0.0f;
-                if (c < R) {
+                if (R > 0) {  // (rows past the last are the first again: of zeros, an infinity in a key would make a NaN)
                     const T* x = at<T>(A.q, S.q0 + (int64_t)i, head);
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s) q[s] = *(const v8*)(x + std::min(16 * s + 8 * h, A.dim - 8));
+                }
+                if (c < R) {
                     const float x2 = A.lse[(S.q0 + (int64_t)i) * A.heads + head];
                     nl[c] = x2 == -INFINITY ? x2 : x2 * -1.4426950408889634f;  // a row that sees no key adds nothing
                     const int64_t sees = A.causal ? (int64_t)S.len - S.n + i + 1 : S.len;

@@ -136,5 +136,6 @@ def key_weights(q, k, lse, spans, group, scale, causal):
                 p = np.where(sees & (L > -np.inf) | sees & np.isnan(L), np.exp(z - L), 0)
                 d = (D + 4) * E * dz + 8 * E * (np.abs(z) + np.where(np.isfinite(L), np.abs(L), 0)) + 8 * E
                 out[k0:k0 + m, g] += p.sum(0)
+                d = np.where(p == 0, 0, d)  # at scores of -infinity d is infinite, the weight 0
                 bound[k0:k0 + m, g] += (p * d).sum(0) + (n * group / 16 + 32) * E * p.sum(0)
     return out, bound

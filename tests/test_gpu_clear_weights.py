@@ -302,3 +302,21 @@ def test_the_weights_of_a_call_sum_to_its_heads(ops):
     got = w.numpy(ops.stream)
     for b, r in enumerate(rows):
         assert np.allclose(got[r].sum(0, dtype=np.float64), new[b] * H // KV, rtol=2e-5)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+def test_key_weights_of_keys_at_minus_infinity(ops, dim, causal):
+    """keys that every query scores -infinity weigh what they did: rows that a tile has room for but the call has none of make no
+    NaN of them (heads of a group that fill no tile, one token, odd prompts)"""
+    say(f"[clear] key_weights, keys at -infinity, {dim} dimensions, causal {causal}")
+
+    def edit(q, k, k0):
+        q[:, :, dim - 3] = co.rounded(np.abs(q[:, :, dim - 3]) + 1, "f16")  # what the device gets
+        for b, j in ((0, 7), (0, 290), (1, 3), (1, 64), (2, 5)):
+            k[k0[b] + j, :, dim - 3] = -np.inf
+
+    for heads, kv, spans in ((4, 2, [(1, 300), (3, 70), (2, 9)]), (6, 2, [(131, 300), (50, 70), (9, 9)]), (7, 1, [(40, 700), (33, 80), (1, 9)])):
+        for page in (0, 16):
+            got = run_weights(ops, "f16", dim, heads, kv, spans, causal, page, edit=edit)
+            assert not np.isnan(got).any()
