@@ -571,6 +571,7 @@ static void choose(Weigh* w, int max_q, uint64_t room) {
     w->slots = (int)std::min(keys, most);
     const int64_t base = (int64_t)w->slots * w->seqs * w->kv_heads;
     w->parts = (int)std::max<int64_t>({1, std::min<int64_t>(512 / base, tiles), std::min<int64_t>(2048 / base, tiles / 4)});
+    if (!w->max_k) w->parts = 1;  // no key is expected: there is nothing to join, and longer runs than expected are not split
     while (w->parts > 1 && (bytes_of(*w, w->parts) > room || w->slots * w->parts > 65535)) w->parts /= 2;
 }
 

@@ -212,6 +212,8 @@ def test_key_weights_s_workspace():
     a = weights_args(tokens=8192, seqs=1, max_q=8192, max_k=4096, kv_rows=8192, work=3, work_bytes=1)
     n = LIB.pcx_key_weights_workspace(C.byref(a))
     assert n > 4 * 4096 and (n - 4 * 4096) % (2 * 4096 * 4) == 0
+    # where no key is expected there is nothing to split
+    assert LIB.pcx_key_weights_workspace(C.byref(weights_args(tokens=8192, seqs=1, max_q=8192, max_k=0, kv_rows=8192))) == 0
 
 
 def test_key_weights_shapes_are_refused(ops):

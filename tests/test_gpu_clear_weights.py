@@ -304,6 +304,14 @@ def test_the_weights_of_a_call_sum_to_its_heads(ops):
         assert np.allclose(got[r].sum(0, dtype=np.float64), new[b] * H // KV, rtol=2e-5)
 
 
+@pytest.mark.parametrize("page_rows", [0, 16])
+def test_key_weights_of_prompts_where_no_key_is_expected(ops, page_rows):
+    """max_q of a prompt beside max_k 0, longer runs than that and none"""
+    say(f"[clear] key_weights, prompts with max_k 0, pages of {page_rows}")
+    run_weights(ops, "bf16", 64, 4, 2, [(300, 700), (40, 40)], True, page_rows, hints=(4096, 0))
+    run_weights(ops, "bf16", 64, 4, 2, [(300, 0), (40, 0)], True, page_rows, hints=(4096, 0))
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("dim", [64, 80, 128, 256])
 def test_key_weights_of_keys_at_minus_infinity(ops, dim, causal):
