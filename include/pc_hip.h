@@ -16,7 +16,9 @@
  *
  * Beside them, the clear side of an encrypted transformer block (pcx_rotary, pcx_qk_norm_rotary, pcx_attention): the
  * operators that make the plaintext queries and the keys an encrypted scoring starts from, and the attention in the
- * clear that its decrypted scores are held against. They take no context.
+ * clear that its decrypted scores are held against; and a cache of keys in pages (pcx_attention_paged), whose keys are cut
+ * to as many as such a scoring holds by the weight they gather (pcx_key_weights, pcx_evict, pcx_move_rows). They take no
+ * context.
  */
 #ifndef PC_HIP_H
 #define PC_HIP_H
@@ -1225,13 +1227,15 @@ uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args); /* as pc
  * [tokens][heads]); a query of -infinity, which sees no key, adds nothing. before (base NULL, or decay 0: not read, 0) may be
  * weights itself. next_place (NULL: none): the last n_b keys of each sequence are its n_b queries' own and new: before is not
  * read for them, and where places (base NULL: none) is given, theirs become next_place[b] - len + j (next_place[b]: the
- * place after the sequence's last token). Rows of no sequence are left as they were; sequences may not share rows. Sums are f32 and have one order.
+ * place after the sequence's last token). Rows of no sequence are left as they were; sequences may not share rows. Sums are f32
+ * and have one order.
  *
  * weights, before: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). Keys on a page outside the pool have
  * no row. Types, dim, scale and alignment as pcx_attention's; a query's row and head strides up to 2^21 elements, a key
- * row's up to 2^22, page_rows times it below 2^31; seqs and kv_heads below 65536; decay >= 0 and finite. max_q and max_k are the longest runs expected: they choose the split of the rows, no result
- * depends on them beyond the order of its sums. work (pcx_key_weights_workspace's bytes, less splits less; it may be attention's, whose
- * counters it leaves alone) holds the parts' sums. */
+ * row's up to 2^22, page_rows times it below 2^31; seqs and kv_heads below 65536; decay >= 0 and finite. max_q and max_k are the
+ * longest runs expected: they choose the split of the rows, no result depends on them beyond the order of its sums. work
+ * (pcx_key_weights_workspace's bytes, less splits less; it may be attention's, whose counters it leaves alone) holds the
+ * parts' sums. */
 typedef struct KeyWeightsArgs {
     HeadsRef q, k, weights, before, places;
     CacheRef cache;
@@ -1251,15 +1255,15 @@ PC_STATIC_ASSERT(sizeof(KeyWeightsArgs) == 256, "KeyWeightsArgs layout");
 int pcx_key_weights(const KeyWeightsArgs* args, pc_stream_t s);
 uint64_t pcx_key_weights_workspace(const KeyWeightsArgs* args);
 
-/* Which keys leave a cache. Of sequence b's len = k_len[b] keys each key head keeps the min(keep, len) of largest weight, the lower
- * key of two alike (NaN weighs less than -infinity); before all others those are kept whose place is below `first` or at
- * least next_place[b] - recent (first + recent <= keep; places NULL: key j's place is j; next_place NULL: len). The kept keys j >= keep in rising order
- * are to go where the evicted ones j < keep lie, in rising order: moves[b][g][i] = (from, to), i < count[b][g], for pcx_move_rows.
- * At most `most` are written (count is what there are: at most keep, and at most len - keep); entries past them are left
- * as they were. kept_len (NULL: none; not k_len itself): min(keep, len), what the sequence's length is once its rows have moved.
- * Keys on a page outside the pool are evicted first. max_k: the longest run expected; it only chooses a kernel. work
- * (pcx_evict_workspace's bytes, 0 but for few long runs, which take longer without; 16-byte aligned; it may be attention's, whose
- * counters it leaves alone).
+/* Which keys leave a cache. Of sequence b's len = k_len[b] keys each key head keeps the min(keep, len) of largest weight, the
+ * lower key of two alike (NaN weighs less than -infinity); before all others those are kept whose place is below `first` or at
+ * least next_place[b] - recent (first + recent <= keep; places NULL: key j's place is j; next_place NULL: len). The kept keys
+ * j >= keep in rising order are to go where the evicted ones j < keep lie, in rising order: moves[b][g][i] = (from, to),
+ * i < count[b][g], for pcx_move_rows. At most `most` are written (count is what there are: at most keep, and at most
+ * len - keep); entries past them are left as they were. kept_len (NULL: none; not k_len itself): min(keep, len), what the
+ * sequence's length is once its rows have moved. Keys on a page outside the pool weigh what NaN does, protected or not. max_k:
+ * the longest run expected; it only chooses a kernel. work (pcx_evict_workspace's bytes, 0 but for few long runs, which take
+ * longer without; 16-byte aligned; it may be attention's, whose counters it leaves alone).
  * weights: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). */
 typedef struct EvictArgs {
     HeadsRef weights, places;
@@ -1279,9 +1283,9 @@ int pcx_evict(const EvictArgs* args, pc_stream_t s);
 uint64_t pcx_evict_workspace(const EvictArgs* args);
 
 /* The moves of pcx_evict, in up to four tensors [rows][kv_heads][dim[i]] at once (keys, values, weights, places), elements of
- * size[i] = 2, 4 or 8 bytes: row `to` of sequence b and key head g becomes row `from`, i < min(count[b][g], most). Moves that leave
- * the cache are skipped. Rows that others are moved to may not be moved from (no move of pcx_evict does that). Sequences that
- * share rows do not keep them. */
+ * size[i] = 2, 4 or 8 bytes: row `to` of sequence b and key head g becomes row `from`, i < min(count[b][g], most). Moves that
+ * leave the cache are skipped. Rows that others are moved to may not be moved from (no move of pcx_evict does that), and
+ * sequences may not share rows. */
 typedef struct MoveRowsArgs {
     HeadsRef t[4];
     CacheRef cache;

@@ -1,10 +1,13 @@
 """The clear side of an encrypted transformer block, on the device: rotary positions, the norms of queries and keys with
-the rotation in the same pass, and attention over packed prompts, chunks and single tokens.
+the rotation in the same pass, and attention over packed prompts, chunks and single tokens, over keys packed, in caches or in
+pages; the weight that cached keys gather, and the eviction of those of least weight.
 
 The encrypted scoring (perseus_amd.attention) multiplies plaintext queries into an encrypted cache of keys. `Clear` makes
 those queries and keys from projected rows, and the attention in the clear that the decrypted scores are held against: its
-log-sum-exp turns a score into a probability, exp(score - lse). The kernels are csrc/rotary.hip and csrc/attend.hip behind
-pcx_rotary, pcx_qk_norm_rotary and pcx_attention (include/pc_hip.h), which a C caller uses directly.
+log-sum-exp turns a score into a probability, exp(score - lse). That cache holds a fixed number of keys: `key_weights` sums
+those probabilities for each key, `evict` and `move_rows` cut a longer cache to the keys that gathered most
+(attention.PagedBlock uses them all). The kernels are csrc/rotary.hip, csrc/attend.h (attend.hip, attend_paged.hip),
+csrc/weigh.hip and csrc/evict.hip behind the pcx entries of the same names (include/pc_hip.h), which a C caller uses directly.
 
 Tensors are `Array`s (a DevBuf with a shape and a type) or any device tensor of another library with data_ptr(), shape,
 stride() and dtype; their last dimension is dense, the others may have any stride the entry takes. Everything is enqueued
@@ -446,8 +449,8 @@ class Clear:
         next_place (i32 [sequences], the place after each sequence's last token): the last keys are the queries' own and new,
         they begin at 0, and get their places (i32 [rows][kv heads], if given). Sequences may not share rows. max_q, max_k: the
         longest runs expected; they only choose how rows are split."""
-        args = self._key_weights(q, k, lse, q_start, k_len, weights, k_start, pages, page_rows, before, decay, places, next_place, scale,
-                                 causal, max_q, max_k)
+        args = self._key_weights(q, k, lse, q_start, k_len, weights, k_start, pages, page_rows, before, decay, places, next_place,
+                                 scale, causal, max_q, max_k)
         check(LIB.pcx_key_weights(args, self.stream.h), "key_weights")
 
     def key_weights_args(self, *args, **kw):
@@ -479,12 +482,13 @@ class Clear:
 
     def evict(self, weights, k_len, keep, moves, count, k_start=None, pages=None, page_rows=None, places=None, next_place=None,
               recent=0, first=0, kept_len=None, max_k=None):
-        """Which keys leave: each key head of a sequence keeps the `keep` of its k_len[b] keys with the largest weights (f32 [rows]
-        [kv heads], by any strides), the lower key of two alike; before all others those whose place (i32, as the weights; None:
-        the key's number) is below `first` or at least next_place[b] (i32; None: the length) - recent, `keep` of them at most. moves (i32 [sequences]
-        [kv heads][most][2]) and count (i32 [sequences][kv heads]) get the rows that move_rows moves, kept keys from behind
-        `keep` to the gaps before it; kept_len (i32, or None) the lengths after that. Moves past `most` are not written (there
-        are never more than keep, or than the longest run less keep). max_k: the longest run expected; it only chooses a kernel."""
+        """Which keys leave: each key head of a sequence keeps the `keep` of its k_len[b] keys with the largest weights (f32
+        [rows][kv heads], by any strides), the lower key of two alike; before all others those whose place (i32, as the weights;
+        None: the key's number) is below `first` or at least next_place[b] (i32; None: the length) - recent, `keep` of them at
+        most. moves (i32 [sequences][kv heads][most][2]) and count (i32 [sequences][kv heads]) get the rows that move_rows moves,
+        kept keys from behind `keep` to the gaps before it; kept_len (i32, or None) the lengths after that. Moves past `most` are
+        not written (there are never more than keep, or than the longest run less keep). max_k: the longest run expected; it only
+        chooses a kernel."""
         seqs = k_len.shape[0]
         rows, kv = weights.shape if len(weights.shape) == 2 else (0, 0)
         shape = moves.shape
@@ -506,7 +510,8 @@ class Clear:
 
     def move_rows(self, moves, count, tensors, k_start=None, pages=None, page_rows=None):
         """The moves that evict chose, in up to four tensors [rows][kv heads][dim] or [rows][kv heads] of any types at once, by any
-        strides of rows and heads: keys, values, their weights and places. Rows move in place, all moves at once."""
+        strides of rows and heads: keys, values, their weights and places. Rows move in place, all moves at once; sequences may
+        not share rows."""
         shape = moves.shape
         if len(shape) != 4 or shape[3] != 2 or not 1 <= len(tensors) <= 4:
             raise ValueError("moves [sequences][kv heads][most][2], and one to four tensors")
