@@ -46,13 +46,15 @@ static int rows_of(const CacheRef& c, int64_t seqs, int64_t rows, Rows* r) {
 // A key's worth is a word of 64 bits, no two alike: the weight's bits in their order (protected keys above all), then the key's
 // number from the top down. Kept are the keys from the keep-th largest word on. That word is found by its digits from the top: the
 // words with the digits found so far are counted by their next one, 11 bits, in 2048 bins in LDS, until the bin that the last kept
-// word is in is kept whole or holds few enough to rank each against all. Weights spread over orders of magnitude take one digit.
+// word is in is kept whole or holds few enough to rank each against all. Weights spread over orders of magnitude take one digit
+// or two.
 //
 // What bounds it are latencies: the loads of pages, weights and places, the counting's atomics, the barriers between. 528 keys x 12
-// heads 5.7 us; 48 caches of 4160 keys x 8 heads 18; 65536 keys x 8 heads 31 in three launches. Three digits of every word in place of
-// one and a ranking: 12, 32 and 168.
-constexpr int WAVES = 16, THREADS = 64 * WAVES, BINS = 2048, RANKED = 1024;
-constexpr int SLICES = 16, GATHERED = 8192, LONG = 16384;
+// heads 5.3 us; 48 caches of 4160 keys x 8 heads 17; 65536 keys x 8 heads 31 in three launches. Three digits of every word in place of
+// one and a ranking: 12, 32 and 168. Ranking up to 1024 words, 700 of them with as many: 32768 -> 8192 keys x 8 heads with the moves
+// 69 us, 128 and fewer 37; up to 64: 48 caches of 4160 keys 27 us, so 23.
+constexpr int WAVES = 16, THREADS = 64 * WAVES, BINS = 2048, RANKED = 128;
+constexpr int SLICES = 16, PAIRS = 128, GATHERED = 8192, LONG = 16384;
 
 struct Choice {
     HeadsRef weights, places;
@@ -60,7 +62,7 @@ struct Choice {
     const int32_t *k_len, *next_place;
     int32_t *moves, *count, *kept_len;
     char* work;
-    int32_t seqs, keep, recent, first, most;
+    int32_t seqs, keep, recent, first, most, slices;
 };
 
 // a float's bits in an order of unsigned words: NaN 0, -infinity above it, +0 and -0 alike; +infinity is below PROTECTED
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(THREADS, E > 8 ? 4 : 8) evict_k(Choice A) {
 }
 
 // ------------------------------------------------------------------------------------------------ long caches
-// Few pairs of long runs: 16 workgroups to each, a slice of its keys each (no slice on both sides of `keep`), in three launches. The
+// Few pairs of long runs: 2 to 16 workgroups to each, a slice of its keys each (no slice on both sides of `keep`), in three launches. The
 // slices' counts of the first digit; the words of the bin that is kept in part, gathered (8192 at most: of more, a few weights shared
 // by thousands of keys, each workgroup goes through all words by itself); the smallest word kept, and the slices' moves.
 struct Pair {
@@ -273,12 +275,12 @@ static_assert(sizeof(Pair) % 8 == 0, "the gathered words stay aligned");
 struct Slice {
     int lo, hi, before;  // its keys; the slices on its side of `keep` begin with this one
 };
-__device__ __forceinline__ Slice slice_of(int s, int len, int keep) {
-    int left = (int)((int64_t)SLICES * keep / len);
-    left = left < 1 ? 1 : left > SLICES - 1 ? SLICES - 1 : left;
+__device__ __forceinline__ Slice slice_of(int s, int slices, int len, int keep) {
+    int left = (int)((int64_t)slices * keep / len);
+    left = left < 1 ? 1 : left > slices - 1 ? slices - 1 : left;
     const auto cut = [](int n, int i, int of) { return (int)((int64_t)n * i / of); };
     if (s < left) return {cut(keep, s, left), cut(keep, s + 1, left), 0};
-    const int n = len - keep, of = SLICES - left;
+    const int n = len - keep, of = slices - left;
     return {keep + cut(n, s - left, of), keep + cut(n, s - left + 1, of), left};
 }
 
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
         return;
     }
     Pair& P = ((Pair*)A.work)[pair];
-    const Slice mine = slice_of(s, len, A.keep);
+    const Slice mine = slice_of(s, A.slices, len, A.keep);
     Words<E, SMALL> W(A, g, b, len, at);
     const bool once = mine.hi - mine.lo <= W.CHUNK;
     if (once) W.load(mine.lo, mine.hi);
@@ -311,8 +313,9 @@ __global__ void __launch_bounds__(THREADS) evict_long_k(Choice A) {
         uint32_t x = 0, y = 0;
         uint2 own = make_uint2(0, 0);
 #pragma unroll
-        for (int i = 0; i < SLICES; ++i) {
-            const uint2 c = *(const uint2*)&P.hist[i][at2];
+        for (int i = 0; i < SLICES; ++i) {  // all asked for at once
+            uint2 c = *(const uint2*)&P.hist[i < A.slices ? i : 0][at2];
+            if (i >= A.slices) c = make_uint2(0, 0);
             x += c.y, y += c.x;
             if (i == s) own = c;
         }
@@ -450,7 +453,7 @@ template <bool SMALL>
 static int run(const Choice& c, int kv_heads, int max_k, bool shared, hipStream_t s) {
     const dim3 block(THREADS);
     if (shared) {
-        const dim3 grid(kv_heads, SLICES, c.seqs);
+        const dim3 grid(kv_heads, c.slices, c.seqs);
         hipLaunchKernelGGL((evict_long_k<0, SMALL>), grid, block, 0, s, c);
         if (int e = launch_rc()) return e;
         hipLaunchKernelGGL((evict_long_k<1, SMALL>), grid, block, 0, s, c);
@@ -471,9 +474,10 @@ static int run(const Choice& c, int kv_heads, int max_k, bool shared, hipStream_
     return launch_rc();
 }
 
-// Few pairs of long runs: their workgroups alone do not fill the chip, and one takes long (65536 -> 16384 keys x 8 heads with the
-// moves: a workgroup each 219 us, so 61).
-static bool is_long(const EvictArgs& a) { return a.max_k > LONG && (int64_t)a.seqs * a.kv_heads < 256; }
+// Few pairs of long runs, which a workgroup's registers do not hold: its own workgroups alone do not fill the chip. A workgroup each,
+// and so, with the moves (8 heads of 64): 16384 keys 24 and 33 us, 20000 57 and 34, 65536 123 and 45; 16 caches of 20000 keys 127 and
+// 113, 30 caches 198 and 210. 16 workgroups to each whatever the pairs: 8 caches of 16384 keys (128 dimensions) 157, a workgroup each 91.
+static bool is_long(const EvictArgs& a) { return a.max_k > LONG && (int64_t)a.seqs * a.kv_heads <= PAIRS; }
 static uint64_t work_bytes(const EvictArgs& a) { return PCX_ATTENTION_COUNTERS * 4 + (uint64_t)a.seqs * a.kv_heads * sizeof(Pair); }
 
 extern "C" uint64_t pcx_evict_workspace(const EvictArgs* a) {
@@ -498,6 +502,7 @@ extern "C" int pcx_evict(const EvictArgs* a, pc_stream_t s) {
     const bool small = a->rows < 0x3fffffff / std::max<int64_t>({1, c.weights.token, c.places.base ? c.places.token : 0});
     const bool shared = is_long(*a) && a->work && a->work_bytes >= work_bytes(*a);
     c.work = (char*)a->work + PCX_ATTENTION_COUNTERS * 4;
+    c.slices = shared ? std::min(SLICES, 2 * PAIRS / (a->seqs * a->kv_heads)) : 1;
     return small ? run<true>(c, a->kv_heads, a->max_k, shared, (hipStream_t)s) : run<false>(c, a->kv_heads, a->max_k, shared, (hipStream_t)s);
 }
 

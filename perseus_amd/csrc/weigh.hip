@@ -9,9 +9,10 @@
 // workgroup, the next tile asked for while this one is used; rows are split over workgroups and joined where the keys are few.
 // weigh_few_k (up to 32 rows): the rows stay in registers and the keys are streamed.
 //
-// 8192 tokens x 32/8 heads of 128, causal, f16: 309 us, 890 TFLOP/s (a 16384^3 product: 1280). Power bounds it: with queries or
-// keys of zeros, whose products switch nothing, the same instructions take 234 us. Without the exponentials 292, without the
-// products 149. One product after the other, then its exponentials: 329; deeper buffers, other interleavings, three waves a SIMD: within 2%.
+// 8192 tokens x 32/8 heads of 128, causal, f16: 295 to 309 us by the card, 930 to 890 TFLOP/s (a 16384^3 product: 1280). Power
+// bounds it: with queries or keys of zeros, whose products switch nothing, the same instructions take 234 us. Without the
+// exponentials 292, without the products 149. One product after the other, then its exponentials: 329; deeper buffers, other
+// interleavings, three waves a SIMD: within 2%.
 #include <algorithm>
 
 #include "tiles.h"

@@ -206,6 +206,14 @@ def test_key_weights_refusals(bad, cache, rc):
     assert LIB.pcx_key_weights(None, None) == -1 and LIB.pcx_key_weights_workspace(None) == 0
 
 
+def test_evict_s_workspace():
+    """none for runs of up to 16384 keys, nor for more than 128 (sequence, key head) pairs; a share for each pair else"""
+    size = lambda **kw: LIB.pcx_evict_workspace(C.byref(evict_args(**kw)))  # noqa: E731
+    assert size(max_k=16384) == size(max_k=20000, seqs=43, kv_heads=3) == size(max_k=20000, seqs=0) == 0
+    one, all = size(max_k=16385, seqs=1, kv_heads=1) - 4 * 4096, size(max_k=20000, seqs=64, kv_heads=2) - 4 * 4096
+    assert one > 0 and all == 128 * one and LIB.pcx_evict_workspace(None) == 0
+
+
 def test_key_weights_s_workspace():
     """none for a token; the parts' sums for a prompt, whatever work says"""
     assert LIB.pcx_key_weights_workspace(C.byref(weights_args(max_q=1))) == 0

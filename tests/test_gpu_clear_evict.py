@@ -302,3 +302,21 @@ def test_evict_of_long_caches_replays_as_a_graph(ops):
         load(i)
         graph.launch(st)
         assert (moves.numpy(st) == eager[i][0]).all() and (count.numpy(st) == eager[i][1]).all()
+
+
+@pytest.mark.parametrize("seqs", [6, 9, 20, 42, 43])
+def test_evict_of_long_caches_by_fewer_workgroups(ops, seqs):
+    """3 heads of 6 to 42 sequences: from 14 slices of a cache down to 2; of 43, none"""
+    say(f"[clear] evict of {seqs} sequences, one of 17000 keys")
+    rng = np.random.default_rng(seqs)
+    lens = [17000] + [int(n) for n in rng.integers(0, 600, seqs - 1)]
+    run_evict(ops, lens, 3, 200, 20, 4, 16, spread)
+    run_evict(ops, lens[1:], 3, 200, 20, 4, 0, spread, max_k=16385)
+
+
+@pytest.mark.parametrize("n", [127, 128, 129, 130, 300, 17000])
+def test_evict_of_weights_within_a_quarter_of_an_octave(ops, n):
+    """one first digit for all: as many to be ranked as there is room for, one fewer and more"""
+    say(f"[clear] evict of {n} weights of one first digit")
+    for keep in (1, n // 2, n - 1):
+        run_evict(ops, [n], 2, keep, 0, 0, 16, lambda rng, m: 1 + 0.249 * rng.random(m))
