@@ -562,7 +562,12 @@ static int checked(const KeyWeightsArgs* a, Weigh* w) {
 }
 
 // How the rows are split: into workgroups for two a CU if they have a tile each, and up to 2048 where they have four tiles and more
-// (8192 tokens x 32 heads: 1024 workgroups 329 us, 2048 317, 4096 323, 8192 354). A workspace that is too small makes fewer.
+// (8192 tokens x 32 heads: 1024 workgroups 329 us, 2048 317, 4096 323, 8192 354; as many parts of late keys, which few queries see,
+// as leave all alike long: 351, a third round of them at its end). Where most queries see all keys of the one sequence, workgroups
+// are alike by themselves, and two a CU are enough if they come out at that (4096 tokens x 32/8 heads, not causal: 2048 workgroups
+// 142 us, 512 132; 2500 x 16/2 of 256 over 3200 131 and 85; 2048 queries x 16/4 heads over 32048 keys 262 and 252; but 384 of 1200
+// queries over 12200 keys 87, where 768 take 79, and 8 sequences of up to 2000 keys 81, where it is 66). A workspace that is too
+// small makes fewer.
 static uint64_t bytes_of(const Weigh& w, int parts) {
     return parts > 1 ? PCX_ATTENTION_COUNTERS * 4 + (uint64_t)parts * w.seqs * w.kv_heads * w.max_k * 4 : 0;
 }
@@ -571,7 +576,9 @@ static void choose(Weigh* w, int max_q, uint64_t room) {
     const int64_t keys = std::max<int64_t>(1, ((int64_t)w->max_k + BK - 1) / BK), most = std::max<int64_t>(1, std::min<int64_t>(65535, (1 << 20) / ((int64_t)w->seqs * w->kv_heads)));
     w->slots = (int)std::min(keys, most);
     const int64_t base = (int64_t)w->slots * w->seqs * w->kv_heads;
-    w->parts = (int)std::max<int64_t>({1, std::min<int64_t>(512 / base, tiles), std::min<int64_t>(2048 / base, tiles / 4)});
+    const bool alike = w->seqs == 1 && (!w->causal || w->max_k / 4 >= max_q) && base <= 512 && 512 % base <= 64;
+    const int64_t most_of = std::min<int64_t>((alike ? 512 : 2048) / base, tiles / 4);
+    w->parts = (int)std::max<int64_t>({1, std::min<int64_t>(512 / base, tiles), most_of});
     if (!w->max_k) w->parts = 1;  // no key is expected: there is nothing to join, and longer runs than expected are not split
     while (w->parts > 1 && (bytes_of(*w, w->parts) > room || w->slots * w->parts > 65535)) w->parts /= 2;
 }

@@ -328,3 +328,12 @@ def test_key_weights_of_keys_at_minus_infinity(ops, dim, causal):
         for page in (0, 16):
             got = run_weights(ops, "f16", dim, heads, kv, spans, causal, page, edit=edit)
             assert not np.isnan(got).any()
+
+
+@pytest.mark.parametrize("dim,heads,kv,spans,causal", [(128, 16, 2, [(600, 900)], False), (64, 4, 4, [(2500, 500)], False),
+                                                       (256, 8, 1, [(300, 1300)], True)])
+def test_key_weights_of_rows_alike(ops, dim, heads, kv, spans, causal):
+    """one sequence most of whose keys all queries see: workgroups alike, two a CU"""
+    say(f"[clear] key_weights {dim} dimensions {heads}/{kv} heads, {spans}, causal {causal}")
+    run_weights(ops, "bf16", dim, heads, kv, spans, causal, 16, hints=(spans[0][0], spans[0][1]))
+    run_weights(ops, "f16", dim, heads, kv, spans, causal, 0, new=True)
