@@ -273,7 +273,10 @@ __global__ void __launch_bounds__(256, 2) weigh_k(Weigh A) {
             __builtin_amdgcn_sched_barrier(0);
             v4f m0[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m0[i] = *(const v4f*)&nl[buf][64 * rb + 8 * i + 4 * h], m1[i] = *(const v4f*)&nl[buf][64 * rb + 32 + 8 * i + 4 * h];
+            for (int i = 0; i < 4; ++i) {
+                m0[i] = *(const v4f*)&nl[buf][64 * rb + 8 * i + 4 * h];
+                m1[i] = *(const v4f*)&nl[buf][64 * rb + 32 + 8 * i + 4 * h];
+            }
             products(buf, 2 * rb + 1, z1);
             weights(z0, m0);
             __builtin_amdgcn_sched_barrier(0);
@@ -557,7 +560,8 @@ static int checked(const KeyWeightsArgs* a, Weigh* w) {
     w->qt = BR / w->hb;
     w->blocks = (w->group + BR - 1) / BR;
     // a tile's offsets: below 2^30 bytes
-    if (w->k.token > 1 << 22 || (!w->k_start && (w->k.token << w->pages.log) > PAGE_MAX) || w->q.token > (1 << 28) / w->qt || w->q.head > (1 << 28) / w->hb) return -2;
+    if (w->k.token > 1 << 22 || (!w->k_start && (w->k.token << w->pages.log) > PAGE_MAX)) return -2;
+    if (w->q.token > (1 << 28) / w->qt || w->q.head > (1 << 28) / w->hb) return -2;
     return 0;
 }
 
@@ -573,7 +577,8 @@ static uint64_t bytes_of(const Weigh& w, int parts) {
 }
 static void choose(Weigh* w, int max_q, uint64_t room) {
     const int64_t tiles = ((int64_t)max_q + w->qt - 1) / w->qt * w->blocks;
-    const int64_t keys = std::max<int64_t>(1, ((int64_t)w->max_k + BK - 1) / BK), most = std::max<int64_t>(1, std::min<int64_t>(65535, (1 << 20) / ((int64_t)w->seqs * w->kv_heads)));
+    const int64_t keys = std::max<int64_t>(1, ((int64_t)w->max_k + BK - 1) / BK), pairs = (int64_t)w->seqs * w->kv_heads;
+    const int64_t most = std::max<int64_t>(1, std::min<int64_t>(65535, (1 << 20) / pairs));
     w->slots = (int)std::min(keys, most);
     const int64_t base = (int64_t)w->slots * w->seqs * w->kv_heads;
     const bool alike = w->seqs == 1 && (!w->causal || w->max_k / 4 >= max_q) && base <= 512 && 512 % base <= 64;
