@@ -1,4 +1,4 @@
-// Shared by the clear side's kernels (rotary.hip, attend.hip): the value types, conversions, argument checks.
+// Shared by the clear side's kernels (rotary.hip, attend.h, weigh.hip, evict.hip): the value types, conversions, argument checks.
 #pragma once
 #include "common.h"
 

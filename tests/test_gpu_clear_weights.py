@@ -337,3 +337,67 @@ def test_key_weights_of_rows_alike(ops, dim, heads, kv, spans, causal):
     say(f"[clear] key_weights {dim} dimensions {heads}/{kv} heads, {spans}, causal {causal}")
     run_weights(ops, "bf16", dim, heads, kv, spans, causal, 16, hints=(spans[0][0], spans[0][1]))
     run_weights(ops, "f16", dim, heads, kv, spans, causal, 0, new=True)
+
+
+def test_key_weights_offsets_past_32_bits(ops):
+    """keys past 2^32 bytes and 2^31 values of a pool, in its pages and in one run"""
+    say("[clear] key_weights far into a pool of 5.4 GB")
+    rows, kv, dim, n, H = 2_600_000, 8, 128, 200, 16
+    rng = np.random.default_rng(4)
+    k = co.rounded(rng.normal(size=(n, kv, dim)), "bf16")
+    first = rows // 16 - 13  # the last 13 pages
+    table = np.arange(first + 12, first - 1, -1).astype(np.int32)[None]
+    shuffled = np.concatenate([np.arange(16 * p, 16 * p + 16) for p in range(12, -1, -1)])[:n]
+    buf = pa.DevBuf(rows * kv * dim // 2)
+    pool = pa.Array((rows, kv, dim), "bf16", buf)
+    weights = pa.Array((rows, kv), "f32", strides=(1, rows))
+    for order, where in ((shuffled, dict(pages=pa.Array.of(table), page_rows=16)),
+                         (np.arange(n), dict(k_start=pa.Array.of(np.array([first * 16], np.int64))))):
+        tail = np.full((13 * 16, kv, dim), np.nan, np.float32)
+        tail[order] = k
+        buf.upload(clear.to_bf16(tail).view(np.uint32), offset=first * 16 * kv * dim // 2)
+        for queries in (1, 90):
+            q = co.rounded(rng.normal(size=(queries, H, dim)), "bf16")
+            runs = [(0, queries, 0, n)]
+            lse = true_lse(q, k, runs, H // kv, dim ** -0.5, True)
+            ops.key_weights(pa.Array.of(q, "bf16"), pool, pa.Array.of(lse), pa.Array.of(np.array([0, queries]), "i32"),
+                            pa.Array.of(np.array([n]), "i32"), weights, max_k=n, **where)
+            want, bound = co.key_weights(q, k, lse, runs, H // kv, dim ** -0.5, True)
+            got = weights.numpy(ops.stream)[first * 16:][order]
+            co.check(got, want, bound + 4 * co.E * np.abs(want) + 2.0 ** -140, f"{queries} queries")
+
+
+def test_calls_of_two_streams_at_once():
+    """split weights and the choice of a long cache on two streams, each with a Clear of its own: what each gives alone"""
+    say("[clear] key_weights and evict on two streams at once")
+    H, KV, D, n, m = 8, 2, 64, 700, 20000
+    sides = []
+    for seed in (1, 2):
+        rng = np.random.default_rng(seed)
+        c = pa.Clear(pa.Stream())
+        args = [pa.Array.of(rng.normal(size=(n, H, D)), "bf16"), pa.Array.of(rng.normal(size=(n, KV, D)), "bf16"),
+                pa.Array.of((rng.random((n, H)) + 6).astype(np.float32)), pa.Array.of(np.array([0, n]), "i32"),
+                pa.Array.of(np.array([n]), "i32"), pa.Array((n, KV), "f32")]
+        long = [pa.Array.of(rng.random((m, KV)).astype(np.float32)), pa.Array.of(np.array([m]), "i32"), 5000,
+                pa.Array.of(np.zeros((1, KV, 5000, 2), np.int32)), pa.Array.of(np.zeros((1, KV), np.int32))]
+        k0 = pa.Array.of(np.zeros(1, np.int64))
+        sides.append((c, args, long, k0))
+
+    def call(side):
+        c, args, long, k0 = side
+        c.key_weights(*args, k_start=k0)
+        c.evict(*long, k_start=k0)
+
+    def answers(side):
+        c, args, long, _ = side
+        return [x.numpy(c.stream) for x in (args[-1], *long[3:])]
+
+    alone = []
+    for side in sides:
+        call(side)
+        alone.append(answers(side))
+    for _ in range(20):
+        for side in sides:
+            call(side)
+    for side, want in zip(sides, alone):
+        assert all(np.array_equal(x, y) for x, y in zip(answers(side), want))
