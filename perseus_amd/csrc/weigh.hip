@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
                 v8 q[STEPS];
 #pragma unroll
                 for (int s = 0; s < STEPS; ++s) q[s] = (v8)(T)0.0f;
-                if (R > 0) {  // (rows past the last are the first again: of zeros, an infinity in a key would make a NaN)
+                if (R > 0) {  // (rows past the last are the first again, whose scores are no NaN where the first's are none)
                     const T* x = at<T>(A.q, S.q0 + (int64_t)i, head);
 #pragma unroll
                     for (int s = 0; s < STEPS; ++s) q[s] = *(const v8*)(x + std::min(16 * s + 8 * h, A.dim - 8));
@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
                 const float decay = begin ? A.decay : 1.0f;
                 const float* const from = (const float*)(given ? A.before.base : A.weights.base) + g * (given ? A.before.head : A.weights.head);
                 const int64_t step = given ? A.before.token : A.weights.token;
-                // the keys that every row sees
-                const int64_t whole = A.causal && S.n > 1 ? (int64_t)S.len - S.n + 1 + (A.group == 1 ? r0 : r0 / A.group) : (int64_t)S.len + KT;
+                // the keys that every row sees; of no row none, as zeros times an infinity in a key would make a NaN
+                const int64_t whole = R < 1 ? 0 : A.causal && S.n > 1 ? (int64_t)S.len - S.n + 1 + (A.group == 1 ? r0 : r0 / A.group) : (int64_t)S.len + KT;
                 settled();
                 int buf = 0;
                 for (int t0 = first; t0 < last; t0 += WINDOW) {
