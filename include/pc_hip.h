@@ -1199,7 +1199,7 @@ uint64_t pcx_attention_workspace(const AttentionArgs* args);
 /* Where the keys of a sequence lie in a cache of rows (an operator's kv_rows or rows of them): key j of sequence b at row
  * start[b] + j, or, where start is NULL, in pages: at row pages[b pages_seq + j / page_rows] page_rows + j mod page_rows.
  * page_rows: a power of two, 16 or more; the pool has its rows' whole pages, a sequence at most `width` of them; pages may lie
- * in any order. Table entries are read up to the page of a sequence's last key. */
+ * in any order. Table entries are read up to the page of a sequence's last key (pcx_move_rows: those of the rows that moves name). */
 typedef struct CacheRef {
     const int64_t* start; /* [seqs] */
     const int32_t* pages; /* [seqs][width] */

@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(64 * NW, DC > 192 ? 1 : 2) rows_k(AttentionArg
     // PAGED: the pages of the tile whose keys are asked for next, and of the one whose values are (the tile after it)
     Runs<NL, NW, CPR> pk, pv;
     page_t* const table = PAGED ? (page_t*)uniform64((uint64_t)(P.table + w.seq * P.seq)) : nullptr;
-    const auto fetch = [&](Runs<NL, NW, CPR>& r, int t) { r.template fetch<KT>(P, table, t > first ? t : first, wave); };
+    const auto fetch = [&](Runs<NL, NW, CPR>& r, int t) { r.template fetch<KT>(P, table, w.len, t > first ? t : first, wave); };
     const auto load_k = [&](int t, const Runs<NL, NW, CPR>& r) {
         if (t < first) return;
         if constexpr (PAGED)
@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     const auto load_v = [&](int t) {
         if constexpr (PAGED) {
             pages.template load<KT, 1024>(P, vp, (uint32_t)A.v.token * 2, A.dim, w.len, t, 0, base + TB, vo);
-            if (t >= first + NW) pages.template fetch<KT>(P, table, t - NW, 0);
+            if (t >= first + NW) pages.template fetch<KT>(P, table, w.len, t - NW, 0);
         } else {
             load(vp, A.v.token, t, base + TB, vo);
         }
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(64 * NW) few_k(AttentionArgs A, Split S, Group
     // this wave's tiles, from the last of those that are `wave` mod NW after the first
     const int mine = tiles - first > wave ? (tiles - first - wave + NW - 1) / NW : 0;
     if (mine) {
-        if constexpr (PAGED) pages.template fetch<KT>(P, table, first + wave + (mine - 1) * NW, 0);
+        if constexpr (PAGED) pages.template fetch<KT>(P, table, w.len, first + wave + (mine - 1) * NW, 0);
         load_k(first + wave + (mine - 1) * NW);
         load_v(first + wave + (mine - 1) * NW);
     }

@@ -1,6 +1,7 @@
 // What the clear side's matrix kernels share (attend.h, weigh.hip): the 32 x 32 products, tiles in LDS and their loads.
 #pragma once
 #include "clear.h"
+#include "pages.h"
 
 namespace pch {
 namespace clear {
@@ -134,7 +135,6 @@ __device__ __forceinline__ void settled() { __builtin_amdgcn_s_waitcnt(0x0f70); 
 // makes while the wave works on the tile before, and the lanes' offsets are within the run. Page numbers are read by scalar loads
 // a tile ahead, so that no tile waits for its table. A run past the sequence's end, or on a page that the pool does not have, is
 // an empty buffer: it reads as zeros.
-constexpr int RUN = 16;
 constexpr int64_t PAGE_MAX = 0x7fffffff;  // elements from a page to the next
 typedef const int32_t __attribute__((address_space(4))) page_t;
 
@@ -147,12 +147,11 @@ struct Runs {
     int page[E];
     // the tile's run that the wave's loads e N .. e N + N - 1 take
     static __device__ __forceinline__ int run(int e, int wave) { return (e * N * NW + wave) * PER / RUN; }
-    // page numbers; a tile begins at a page or lies in one
+    // page numbers of tile t, which may be past the last of the sequence's len keys
     template <int KT>
-    __device__ __forceinline__ void fetch(const PagesRef& P, page_t* table, int t, int wave) {
-        const uint32_t first = ((uint32_t)t * KT) >> P.log;
+    __device__ __forceinline__ void fetch(const PagesRef& P, page_t* table, int len, int t, int wave) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) page[e] = table[min(first + ((uint32_t)(run(e, wave) * RUN) >> P.log), (uint32_t)P.width - 1)];
+        for (int e = 0; e < E; ++e) page[e] = table[entry_of<KT>(t, run(e, wave) * RUN, P.log, len)];
     }
     // The scalar unit's instructions are in the way of the wave's others, so they are few for each run: what the tile alone decides
     // is made once (6 chunks of up to 512 queries over up to 6000 keys 169 -> 156 us; over one run of rows 128, the same for pages of

@@ -418,9 +418,9 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
             // 32 rows, query * group + head of the group; more only where more queries came than were expected: each 32 add to the last's
             const int64_t all = (int64_t)S.n * A.group;
             for (int64_t r0 = 0; r0 == 0 || r0 < all; r0 += 32) {
-                if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, first, 0);
+                if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, S.len, first, 0);
                 load(first, 0);
-                if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, first + 1, 0);
+                if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, S.len, first + 1, 0);
                 const int R = all - r0 < 32 ? (int)(all - r0) : 32;
                 const uint32_t r = (uint32_t)r0 + (c < R ? c : 0), i = A.group == 1 ? r : r / (uint32_t)A.group;
                 const int64_t head = (int64_t)g * A.group + (r - i * A.group);
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(64 * NW) weigh_few_k(Weigh A) {
                     for (int t = t0; t < t1; ++t, buf ^= 1) {
                         if (t + 1 < last) {
                             load(t + 1, buf ^ 1);
-                            if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, t + 2, 0);
+                            if constexpr (PAGED) pages.template fetch<KT>(A.pages, table, S.len, t + 2, 0);
                             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NL) : "memory");
                         } else {
                             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
