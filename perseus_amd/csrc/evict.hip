@@ -152,7 +152,8 @@ struct Words {
 
     __device__ __forceinline__ Words(const Choice& a, int g, int b, int len, int64_t at)
         : A(a), g(g), len(len), at(at), next(a.next_place ? a.next_place[b] : len), from(0), seg(0) {}
-    __device__ __forceinline__ int first() const { return from + (int)(threadIdx.x >> 6) * seg + (int)(threadIdx.x & 63); }
+    // this lane's first key (unsigned: past a run's last key a chunk has room for some beyond 2^31)
+    __device__ __forceinline__ uint32_t first() const { return (uint32_t)from + (threadIdx.x >> 6) * (uint32_t)seg + (threadIdx.x & 63); }
     // The chunk of keys lo .. hi - 1, E loads of each kind on their way at once; those past the end read the last key again (loads under
     // a condition each: 48 caches of 4160 keys 25.6 us, so 23.7). SMALL: rows and their offsets in 32 bits.
     __device__ __forceinline__ void load(int lo, int hi) {
@@ -168,7 +169,7 @@ struct Words {
         if (lo >= hi) return;  // a slice of no key: there is no last one to read again
         int page[E], place[E];
         float x[E];
-        const auto key_of = [&](int e) { return (uint32_t)std::min(first() + e * 64, hi - 1); };
+        const auto key_of = [&](int e) { return std::min(first() + e * 64, (uint32_t)hi - 1); };
         if (paged)
 #pragma unroll
             for (int e = 0; e < E; ++e) page[e] = table[key_of(e) >> A.cache.p.log];
@@ -195,8 +196,8 @@ struct Words {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             if (e * 64 >= seg) break;
-            const int j = first() + e * 64;
-            f(e, j, word(key[e], j), j < hi);
+            const uint32_t j = first() + e * 64;
+            f(e, j, word(key[e], j), j < (uint32_t)hi);
         }
     }
     // f(word) for the keys lo .. hi - 1; loaded: they are in registers
@@ -205,7 +206,7 @@ struct Words {
         for (int c = lo; c < hi; c += std::min(CHUNK, hi - c)) {
             const int end = c + std::min(CHUNK, hi - c);
             if (!loaded) load(c, end);
-            each(end, [&](int, int, uint64_t w, bool in) {
+            each(end, [&](int, uint32_t, uint64_t w, bool in) {
                 if (in) f(w);
             });
         }
@@ -214,20 +215,21 @@ struct Words {
     // `keep`), added to.
     __device__ __forceinline__ void emit(Shared& S, int lo, int hi, bool loaded, uint64_t least, int32_t* moves, uint32_t& movers, uint32_t& holes) {
         const uint64_t below = ((uint64_t)1 << (threadIdx.x & 63)) - 1;
+        const uint32_t keep = A.keep;
         for (int c = lo; c < hi; c += std::min(CHUNK, hi - c)) {
             const int end = c + std::min(CHUNK, hi - c);
             if (!loaded) load(c, end);
             uint32_t m = 0, h = 0, all_m, all_h;
-            each(end, [&](int, int j, uint64_t w, bool in) {
-                m += __popcll(__ballot(in && w >= least && j >= A.keep));
-                h += __popcll(__ballot(in && w < least && j < A.keep));
+            each(end, [&](int, uint32_t j, uint64_t w, bool in) {
+                m += __popcll(__ballot(in && w >= least && j >= keep));
+                h += __popcll(__ballot(in && w < least && j < keep));
             });
             m = movers + waves_before(S.sums[0], m, &all_m);
             h = holes + waves_before(S.sums[1], h, &all_h);
             movers += all_m;
             holes += all_h;
-            each(end, [&](int, int j, uint64_t w, bool in) {
-                const bool mover = in && w >= least && j >= A.keep, hole = in && w < least && j < A.keep;
+            each(end, [&](int, uint32_t j, uint64_t w, bool in) {
+                const bool mover = in && w >= least && j >= keep, hole = in && w < least && j < keep;
                 const uint64_t ms = __ballot(mover), hs = __ballot(hole);
                 const uint32_t to = m + __popcll(ms & below), gap = h + __popcll(hs & below);
                 if (mover && to < (uint32_t)A.most) moves[2 * (int64_t)to] = j;

@@ -1,5 +1,5 @@
-"""The cache's operators at the edges of what their header allows: sequences without queries beside keys that hold infinities and NaN.
-Each test prints its case before the GPU runs."""
+"""The cache's operators at the edges of what their header allows: sequences without queries beside keys that hold infinities and NaN,
+runs of as many keys as there are numbers. Each test prints its case before the GPU runs."""
 import sys
 
 import numpy as np
@@ -41,3 +41,25 @@ def test_key_weights_of_sequences_without_queries(ops, kind, page_rows, dim, hea
                 got = run_weights(ops, kind, dim, heads, kv, spans, causal, page_rows, hints=hints, edit=edit)
                 assert np.isfinite(got).all()
                 run_weights(ops, kind, dim, heads, kv, spans, causal, page_rows, hints=hints, edit=edit, inplace=True, new=True)
+
+
+@pytest.mark.parametrize("sliced", [True, False])
+def test_evict_of_as_many_keys_as_there_are_numbers(sliced):
+    """2^31 - 1 keys, the most of a run: pages of one pool again and again, weights above all others in two of them, the last key's
+    among them; in slices, and by one workgroup that expects few keys"""
+    say(f"[clear] evict of 2^31 - 1 keys, in slices: {sliced}")
+    ops = pa.Clear(pa.Stream(), workspace=64 << 20 if sliced else 0)
+    page, pool, n, keep, high = 1 << 20, 8, 2 ** 31 - 1, 1500, 1000
+    rng = np.random.default_rng(3)
+    w = rng.random((pool, page), np.float32)
+    w[-1, -high:] = 10 + rng.permutation(high) / np.float32(high)  # on the pool's last page: no two alike
+    table = (np.arange(2048) % (pool - 1)).astype(np.int32)
+    table[[5, 2047]] = pool - 1
+    moves, count, kept = pa.Array.of(np.full((1, 1, keep, 2), -9, np.int32)), pa.Array.of(np.zeros((1, 1), np.int32)), pa.Array.of(np.zeros(1, np.int32))
+    ops.evict(pa.Array.of(w.reshape(-1, 1)), pa.Array.of(np.array([n]), "i32"), keep, moves, count, pages=pa.Array.of(table[None]),
+              page_rows=page, kept_len=kept, max_k=n if sliced else 5000)
+    j = np.concatenate([e * page + np.arange(page - high, page) for e in (5, 2047)])[:-1]  # the last row has no key
+    stay = np.sort(j[np.lexsort((j, -w[-1, j % page]))[:keep]])
+    got = moves.numpy(ops.stream)[0, 0]
+    assert count.numpy(ops.stream)[0, 0] == keep == kept.numpy(ops.stream)[0]
+    assert (got[:, 0] == stay).all() and (got[:, 1] == np.arange(keep)).all()
