@@ -197,6 +197,8 @@ class PagedBlock:
             raise ValueError("sequences, pages, tokens and keep: one or more; recent and first at most keep together; decay 0 or more")
         if page_rows < 16 or page_rows & (page_rows - 1):
             raise ValueError(f"page_rows {page_rows}: a power of two, 16 or more")
+        if decay > 3.4e38 or max(seqs, kv_heads) > 65535 or kv_heads * dim > 1 << 22 or page_rows * kv_heads * dim >= 1 << 31:
+            raise ValueError("decay: finite in 32 bits; up to 65535 sequences and key heads, 2^22 values a row of keys, below 2^31 a page")
         self.ops, self.heads, self.kv_heads, self.dim, self.page_rows = ops, heads, kv_heads, dim, page_rows
         self.keep, self.recent, self.first, self.decay, self.tokens = keep, recent, first, decay, tokens
         self.table, self.layout, self.q_weight, self.k_weight, self.eps = table, layout, q_weight, k_weight, eps
