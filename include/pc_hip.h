@@ -1224,11 +1224,11 @@ uint64_t pcx_attention_paged_workspace(const AttentionPagedArgs* args); /* as pc
  * rows as CacheRef says,
  *     weights[row(j)][g] = decay before[row(j)][g] + sum exp(scale q . k_j - lse)
  * over the queries that see j and the query heads of g. lse: what the attention of the same queries gave (f32
- * [tokens][heads]); a query of -infinity, which sees no key, adds nothing. before (base NULL, or decay 0: not read, 0) may be
- * weights itself. next_place (NULL: none): the last n_b keys of each sequence are its n_b queries' own and new: before is not
- * read for them, and where places (base NULL: none) is given, theirs become next_place[b] - len + j (next_place[b]: the
- * place after the sequence's last token). Rows of no sequence are left as they were; sequences may not share rows. Sums are f32
- * and have one order.
+ * [tokens][heads]); a query of -infinity, which sees no key or whose scores are all -infinity, adds nothing. before (base NULL, or
+ * decay 0: not read, 0) may be weights itself. next_place (NULL: none): the last n_b keys of each sequence are its n_b queries' own
+ * and new: before is not read for them, and where places (base NULL: none) is given, theirs become next_place[b] - len + j
+ * (next_place[b]: the place after the sequence's last token). Rows of no sequence are left as they were; sequences may not share
+ * rows. Sums are f32 and have one order.
  *
  * weights, before: f32 [rows][kv_heads], places: i32, by any strides (token: of a row). Keys on a page outside the pool have
  * no row. Types, dim, scale and alignment as pcx_attention's; a query's row and head strides up to 2^21 elements, a key

@@ -184,8 +184,9 @@ class PagedBlock:
     in the sequence, which it is rotated by and keeps.
 
     `rows` are the block's projected rows of several sequences one after the other, an Array (or another library's device tensor)
-    [tokens][heads + 2 kv_heads][dim]: queries, then keys, then values. A call uploads where its tokens go and waits for that (so for
-    the stream's work before it); nothing is allocated after the constructor. tokens: the most of one call."""
+    [tokens][heads + 2 kv_heads][dim]: queries, then keys, then values. A call uploads where its tokens go, a plan of seqs x pages
+    words whatever it uses of them, and waits for that (so for the stream's work before it); nothing is allocated after the
+    constructor. tokens: the most of one call."""
 
     def __init__(self, ops, heads, kv_heads, dim, seqs, pages, page_rows=16, keep=TOKENS, recent=32, first=4, tokens=TOKENS,
                  dtype="bf16", table=None, layout="half", q_weight=None, k_weight=None, eps=1e-6, decay=1.0):
@@ -282,8 +283,9 @@ class PagedBlock:
 
     def evict(self):
         """Cuts each sequence longer than `keep` to that many keys; their pages go back to the pool. Returns the (moves, count) of
-        move_rows, for a copy of the cache elsewhere (encrypted keys, say) that is to be kept alike: row moves[b][g][i][0] of
-        sequence b and key head g went to row [i][1], i < count[b][g]; (None, None) where no sequence is longer."""
+        move_rows, for a copy of the cache elsewhere (on the host, say) that is to be kept alike: row moves[b][g][i][0] of
+        sequence b and key head g went to row [i][1], i < count[b][g]; (None, None) where no sequence is longer. Nothing here
+        moves the slots of an encrypted copy: that is made anew from keys()."""
         P, longest = self.page_rows, max(self.lengths)
         if longest <= self.keep:
             return None, None

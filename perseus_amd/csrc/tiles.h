@@ -154,8 +154,8 @@ struct Runs {
         for (int e = 0; e < E; ++e) page[e] = table[entry_of<KT>(t, run(e, wave) * RUN, P.log, len)];
     }
     // The scalar unit's instructions are in the way of the wave's others, so they are few for each run: what the tile alone decides
-    // is made once (6 chunks of up to 512 queries over up to 6000 keys 169 -> 156 us; over one run of rows 128, the same for pages of
-    // 16 to 1024 rows in any order). Nearer to it came neither one buffer for a tile of one page (165), nor one for the whole pool with a
+    // is made once (6 chunks of up to 512 queries over up to 6000 keys 169 -> 156 us; 161 where one run of rows takes 133, the same for
+    // pages of 16 to 1024 rows in any order). Nearer to it came neither one buffer for a tile of one page (165), nor one for the whole pool with a
     // run as the scalar offset (33% behind), nor page numbers through LDS (157): what is left is not the number of these instructions
     // but the scalar registers, whose spilling takes vector registers that the products' addresses had. token: a row's distance in
     // bytes; a page's bytes stay in 32 bits.

@@ -9,9 +9,10 @@
 // workgroup, the next tile asked for while this one is used; rows are split over workgroups and joined where the keys are few.
 // weigh_few_k (up to 32 rows): the rows stay in registers and the keys are streamed.
 //
-// 8192 tokens x 32/8 heads of 128, causal, f16: 295 to 309 us by the card, 930 to 890 TFLOP/s (a 16384^3 product: 1280). Power
-// bounds it: with queries or keys of zeros, whose products switch nothing, the same instructions take 234 us. Without the
-// exponentials 292, without the products 149. One product after the other, then its exponentials: 329; deeper buffers, other
+// 8192 tokens x 32/8 heads of 128, causal, f16: 295 to 314 us by the card, 930 to 880 TFLOP/s (a 16384^3 product: 1280). Power
+// takes a part of it: with queries or keys of zeros, whose products switch nothing, the same instructions take 234 us. Without the
+// exponentials 292, without the products 149; what else keeps the products from the large product's rate is not measured (a
+// 16-byte LDS reading serves two products here). One product after the other, then its exponentials: 329; deeper buffers, other
 // interleavings, three waves a SIMD: within 2%.
 #include <algorithm>
 
@@ -36,7 +37,7 @@ struct Weigh {
     int32_t slots, parts;           // workgroups of a sequence's keys, parts of their rows
     uint32_t per_hb;                // 2^16 / hb, rounded up
     float scale, decay;
-    // the query of a tile's row (below 64)
+    // the query of a tile's row (exact for every lane of a workgroup: below 256)
     __device__ __forceinline__ int query(int x) const { return (int)(((uint32_t)x * per_hb) >> 16); }
 };
 
